@@ -6,6 +6,9 @@ The compute path is a C-ABI CUDA library (``libflashbias_b200.so``, built in-tre
 """
 from .flash_bias import (FlashBiasAlibiFunc, FlashBiasFunc, check_device_status, flash_bias_alibi_func,
                          flash_bias_backward, flash_bias_forward, flash_bias_func)
+from .paged import PagedPlan, flash_bias_paged_func, paged_append, paged_plan
+from .rotary import norm_rope_func
 
 __all__ = ["FlashBiasFunc", "flash_bias_func", "flash_bias_forward", "flash_bias_backward",
-           "FlashBiasAlibiFunc", "flash_bias_alibi_func", "check_device_status"]
+           "FlashBiasAlibiFunc", "flash_bias_alibi_func", "check_device_status", "norm_rope_func",
+           "PagedPlan", "paged_plan", "paged_append", "flash_bias_paged_func"]

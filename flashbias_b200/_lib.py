@@ -12,7 +12,7 @@ import threading
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libflashbias_b200.so")
 
-FB_DTYPE_F16, FB_DTYPE_BF16, FB_DTYPE_F32 = 0, 1, 2
+FB_DTYPE_F16, FB_DTYPE_BF16, FB_DTYPE_F32, FB_DTYPE_F64 = 0, 1, 2, 3
 FB_MASK_NONE, FB_MASK_VECTOR, FB_MASK_MATRIX = 0, 1, 2
 FB_FLAG_FORCE_GENERAL = 1
 FB_FLAG_BWD_QUERY_MAJOR = 2
@@ -49,6 +49,55 @@ class FbParams(C.Structure):
     ]
 
 
+I64x2 = C.c_int64 * 2
+
+
+class FbRopeParams(C.Structure):
+    """Mirror of ``struct fb_rope_params``."""
+    _fields_ = [
+        *[(n, C.c_int32) for n in ("B", "S", "Hq", "Hk", "D", "dtype", "weight_dtype", "rot", "interleaved", "naxes",
+                                   "position_bits", "freq_dtype")],
+        ("eps", C.c_float), ("flags", C.c_int32), ("pair_axis", C.c_uint8 * 64),
+        *[(n, C.c_void_p) for n in ("q", "k", "q_weight", "k_weight", "positions", "inv_freq")],
+        *[(n, I64x3) for n in ("q_stride", "k_stride", "position_stride")],
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("q_out_stride", I64x3), ("k_out_stride", I64x3),
+        ("dq_out", C.c_void_p), ("dk_out", C.c_void_p), ("dq_out_stride", I64x3), ("dk_out_stride", I64x3),
+        *[(n, C.c_void_p) for n in ("dq", "dk", "dq_weight", "dk_weight")], ("dq_stride", I64x3), ("dk_stride", I64x3),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("v", C.c_void_p), ("k_bias", C.c_void_p), ("v_stride", I64x3), ("k_bias_stride", I64x3),
+        *[(n, C.c_void_p) for n in ("key_cache", "value_cache", "bias_cache")],
+        *[(n, I64x3) for n in ("key_cache_stride", "value_cache_stride", "bias_cache_stride")],
+        ("slots", C.c_void_p), ("slot_stride", C.c_int64), ("slot_bits", C.c_int32), ("page_size", C.c_int32),
+        ("num_pages", C.c_int64), ("R", C.c_int32), ("bias_heads", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
+class FbPlanParams(C.Structure):
+    """Mirror of ``struct fb_plan_params``."""
+    _fields_ = [
+        *[(n, C.c_int32) for n in ("B", "num_tokens", "page_size", "table_width", "stack_size", "mask_words")],
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+        *[(n, C.c_void_p) for n in ("pages_held", "free_pages", "free_count", "lens", "new_lens", "parents", "cu_tokens",
+                                    "lens_out", "positions", "slots", "tree_mask", "status")],
+    ]
+
+
+class FbPagedParams(C.Structure):
+    """Mirror of ``struct fb_paged_params``."""
+    _fields_ = [
+        *[(n, C.c_int32) for n in ("N", "B", "Hq", "Hk", "D", "R", "dtype", "page_size", "table_width", "mask_words",
+                                   "bias_heads", "flags")],
+        ("num_pages", C.c_int64), ("softmax_scale", C.c_float),
+        *[(n, C.c_void_p) for n in ("q", "q_bias", "key_cache", "value_cache", "bias_cache")],
+        ("q_stride", I64x2), ("q_bias_stride", I64x2),
+        *[(n, I64x3) for n in ("key_cache_stride", "value_cache_stride", "bias_cache_stride")],
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+        *[(n, C.c_void_p) for n in ("lens", "cu_tokens", "positions", "tree_mask")], ("mask_stride", C.c_int64),
+        ("slopes", C.c_void_p), ("o", C.c_void_p), ("o_stride", I64x2), ("lse", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+    ]
+
+
 EXPORTS = {
     "fb_version": (C.c_int, []),
     "fb_params_size": (C.c_size_t, []),
@@ -69,6 +118,16 @@ EXPORTS = {
     "fb_prepare_rows": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(C.c_int64), C.c_void_p, C.c_int32,
                                   C.POINTER(C.c_int64), C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                   C.c_void_p, C.c_float, C.c_void_p]),
+    "fb_rope_params_size": (C.c_size_t, []),
+    "fb_norm_rope": (C.c_int, [C.POINTER(FbRopeParams), C.c_void_p]),
+    "fb_norm_rope_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(FbRopeParams)]),
+    "fb_norm_rope_bwd": (C.c_int, [C.POINTER(FbRopeParams), C.c_void_p]),
+    "fb_paged_append": (C.c_int, [C.POINTER(FbRopeParams), C.c_void_p]),
+    "fb_plan_params_size": (C.c_size_t, []),
+    "fb_paged_plan": (C.c_int, [C.POINTER(FbPlanParams), C.c_void_p]),
+    "fb_paged_params_size": (C.c_size_t, []),
+    "fb_paged_workspace_bytes": (C.c_size_t, [C.POINTER(FbPagedParams)]),
+    "fb_paged_fwd": (C.c_int, [C.POINTER(FbPagedParams), C.c_void_p]),
     "fb_launch_count": (C.c_longlong, []),
     "fb_prof_begin": (C.c_int, [C.c_int]),
     "fb_prof_end": (C.c_int, [C.POINTER(C.c_float), C.POINTER(C.c_int)]),
@@ -97,8 +156,10 @@ def load() -> C.CDLL:
                 fn = getattr(lib, name)  # AttributeError if the symbol is not exported
                 fn.restype = res
                 fn.argtypes = args
-            if lib.fb_params_size() != C.sizeof(FbParams):
-                raise RuntimeError("fb_params layout mismatch between the Python binding and the built library")
+            for size, mirror in ((lib.fb_params_size, FbParams), (lib.fb_rope_params_size, FbRopeParams),
+                                 (lib.fb_plan_params_size, FbPlanParams), (lib.fb_paged_params_size, FbPagedParams)):
+                if size() != C.sizeof(mirror):
+                    raise RuntimeError(f"{size.__name__[:-5]} layout mismatch between the Python binding and the built library")
             _lib = lib
     return _lib
 

@@ -166,6 +166,8 @@ extern "C" const char* fb_strerror(int code) {
     case FB_ENOTBUILT: return "kernel variant not available in this build";
     case FB_EDEVICE: return "a kernel reported a device-side error";
     case FB_EINVAL_SIZE: return "problem needs more scratch than the fixed-capacity entry point holds";
+    case FB_EINVAL_ROPE: return "rotated columns, axes, frequencies or positions do not fit each other";
+    case FB_EINVAL_PAGE: return "page size, page count or table width not positive, or too many slots";
     default: return code > 0 ? cudaGetErrorString(static_cast<cudaError_t>(code)) : "unknown flashbias error";
   }
 }
@@ -175,6 +177,7 @@ extern "C" const char* fb_status_string(int32_t value) {
     case FB_DEV_OK: return "ok";
     case FB_DEV_WAIT_TIMEOUT: return "a bounded wait inside a kernel expired; the results of that call are invalid";
     case FB_DEV_FACTOR_OVERFLOW: return "a pre-scaled bias factor left the range of the 16-bit type";
+    case FB_DEV_BAD_INDEX: return "an index in device memory (page, slot, offset, parent, page count) is out of range; what it names was not accessed";
     default: return "unknown device status";
   }
 }

@@ -1,0 +1,171 @@
+// Attention of the newest tokens of every request over its pages: one token (decoding), several, or a tree of drafted ones.
+//
+//   logit = scale q.k + slope (pos_key - pos_token)  |  + q_bias . bias_cache;   o = softmax(logit) v, statistics in fp32
+//
+// Bound by reading K and V of every request once while there are few rows per key head, by the products beyond.
+#include <float.h>
+
+#include "fb_common.cuh"
+#include "fb_internal.h"
+
+namespace fb {
+
+constexpr float kLog2eP = 1.4426950408889634f;
+constexpr float kLn2P = 0.6931471805599453f;
+
+__device__ __forceinline__ void paged_bad_index(const fb_paged_params& p) {
+  if (p.status) *reinterpret_cast<volatile int32_t*>(p.status) = FB_DEV_BAD_INDEX;
+}
+
+// Offsets within [0, N], whatever the device array holds.
+__device__ __forceinline__ int cu_at(const fb_paged_params& p, int b) { return min(max(p.cu_tokens[b], 0), p.N); }
+
+// ---- general kernel: any head_dim up to 128, any strides; one block per (token, head), keys over its warps ---------
+template <typename T>
+__global__ void __launch_bounds__(128) paged_general_kernel(const __grid_constant__ fb_paged_params p) {
+  __shared__ float qs[128], qbs[256], s_acc[4][128], s_m[4], s_l[4];
+  const int n = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq, hk = h / (p.Hq / p.Hk);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int lo = 0, hi = p.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu_at(p, mid + 1) > n) hi = mid;
+    else lo = mid + 1;
+  }
+  const int first = cu_at(p, lo), end = cu_at(p, lo + 1), len = p.lens[lo], t = n - first;
+  const bool live = n >= first && n < end && len >= 0;
+  int64_t keys = live ? (int64_t)len + (end - first) : 0;
+  const int64_t room = (int64_t)p.table_width * p.page_size;
+  if (keys > room) {
+    if (threadIdx.x == 0) paged_bad_index(p);
+    keys = room;
+  }
+  const int my_pos = live ? (p.positions ? p.positions[n] : len + t) : 0;
+  const float slope = p.slopes ? p.slopes[h] : 0.f;
+  const int64_t* words = p.tree_mask ? p.tree_mask + n * p.mask_stride : nullptr;
+  const T* q = reinterpret_cast<const T*>(p.q) + n * p.q_stride[0] + h * p.q_stride[1];
+  for (int c = threadIdx.x; c < p.D; c += 128) qs[c] = to_f32(q[c]) * p.softmax_scale;
+  if (p.R) {
+    const T* qb = reinterpret_cast<const T*>(p.q_bias) + n * p.q_bias_stride[0] + h * p.q_bias_stride[1];
+    for (int c = threadIdx.x; c < p.R; c += 128) qbs[c] = to_f32(qb[c]);
+  }
+  __syncthreads();
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t j0 = warp * 32; j0 < keys; j0 += 128) {
+    const int64_t j = j0 + lane;
+    int page = -1, place = 0;
+    if (j < keys) {
+      const int col = (int)(j / p.page_size);
+      place = (int)(j - (int64_t)col * p.page_size);
+      page = p.block_table[lo * p.table_stride + col];
+      if (page < 0 || page >= p.num_pages) {
+        paged_bad_index(p);
+        page = -1;
+      }
+    }
+    const int td = (int)(j - len);
+    bool seen = page >= 0;
+    if (seen && td >= 0) seen = words ? (td >> 6) < p.mask_words && ((words[td >> 6] >> (td & 63)) & 1) : td <= t;
+    float s = -INFINITY;
+    if (seen) {
+      const T* k = reinterpret_cast<const T*>(p.key_cache) + page * p.key_cache_stride[0] + place * p.key_cache_stride[1] + hk * p.key_cache_stride[2];
+      s = 0.f;
+      for (int c = 0; c < p.D; ++c) s = fmaf(qs[c], to_f32(k[c]), s);
+      if (p.slopes) {
+        const int pos = td >= 0 && p.positions ? p.positions[first + td] : (int)j;
+        s = fmaf(slope, (float)(pos - my_pos), s);
+      }
+      if (p.R) {
+        const T* kb = reinterpret_cast<const T*>(p.bias_cache) + page * p.bias_cache_stride[0] + place * p.bias_cache_stride[1] +
+                      (p.bias_heads > 1 ? hk * p.bias_cache_stride[2] : 0);
+        for (int c = 0; c < p.R; ++c) s = fmaf(qbs[c], to_f32(kb[c]), s);
+      }
+      s *= kLog2eP;
+    }
+    float mx = s;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = fmaxf(m, mx);
+    const float msub = fmaxf(mx, -FLT_MAX), alpha = fast_exp2(m - msub);
+    m = mx;
+    const float e = seen ? fast_exp2(s - msub) : 0.f;
+    l = l * alpha + e;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= alpha;
+    for (uint32_t left = __ballot_sync(0xffffffffu, seen); left; left &= left - 1) {  // (what is not seen is not read)
+      const int src = __ffs(left) - 1;
+      const float pe = __shfl_sync(0xffffffffu, e, src);
+      const T* v = reinterpret_cast<const T*>(p.value_cache) + (int64_t)__shfl_sync(0xffffffffu, page, src) * p.value_cache_stride[0] +
+                   __shfl_sync(0xffffffffu, place, src) * p.value_cache_stride[1] + hk * p.value_cache_stride[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < p.D) acc[i] = fmaf(pe, to_f32(v[lane + 32 * i]), acc[i]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s_acc[warp][lane + 32 * i] = acc[i];
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float msub = fmaxf(m, -FLT_MAX);
+  l = 0.f;
+  float o = 0.f;
+  for (int w = 0; w < 4; ++w) {
+    const float f = fast_exp2(s_m[w] - msub);
+    l += s_l[w] * f;
+    o += s_acc[w][threadIdx.x] * f;
+  }
+  if (threadIdx.x < p.D)
+    reinterpret_cast<T*>(p.o)[n * p.o_stride[0] + h * p.o_stride[1] + threadIdx.x] = from_f32<T>(l > 0.f ? o / l : l == 0.f ? 0.f : l);
+  if (p.lse && threadIdx.x == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+static int validate_paged(const fb_paged_params* p) {
+  if (!p) return FB_EINVAL_NULL;
+  if (p->N <= 0 || p->B <= 0 || p->Hq <= 0 || p->Hk <= 0 || p->Hq % p->Hk || (int64_t)p->N * p->Hq > 0x7fffffffLL) return FB_EINVAL_SHAPE;
+  if (p->D <= 0 || p->D > 128 || p->R < 0 || p->R > 256) return FB_EINVAL_SHAPE;
+  if (p->dtype != FB_DTYPE_F16 && p->dtype != FB_DTYPE_BF16) return FB_EINVAL_DTYPE;
+  if (p->page_size <= 0 || p->table_width <= 0 || p->num_pages <= 0 || (int64_t)p->table_width * p->page_size > 0x7fffffffLL) return FB_EINVAL_PAGE;
+  if (!p->q || !p->key_cache || !p->value_cache || !p->block_table || !p->lens || !p->cu_tokens || !p->o) return FB_EINVAL_NULL;
+  if (p->R) {
+    if (!p->q_bias || !p->bias_cache || p->slopes || (p->bias_heads != 1 && p->bias_heads != p->Hk)) return FB_EINVAL_BIAS;
+  } else if (p->q_bias || p->bias_cache) {
+    return FB_EINVAL_BIAS;
+  }
+  if (p->tree_mask && (p->mask_words <= 0 || p->mask_stride < 0)) return FB_EINVAL_MASK;
+  if (p->table_stride < 0) return FB_EINVAL_STRIDE;
+  for (int i = 0; i < 3; ++i) {
+    if (p->key_cache_stride[i] < 0 || p->value_cache_stride[i] < 0 || p->bias_cache_stride[i] < 0) return FB_EINVAL_STRIDE;
+    if (i < 2 && (p->q_stride[i] < 0 || p->q_bias_stride[i] < 0 || p->o_stride[i] < 0)) return FB_EINVAL_STRIDE;
+  }
+  return 0;
+}
+
+}  // namespace fb
+
+using namespace fb;
+
+extern "C" size_t fb_paged_params_size(void) { return sizeof(fb_paged_params); }
+
+extern "C" size_t fb_paged_workspace_bytes(const fb_paged_params* p) {
+  if (validate_paged(p)) return 0;
+  return 0;
+}
+
+extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
+  if (const int rc = validate_paged(p)) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+  const unsigned grid = (unsigned)(p->N * p->Hq);
+  if (p->dtype == FB_DTYPE_F16) paged_general_kernel<__half><<<grid, 128, 0, st>>>(*p);
+  else paged_general_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(*p);
+  note_launch();
+  return (int)cudaGetLastError();
+}

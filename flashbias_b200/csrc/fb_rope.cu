@@ -1,0 +1,317 @@
+// Norm of queries and keys per head with the rotation by position in the same pass, forward and backward, and the serving
+// form that writes keys and values into the pages of a cache.
+//
+//   r = rsqrt(mean(x^2) + eps),  y = x r w,  (out_lo, out_hi) = (y_lo c - y_hi s, y_hi c + y_lo s)
+//   g = rotation of dout by the opposite angle,  dw = sum over rows of g x r,  dx = r (w g - x r^2 mean(w g x))
+//
+// Bound by reading x (and dout) once and writing the result once.  The angle position * inv_freq is taken in 64 bits and
+// reduced to a fraction of a turn before its sine and cosine are taken in 32: at position 1e6 a 32-bit product is off by up to
+// 0.03 rad.  It costs one pair of functions per token and frequency, shared by the token's heads, so no table is kept.
+#include "fb_common.cuh"
+#include "fb_internal.h"
+
+namespace fb {
+
+constexpr int kRopeWarps = 4;
+constexpr int kRopeThreads = 32 * kRopeWarps;
+constexpr int kRopeMaxD = 128;
+constexpr double kInv2Pi = 0.15915494309189533576888;
+
+__device__ __forceinline__ float load_scalar(const void* p, int dtype, int i) {
+  return dtype == FB_DTYPE_F32   ? reinterpret_cast<const float*>(p)[i]
+         : dtype == FB_DTYPE_F16 ? __half2float(reinterpret_cast<const __half*>(p)[i])
+                                 : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_scalar(void* p, int dtype, int i, float v) {
+  if (dtype == FB_DTYPE_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == FB_DTYPE_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+  else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// (cos, sin) of the angle of pair `pr` at token (b, s)
+__device__ __forceinline__ float2 rope_turn(const fb_rope_params& p, int b, int s, int pr) {
+  const int64_t at = p.pair_axis[pr] * p.position_stride[0] + b * p.position_stride[1] + s * p.position_stride[2];
+  const double pos = p.position_bits == 64 ? (double)reinterpret_cast<const int64_t*>(p.positions)[at]
+                                           : (double)reinterpret_cast<const int32_t*>(p.positions)[at];
+  const double f = p.freq_dtype == FB_DTYPE_F64 ? reinterpret_cast<const double*>(p.inv_freq)[pr]
+                                                : (double)reinterpret_cast<const float*>(p.inv_freq)[pr];
+  const double turns = pos * (f * kInv2Pi);
+  float2 cs;
+  sincospif(2.f * (float)(turns - rint(turns)), &cs.y, &cs.x);
+  return cs;
+}
+
+// Where token s goes in the cache; false if nowhere.
+__device__ __forceinline__ bool cache_place(const fb_rope_params& p, int s, int64_t& page, int& place) {
+  const int64_t slot = p.slot_bits == 64 ? reinterpret_cast<const int64_t*>(p.slots)[s * p.slot_stride]
+                                         : (int64_t) reinterpret_cast<const int32_t*>(p.slots)[s * p.slot_stride];
+  if (slot < 0) return false;
+  page = slot / p.page_size;
+  place = (int)(slot - page * p.page_size);
+  if (page < p.num_pages) return true;
+  if (p.status) *reinterpret_cast<volatile int32_t*>(p.status) = FB_DEV_BAD_INDEX;
+  return false;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// ---- general kernels: any D up to 128, any strides; a warp per row ------------------------------------------------
+template <typename T, bool APPEND>
+__global__ void __launch_bounds__(kRopeThreads) rope_general_kernel(const __grid_constant__ fb_rope_params p) {
+  __shared__ float2 turn[kRopeMaxD / 2];
+  __shared__ float rows[kRopeWarps][kRopeMaxD];
+  const int b = blockIdx.x / p.S, s = blockIdx.x % p.S;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = p.rot >> 1;
+  if (threadIdx.x < half) turn[threadIdx.x] = rope_turn(p, b, s, threadIdx.x);
+  __syncthreads();
+  int64_t page = 0;
+  int place = 0;
+  const bool cached = APPEND && cache_place(p, s, page, place);
+  float* row = rows[warp];
+  for (int r = warp; r < p.Hq + p.Hk; r += kRopeWarps) {
+    const bool is_q = r < p.Hq;
+    const int h = is_q ? r : r - p.Hq;
+    if (APPEND && !is_q && !cached) break;
+    const int64_t* xs = is_q ? p.q_stride : p.k_stride;
+    const T* x = reinterpret_cast<const T*>(is_q ? p.q : p.k) + b * xs[0] + h * xs[1] + s * xs[2];
+    const void* w = is_q ? p.q_weight : p.k_weight;
+    T* y;
+    if (APPEND && !is_q) {
+      y = reinterpret_cast<T*>(p.key_cache) + page * p.key_cache_stride[0] + place * p.key_cache_stride[1] + h * p.key_cache_stride[2];
+    } else {
+      const int64_t* ys = is_q ? p.q_out_stride : p.k_out_stride;
+      y = reinterpret_cast<T*>(is_q ? p.q_out : p.k_out) + b * ys[0] + h * ys[1] + s * ys[2];
+    }
+    float ss = 0.f;
+    for (int c = lane; c < p.D; c += 32) {
+      const float v = to_f32(x[c]);
+      row[c] = v;
+      ss += v * v;
+    }
+    __syncwarp();
+    if (w) {
+      const float rr = rsqrtf(warp_sum(ss) / p.D + p.eps);
+      for (int c = lane; c < p.D; c += 32) row[c] = row[c] * rr * load_scalar(w, p.weight_dtype, c);
+      __syncwarp();
+    }
+    for (int i = lane; i < half; i += 32) {
+      const int lo = p.interleaved ? 2 * i : i, hi = p.interleaved ? 2 * i + 1 : i + half;
+      const float2 cs = turn[i];
+      y[lo] = from_f32<T>(row[lo] * cs.x - row[hi] * cs.y);
+      y[hi] = from_f32<T>(row[hi] * cs.x + row[lo] * cs.y);
+    }
+    for (int c = p.rot + lane; c < p.D; c += 32) y[c] = w ? from_f32<T>(row[c]) : x[c];  // (untouched values keep their bits)
+    __syncwarp();
+  }
+  if constexpr (!APPEND) return;
+  if (!cached) return;
+  for (int i = threadIdx.x; i < p.Hk * p.D; i += kRopeThreads) {
+    const int h = i / p.D, c = i - h * p.D;
+    reinterpret_cast<T*>(p.value_cache)[page * p.value_cache_stride[0] + place * p.value_cache_stride[1] + h * p.value_cache_stride[2] + c] =
+        reinterpret_cast<const T*>(p.v)[h * p.v_stride[1] + s * p.v_stride[2] + c];
+  }
+  for (int i = threadIdx.x; i < p.bias_heads * p.R; i += kRopeThreads) {
+    const int h = i / p.R, c = i - h * p.R;
+    reinterpret_cast<T*>(p.bias_cache)[page * p.bias_cache_stride[0] + place * p.bias_cache_stride[1] + h * p.bias_cache_stride[2] + c] =
+        reinterpret_cast<const T*>(p.k_bias)[h * p.k_bias_stride[1] + s * p.k_bias_stride[2] + c];
+  }
+}
+
+// Partial sums of the weight gradients: (CTAs, 2, D) floats, added up in the order of the CTAs by rope_weight_kernel.
+template <typename T>
+__global__ void __launch_bounds__(kRopeThreads) rope_bwd_general_kernel(const __grid_constant__ fb_rope_params p, int64_t tokens) {
+  __shared__ float2 turn[kRopeMaxD / 2];
+  __shared__ float rows[kRopeWarps][2 * kRopeMaxD];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = p.rot >> 1;
+  float* row = rows[warp];         // x
+  float* grad = row + kRopeMaxD;   // dout, then g
+  float dw[2][kRopeMaxD / 32] = {};
+  for (int64_t tok = blockIdx.x; tok < tokens; tok += gridDim.x) {
+    const int b = (int)(tok / p.S), s = (int)(tok % p.S);
+    __syncthreads();
+    if (threadIdx.x < half) turn[threadIdx.x] = rope_turn(p, b, s, threadIdx.x);
+    __syncthreads();
+    for (int r = warp; r < p.Hq + p.Hk; r += kRopeWarps) {
+      const bool is_q = r < p.Hq;
+      const int h = is_q ? r : r - p.Hq;
+      const int64_t *xs = is_q ? p.q_stride : p.k_stride, *gs = is_q ? p.dq_out_stride : p.dk_out_stride,
+                    *ds = is_q ? p.dq_stride : p.dk_stride;
+      const T* x = reinterpret_cast<const T*>(is_q ? p.q : p.k) + b * xs[0] + h * xs[1] + s * xs[2];
+      const T* go = reinterpret_cast<const T*>(is_q ? p.dq_out : p.dk_out) + b * gs[0] + h * gs[1] + s * gs[2];
+      T* dx = reinterpret_cast<T*>(is_q ? p.dq : p.dk) + b * ds[0] + h * ds[1] + s * ds[2];
+      const void* w = is_q ? p.q_weight : p.k_weight;
+      for (int c = lane; c < p.D; c += 32) grad[c] = to_f32(go[c]);
+      __syncwarp();
+      for (int i = lane; i < half; i += 32) {
+        const int lo = p.interleaved ? 2 * i : i, hi = p.interleaved ? 2 * i + 1 : i + half;
+        const float2 cs = turn[i];
+        const float gl = grad[lo], gh = grad[hi];
+        grad[lo] = gl * cs.x + gh * cs.y;
+        grad[hi] = gh * cs.x - gl * cs.y;
+      }
+      __syncwarp();
+      if (!w) {
+        for (int c = lane; c < p.D; c += 32) dx[c] = from_f32<T>(grad[c]);
+        __syncwarp();
+        continue;
+      }
+      float ss = 0.f, sg = 0.f;
+      for (int c = lane; c < p.D; c += 32) {
+        const float v = to_f32(x[c]);
+        row[c] = v;
+        ss += v * v;
+        sg += v * grad[c] * load_scalar(w, p.weight_dtype, c);
+      }
+      const float rr = rsqrtf(warp_sum(ss) / p.D + p.eps), mean = warp_sum(sg) / p.D;
+#pragma unroll
+      for (int j = 0; j < kRopeMaxD / 32; ++j) {
+        const int c = lane + 32 * j;
+        if (c >= p.D) break;
+        const float xr = row[c] * rr;
+        if (is_q) dw[0][j] += grad[c] * xr;
+        else dw[1][j] += grad[c] * xr;
+        dx[c] = from_f32<T>(rr * (load_scalar(w, p.weight_dtype, c) * grad[c] - xr * (rr * mean)));
+      }
+      __syncwarp();
+    }
+  }
+  if (!p.workspace) return;
+  float* part = reinterpret_cast<float*>(p.workspace) + (int64_t)blockIdx.x * 2 * p.D;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kRopeMaxD / 32; ++j) row[lane + 32 * j] = dw[t][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.D; c += kRopeThreads) {
+      float v = 0.f;
+      for (int w = 0; w < kRopeWarps; ++w) v += rows[w][c];
+      part[t * p.D + c] = v;
+    }
+  }
+}
+
+// Block (32, 32): 32 columns of one weight, the partial sums spread over the other dimension.
+__global__ void __launch_bounds__(1024) rope_weight_kernel(const __grid_constant__ fb_rope_params p, int parts) {
+  __shared__ float s[32][33];
+  grid_dep_wait();
+  const int c = blockIdx.x * 32 + threadIdx.x, t = blockIdx.y;
+  float v = 0.f;
+  if (c < p.D)
+    for (int i = threadIdx.y; i < parts; i += 32) v += reinterpret_cast<const float*>(p.workspace)[((int64_t)i * 2 + t) * p.D + c];
+  s[threadIdx.y][threadIdx.x] = v;
+  __syncthreads();
+  if (threadIdx.y) return;
+  v = 0.f;
+  for (int i = 0; i < 32; ++i) v += s[i][threadIdx.x];
+  void* out = t ? p.dk_weight : p.dq_weight;
+  if (out && c < p.D) store_scalar(out, p.weight_dtype, c, v);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+namespace {
+bool negative(const int64_t (&s)[3]) { return s[0] < 0 || s[1] < 0 || s[2] < 0; }
+
+int validate_rope(const fb_rope_params* p) {
+  if (!p) return FB_EINVAL_NULL;
+  if (p->B <= 0 || p->S <= 0 || p->Hq < 0 || p->Hk < 0 || p->Hq + (int64_t)p->Hk <= 0 || p->Hq + (int64_t)p->Hk > 65536) return FB_EINVAL_SHAPE;
+  if (p->D <= 0 || p->D > kRopeMaxD || (int64_t)p->B * p->S > 0x7fffffffLL) return FB_EINVAL_SHAPE;
+  if (p->dtype != FB_DTYPE_F16 && p->dtype != FB_DTYPE_BF16) return FB_EINVAL_DTYPE;
+  if (p->q_weight || p->k_weight) {
+    if (p->weight_dtype != FB_DTYPE_F16 && p->weight_dtype != FB_DTYPE_BF16 && p->weight_dtype != FB_DTYPE_F32) return FB_EINVAL_DTYPE;
+    if (!(p->eps >= 0.f)) return FB_EINVAL_SHAPE;
+  }
+  if (p->rot < 0 || p->rot > p->D || p->rot % 2) return FB_EINVAL_ROPE;
+  if (p->rot) {
+    if (!p->positions || !p->inv_freq || p->naxes < 1 || p->naxes > 4) return FB_EINVAL_ROPE;
+    if (p->position_bits != 32 && p->position_bits != 64) return FB_EINVAL_DTYPE;
+    if (p->freq_dtype != FB_DTYPE_F32 && p->freq_dtype != FB_DTYPE_F64) return FB_EINVAL_DTYPE;
+    for (int i = 0; i < p->rot / 2; ++i)
+      if (p->pair_axis[i] >= p->naxes) return FB_EINVAL_ROPE;
+  }
+  if ((p->Hq && !p->q) || (p->Hk && !p->k)) return FB_EINVAL_NULL;
+  if (negative(p->q_stride) || negative(p->k_stride)) return FB_EINVAL_STRIDE;
+  return 0;
+}
+
+int rope_bwd_ctas(const fb_rope_params* p) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int64_t most = 8ll * (device_sm_count(dev) > 0 ? device_sm_count(dev) : 148), tokens = (int64_t)p->B * p->S;
+  return (int)(tokens < most ? tokens : most);
+}
+bool wants_weights(const fb_rope_params* p) { return p->dq_weight || p->dk_weight; }
+}  // namespace
+
+}  // namespace fb
+
+using namespace fb;
+
+extern "C" size_t fb_rope_params_size(void) { return sizeof(fb_rope_params); }
+
+extern "C" int fb_norm_rope(const fb_rope_params* p, void* cuda_stream) {
+  if (const int rc = validate_rope(p)) return rc;
+  if ((p->Hq && !p->q_out) || (p->Hk && !p->k_out)) return FB_EINVAL_NULL;
+  if (negative(p->q_out_stride) || negative(p->k_out_stride)) return FB_EINVAL_STRIDE;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+  const unsigned grid = (unsigned)(p->B * p->S);
+  if (p->dtype == FB_DTYPE_F16) rope_general_kernel<__half, false><<<grid, kRopeThreads, 0, st>>>(*p);
+  else rope_general_kernel<__nv_bfloat16, false><<<grid, kRopeThreads, 0, st>>>(*p);
+  note_launch();
+  return (int)cudaGetLastError();
+}
+
+extern "C" size_t fb_norm_rope_bwd_workspace_bytes(const fb_rope_params* p) {
+  if (validate_rope(p) || !wants_weights(p)) return 0;
+  return round256((size_t)rope_bwd_ctas(p) * 2 * p->D * 4);
+}
+
+extern "C" int fb_norm_rope_bwd(const fb_rope_params* p, void* cuda_stream) {
+  if (const int rc = validate_rope(p)) return rc;
+  if ((p->Hq && (!p->dq_out || !p->dq)) || (p->Hk && (!p->dk_out || !p->dk))) return FB_EINVAL_NULL;
+  if (negative(p->dq_out_stride) || negative(p->dk_out_stride) || negative(p->dq_stride) || negative(p->dk_stride)) return FB_EINVAL_STRIDE;
+  if ((p->dq_weight && !p->q_weight) || (p->dk_weight && !p->k_weight)) return FB_EINVAL_NULL;
+  fb_rope_params a = *p;
+  const size_t need = fb_norm_rope_bwd_workspace_bytes(p);
+  if (need && (!p->workspace || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255))) return FB_EINVAL_WORKSPACE;
+  if (!need) a.workspace = nullptr;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+  const int ctas = rope_bwd_ctas(p);
+  const int64_t tokens = (int64_t)p->B * p->S;
+  if (p->dtype == FB_DTYPE_F16) rope_bwd_general_kernel<__half><<<ctas, kRopeThreads, 0, st>>>(a, tokens);
+  else rope_bwd_general_kernel<__nv_bfloat16><<<ctas, kRopeThreads, 0, st>>>(a, tokens);
+  note_launch();
+  if (need) {
+    rope_weight_kernel<<<dim3((p->D + 31) / 32, 2), dim3(32, 32), 0, st>>>(a, ctas);
+    note_launch();
+  }
+  return (int)cudaGetLastError();
+}
+
+extern "C" int fb_paged_append(const fb_rope_params* p, void* cuda_stream) {
+  if (const int rc = validate_rope(p)) return rc;
+  if (p->B != 1 || !p->Hk) return FB_EINVAL_SHAPE;
+  if ((p->Hq && !p->q_out) || !p->v || !p->key_cache || !p->value_cache || !p->slots) return FB_EINVAL_NULL;
+  if (negative(p->q_out_stride) || negative(p->v_stride) || negative(p->key_cache_stride) || negative(p->value_cache_stride) || p->slot_stride < 0)
+    return FB_EINVAL_STRIDE;
+  if (p->slot_bits != 32 && p->slot_bits != 64) return FB_EINVAL_DTYPE;
+  if (p->page_size <= 0 || p->num_pages <= 0) return FB_EINVAL_PAGE;
+  if (p->R < 0 || p->R > 256) return FB_EINVAL_SHAPE;
+  if (p->R) {
+    if (!p->k_bias || !p->bias_cache || (p->bias_heads != 1 && p->bias_heads != p->Hk)) return FB_EINVAL_BIAS;
+    if (negative(p->k_bias_stride) || negative(p->bias_cache_stride)) return FB_EINVAL_STRIDE;
+  } else if (p->k_bias || p->bias_cache || p->bias_heads) {
+    return FB_EINVAL_BIAS;
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+  if (p->dtype == FB_DTYPE_F16) rope_general_kernel<__half, true><<<p->S, kRopeThreads, 0, st>>>(*p);
+  else rope_general_kernel<__nv_bfloat16, true><<<p->S, kRopeThreads, 0, st>>>(*p);
+  note_launch();
+  return (int)cudaGetLastError();
+}

@@ -7,6 +7,7 @@
 // Mirrors FlashBiasFunc / flash_bias_func of the reference (flash_bias/flash_bias_triton.py:1345-1405): same
 // positional signature, layouts ((B, S, H, D) tensors, (B|1, S, H|1, R) factors, 4-D additive mask), host-side checks
 // and messages (:1102-1127, :1206-1210, :1371); outputs are fresh tensors, inputs are never mutated.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -418,6 +419,8 @@ Tensor prepare_bhsd(const Tensor& x, at::ScalarType dtype, bool normalize, const
   return y.permute({0, 2, 1, 3});
 }
 
+#include "torch_paged.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -444,4 +447,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_bias_alibi", &flash_bias_alibi, release(), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("slopes"),
         py::arg("causal") = true, py::arg("softmax_scale") = py::none());
   m.def("prepare_bhsd", &prepare_bhsd, release());
+  m.def("norm_rope", &norm_rope, release());
+  m.def("paged_append", &paged_append, release());
+  m.def("paged_plan", &paged_plan, release());
+  m.def("paged_forward", &paged_forward, release());
 }

@@ -29,7 +29,8 @@ extern "C" {
 /* element types */
 #define FB_DTYPE_F16 0
 #define FB_DTYPE_BF16 1
-#define FB_DTYPE_F32 2 /* mask only */
+#define FB_DTYPE_F32 2 /* mask, norm weights, frequencies only */
+#define FB_DTYPE_F64 3 /* frequencies only */
 
 /* additive mask kinds: last two dims (1, Sk) = vector, (Sq, Sk) = matrix
  * (flash_bias/flash_bias_triton.py:1120-1127) */
@@ -62,6 +63,8 @@ extern "C" {
 #define FB_ENOTBUILT -9        /* the library was built without the requested kernel */
 #define FB_EDEVICE -10         /* a kernel reported a device-side error through the status word */
 #define FB_EINVAL_SIZE -11     /* the problem needs more scratch than a fixed-capacity entry point holds */
+#define FB_EINVAL_ROPE -12     /* rotated columns, axes, frequencies or positions do not fit each other */
+#define FB_EINVAL_PAGE -13     /* page size, page count or table width not positive, or too many slots */
 
 /*
  * One problem description, shared by forward and backward.
@@ -124,6 +127,8 @@ typedef struct fb_params {
 #define FB_DEV_OK 0
 #define FB_DEV_WAIT_TIMEOUT 1    /* a bounded wait inside a kernel expired; the results of that call are invalid */
 #define FB_DEV_FACTOR_OVERFLOW 2 /* a pre-scaled bias factor left the range of the 16-bit type */
+#define FB_DEV_BAD_INDEX 3       /* an index in device memory (page, slot, offset, parent, page count) is out of range: what it
+                                    names was not accessed */
 
 int fb_version(void);
 size_t fb_params_size(void); /* sizeof(fb_params) as compiled, for bindings to check their mirror of the struct */
@@ -181,6 +186,140 @@ const char *fb_status_string(int32_t value);
 int fb_prepare_rows(const void *x, int32_t x_dtype, const int64_t *x_stride, void *y, int32_t y_dtype,
                     const int64_t *y_stride, int32_t B, int32_t H, int32_t S, int32_t D, int32_t normalize,
                     const float *head_scale, float eps, void *cuda_stream);
+
+/*
+ * Norm of queries and keys per head with the rotation by position in the same pass; and, with the cache fields, the same
+ * pass with the rotated keys, the values and the keys' bias factors going into the pages of a cache.  No counterpart in the
+ * reference; what its call sites run in front of flash_bias_func is fb_prepare_rows.
+ *
+ *   y   = x * rsqrt(mean(x^2) + eps) * weight           (weight null: y = x)
+ *   out = y with every pair (lo, hi) of its first `rot` columns turned by the angle position[axis(pair)] * inv_freq[pair]
+ *
+ * Pair p is (p, p + rot/2), or with `interleaved` (2p, 2p + 1).  Angles are taken in 64 bits, everything else in 32, and the
+ * result is rounded once.  Tensors: ptr[b*stride[0] + h*stride[1] + row*stride[2] + col], element strides; q (B, S, Hq, D),
+ * k (B, S, Hk, D); Hq or Hk = 0 leaves a tensor out.
+ */
+typedef struct fb_rope_params {
+  int32_t B, S, Hq, Hk, D;
+  int32_t dtype;        /* FB_DTYPE_F16 | FB_DTYPE_BF16: q, k, v and their results */
+  int32_t weight_dtype; /* FB_DTYPE_F16 | FB_DTYPE_BF16 | FB_DTYPE_F32 */
+  int32_t rot;          /* rotated columns: even, 0 (no rotation; positions and inv_freq unused) to D */
+  int32_t interleaved;
+  int32_t naxes;         /* 1 to 4 position axes */
+  int32_t position_bits; /* 32 or 64: type of positions */
+  int32_t freq_dtype;    /* FB_DTYPE_F32 | FB_DTYPE_F64 */
+  float eps;
+  int32_t flags;         /* FB_FLAG_FORCE_GENERAL */
+  uint8_t pair_axis[64]; /* axis of each of the rot/2 pairs */
+  const void *q, *k, *q_weight, *k_weight, *positions, *inv_freq;
+  int64_t q_stride[3], k_stride[3];
+  int64_t position_stride[3]; /* (axis, batch, row); 0 where shared; may be negative */
+  void *q_out, *k_out;
+  int64_t q_out_stride[3], k_out_stride[3];
+
+  /* backward only: gradients of q_out and k_out in, of q, k and the weights (weight_dtype, D values) out */
+  const void *dq_out, *dk_out;
+  int64_t dq_out_stride[3], dk_out_stride[3];
+  void *dq, *dk, *dq_weight, *dk_weight; /* a weight gradient may be null */
+  int64_t dq_stride[3], dk_stride[3];
+  void *workspace; /* fb_norm_rope_bwd_workspace_bytes(), 256-byte aligned */
+  size_t workspace_bytes;
+
+  /* fb_paged_append only: B = 1, S tokens; k_out unused.  Cache: ptr[page*stride[0] + slot*stride[1] + h*stride[2] + col];
+   * key and value (num_pages, page_size, Hk, D), bias (num_pages, page_size, bias_heads, R).  Token n goes to
+   * page slots[n] / page_size, place slots[n] % page_size; a negative slot is a token of no request: nothing is written. */
+  const void *v, *k_bias;
+  int64_t v_stride[3], k_bias_stride[3];
+  void *key_cache, *value_cache, *bias_cache;
+  int64_t key_cache_stride[3], value_cache_stride[3], bias_cache_stride[3];
+  const void *slots;
+  int64_t slot_stride;
+  int32_t slot_bits; /* 32 or 64 */
+  int32_t page_size;
+  int64_t num_pages;
+  int32_t R, bias_heads; /* 0, or the rank and 1 or Hk */
+  int32_t *status;       /* optional, as in fb_params */
+} fb_rope_params;
+
+size_t fb_rope_params_size(void);
+int fb_norm_rope(const fb_rope_params *p, void *cuda_stream);
+size_t fb_norm_rope_bwd_workspace_bytes(const fb_rope_params *p);
+int fb_norm_rope_bwd(const fb_rope_params *p, void *cuda_stream);
+int fb_paged_append(const fb_rope_params *p, void *cuda_stream);
+
+/*
+ * The plan of one serving step, on the device from device lengths: page counts follow the lengths, the stack of free pages
+ * follows the page counts, and every new token gets its request, slot, position and (for a tree of drafted tokens) the bits of
+ * its ancestors.  All integers are int32 unless said otherwise.  No counterpart in the reference.
+ *
+ * Request b holds pages_held[b] pages, the first entries of its row of block_table, and lens[b] tokens; new_lens[b] tokens
+ * join.  With need = ceil((lens + new_lens) / page_size):
+ *   - pages beyond need go back to the stack, in the order of the requests, the first one on top;
+ *   - missing pages are taken from the top of the stack, in the order of the requests, while it lasts.
+ * A request is refused when its pages do not last, its row is too short, its tokens pass num_tokens, its tree has more than
+ * 64 * mask_words tokens, or a length is negative; it keeps its pages and length, its tokens get slot -1, position 0 and no
+ * bits, and lens_out[b] is -1 (its tokens still count in cu_tokens; negative new_lens count as none).  Once a request does not
+ * get its pages, no later one of the call gets any.  lens_out[b] is lens[b] otherwise.
+ */
+typedef struct fb_plan_params {
+  int32_t B, num_tokens, page_size, table_width, stack_size, mask_words;
+  int32_t *block_table; /* (B, table_width), updated */
+  int64_t table_stride;
+  int32_t *pages_held; /* (B), updated */
+  int32_t *free_pages; /* (stack_size), the first *free_count of them are free; updated */
+  int32_t *free_count; /* (1), updated */
+  const int32_t *lens, *new_lens;
+  const int32_t *parents; /* optional (num_tokens): index within its request of a token's parent, before the token's own; < 0: the
+                             cached context.  Null: each token follows the one before. */
+  int32_t *cu_tokens, *lens_out, *positions; /* (B + 1), (B), (num_tokens) */
+  int64_t *slots;                            /* (num_tokens), -1 for what no request owns */
+  int64_t *tree_mask;                        /* with parents: (num_tokens, mask_words), bit j % 64 of word j / 64: token j of the
+                                                same request is this token or one of its ancestors */
+  int32_t *status;                           /* optional, as in fb_params */
+} fb_plan_params;
+
+size_t fb_plan_params_size(void);
+int fb_paged_plan(const fb_plan_params *p, void *cuda_stream);
+
+/*
+ * Attention of the newest tokens of every request over its pages.  Request b owns tokens cu_tokens[b] .. cu_tokens[b + 1] - 1
+ * of q, T_b in number; its keys are the first lens[b] + T_b places of its pages, the last T_b of them those tokens' own.  Token
+ * t sees the lens[b] cached keys, and key lens[b] + t' if bit t' of its tree_mask is set (tree_mask null: if t' <= t).
+ *
+ *   o = softmax(softmax_scale * q.k + bias) v,   bias = slopes[h] * (pos_key - pos_token), or q_bias . bias_cache, or none
+ *
+ * pos of cached key j is j; of token t (and of its key) positions[cu_tokens[b] + t], or lens[b] + t without positions.  Query
+ * head h reads key head h / (Hq / Hk).  lens[b] < 0, tokens that no request owns, and rows that see no key: o = 0, lse = -inf.
+ * A page outside the cache, or a place behind the row of the table, sets FB_DEV_BAD_INDEX and is left out.  No counterpart in
+ * the reference, whose forward reads dense tensors.
+ */
+typedef struct fb_paged_params {
+  int32_t N, B, Hq, Hk, D, R;
+  int32_t dtype;
+  int32_t page_size, table_width, mask_words, bias_heads; /* bias_heads: heads of bias_cache, 1 or Hk */
+  int32_t flags;                                          /* FB_FLAG_FORCE_GENERAL */
+  int64_t num_pages;
+  float softmax_scale;
+  const void *q, *q_bias, *key_cache, *value_cache, *bias_cache;
+  int64_t q_stride[2], q_bias_stride[2];                                    /* (token, head) */
+  int64_t key_cache_stride[3], value_cache_stride[3], bias_cache_stride[3]; /* (page, place, head) */
+  const int32_t *block_table;
+  int64_t table_stride;
+  const int32_t *lens, *cu_tokens, *positions; /* positions optional */
+  const int64_t *tree_mask;                    /* optional, (N, mask_words) */
+  int64_t mask_stride;
+  const float *slopes; /* optional, Hq values */
+  void *o;
+  int64_t o_stride[2];
+  float *lse; /* optional, (N, Hq) contiguous */
+  void *workspace; /* fb_paged_workspace_bytes(), 256-byte aligned */
+  size_t workspace_bytes;
+  int32_t *status; /* optional, as in fb_params */
+} fb_paged_params;
+
+size_t fb_paged_params_size(void);
+size_t fb_paged_workspace_bytes(const fb_paged_params *p);
+int fb_paged_fwd(const fb_paged_params *p, void *cuda_stream);
 
 /*
  * fb_fwd for callers that cannot allocate device memory.  This entry point has no counterpart in the
