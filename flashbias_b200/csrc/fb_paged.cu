@@ -2,23 +2,11 @@
 //
 //   logit = scale q.k + slope (pos_key - pos_token)  |  + q_bias . bias_cache;   o = softmax(logit) v, statistics in fp32
 //
-// Bound by reading K and V of every request once while there are few rows per key head, by the products beyond.
-#include <float.h>
-
-#include "fb_common.cuh"
-#include "fb_internal.h"
+// Bound by reading K and V of every request once while there are few rows per key head, by the products beyond.  Here: the
+// shape-generic kernel, the choice of the kernel and the entry points.
+#include "fb_paged.cuh"
 
 namespace fb {
-
-constexpr float kLog2eP = 1.4426950408889634f;
-constexpr float kLn2P = 0.6931471805599453f;
-
-__device__ __forceinline__ void paged_bad_index(const fb_paged_params& p) {
-  if (p.status) *reinterpret_cast<volatile int32_t*>(p.status) = FB_DEV_BAD_INDEX;
-}
-
-// Offsets within [0, N], whatever the device array holds.
-__device__ __forceinline__ int cu_at(const fb_paged_params& p, int b) { return min(max(p.cu_tokens[b], 0), p.N); }
 
 // ---- general kernel: any head_dim up to 128, any strides; one block per (token, head), keys over its warps ---------
 template <typename T>
@@ -32,14 +20,10 @@ __global__ void __launch_bounds__(128) paged_general_kernel(const __grid_constan
     if (cu_at(p, mid + 1) > n) hi = mid;
     else lo = mid + 1;
   }
-  const int first = cu_at(p, lo), end = cu_at(p, lo + 1), len = p.lens[lo], t = n - first;
-  const bool live = n >= first && n < end && len >= 0;
-  int64_t keys = live ? (int64_t)len + (end - first) : 0;
-  const int64_t room = (int64_t)p.table_width * p.page_size;
-  if (keys > room) {
-    if (threadIdx.x == 0) paged_bad_index(p);
-    keys = room;
-  }
+  const Request rq = request_at(p, lo);
+  const int first = rq.first, len = rq.len, t = n - first;
+  const bool live = t >= 0 && t < rq.tokens && len >= 0;
+  const int64_t keys = live ? rq.keys : 0;
   const int my_pos = live ? (p.positions ? p.positions[n] : len + t) : 0;
   const float slope = p.slopes ? p.slopes[h] : 0.f;
   const int64_t* words = p.tree_mask ? p.tree_mask + n * p.mask_stride : nullptr;
@@ -149,6 +133,35 @@ static int validate_paged(const fb_paged_params* p) {
   return 0;
 }
 
+// The kernel of a call.  Rows that are whole aligned 16-byte chunks take the split kernel.
+static PagedPlan plan_paged(const fb_paged_params* p) {
+  PagedPlan plan = {};
+  uintptr_t bits = reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->key_cache) | reinterpret_cast<uintptr_t>(p->value_cache) |
+                   reinterpret_cast<uintptr_t>(p->o);
+  for (int i = 0; i < 3; ++i) {
+    bits |= (uintptr_t)(p->key_cache_stride[i] | p->value_cache_stride[i]) * 2;
+    if (i < 2) bits |= (uintptr_t)(p->q_stride[i] | p->o_stride[i]) * 2;
+  }
+  const int G = p->Hq / p->Hk;
+  if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 8 || (bits & 15) || (int64_t)p->N * G > 0x7fffffffLL) return plan;
+  plan.kernel = 1;
+  plan.TD = p->D <= 32 ? 32 : p->D <= 64 ? 64 : 128;
+  const int64_t rows = ((int64_t)p->N * G + p->B - 1) / p->B;  // per request on average
+  plan.MT = rows <= 16 ? 16 : 32;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  plan.ctas = 2 * (device_sm_count(dev) > 0 ? device_sm_count(dev) : 148);
+  // The heads of a group are read side by side, whole rows of the cache; where the longest requests that the table can hold do
+  // not fill the GPU that way, one head is spread over the CTA's warps.
+  const int64_t tiles = (int64_t)p->B * (((int64_t)p->table_width * p->page_size + 63) / 64) * p->Hk;
+  plan.WH = p->Hk % 4 == 0 && tiles / 4 >= 4 * plan.ctas ? 4 : p->Hk % 2 == 0 && tiles / 2 >= 4 * plan.ctas ? 2 : 1;
+  const size_t prows = (size_t)plan.ctas * 2 * plan.WH * plan.MT;
+  plan.part_bytes = round256(prows * plan.TD * 4);
+  plan.ml_bytes = round256(prows * 8);
+  plan.desc_bytes = round256((size_t)plan.ctas * 16);
+  return plan;
+}
+
 }  // namespace fb
 
 using namespace fb;
@@ -157,12 +170,29 @@ extern "C" size_t fb_paged_params_size(void) { return sizeof(fb_paged_params); }
 
 extern "C" size_t fb_paged_workspace_bytes(const fb_paged_params* p) {
   if (validate_paged(p)) return 0;
-  return 0;
+  const PagedPlan plan = plan_paged(p);
+  return plan.part_bytes + plan.ml_bytes + plan.desc_bytes;
 }
 
 extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
   if (const int rc = validate_paged(p)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+  const PagedPlan plan = plan_paged(p);
+  if (plan.kernel == 1) {
+    const size_t need = plan.part_bytes + plan.ml_bytes + plan.desc_bytes;
+    if (!p->workspace || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255)) return FB_EINVAL_WORKSPACE;
+    PagedArgs a = {};
+    a.p = *p;
+    a.G = p->Hq / p->Hk;
+    a.page_div = Div(p->page_size);
+    a.group_div = Div(a.G);
+    a.scale_log2 = p->softmax_scale * kLog2eP;
+    uint8_t* ws = reinterpret_cast<uint8_t*>(p->workspace);
+    a.part = reinterpret_cast<float*>(ws);
+    a.ml = reinterpret_cast<float2*>(ws + plan.part_bytes);
+    a.desc = reinterpret_cast<int4*>(ws + plan.part_bytes + plan.ml_bytes);
+    return plan.TD == 32 ? launch_paged_split_d32(a, plan, st) : plan.TD == 64 ? launch_paged_split_d64(a, plan, st) : launch_paged_split_d128(a, plan, st);
+  }
   const unsigned grid = (unsigned)(p->N * p->Hq);
   if (p->dtype == FB_DTYPE_F16) paged_general_kernel<__half><<<grid, 128, 0, st>>>(*p);
   else paged_general_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(*p);

@@ -1,0 +1,176 @@
+// Shared by the kernels of attention over pages: offsets and lengths as the device arrays hold them, and the schedule that
+// cuts the work of a call into equal parts.
+//
+// The lengths live on the device and a call reads nothing back, so the grid cannot follow them.  Instead the key tiles of all
+// (request, row tile, head group) items are numbered through, and CTA c of a fixed grid takes the numbers from c U / C to
+// (c + 1) U / C: every CTA reads the same amount of K and V whatever the lengths are.  An item that spans several CTAs leaves
+// unnormalised sums in the workspace, at most two per CTA, and a second small kernel joins them in the order of the CTAs.
+#pragma once
+
+#include <float.h>
+
+#include "fb_common.cuh"
+#include "fb_internal.h"
+
+namespace fb {
+
+constexpr float kLog2eP = 1.4426950408889634f;
+constexpr float kLn2P = 0.6931471805599453f;
+
+struct PagedArgs {
+  fb_paged_params p;
+  Div page_div, group_div;  // by page_size, by the query heads of a key head
+  int G;                    // query heads of a key head
+  float scale_log2;
+  float* part;    // (CTAs, 2, heads of a group, rows of a tile, columns): sums of items that span CTAs
+  float2* ml;     // the same without columns: maximum (log2 units) and sum
+  int4* desc;     // (CTAs): the item that begins in a CTA and ends in another: request, row tile, head group, last CTA; x = -1: none
+};
+
+__device__ __forceinline__ void paged_bad_index(const fb_paged_params& p) {
+  if (p.status) *reinterpret_cast<volatile int32_t*>(p.status) = FB_DEV_BAD_INDEX;
+}
+
+// Offsets within [0, N], whatever the device array holds.
+__device__ __forceinline__ int cu_at(const fb_paged_params& p, int b) { return min(max(p.cu_tokens[b], 0), p.N); }
+
+// A request as the kernels see it.  Two more than p.B: the tokens behind the last request and before the first one, as
+// requests without keys, so that their rows are written.
+struct Request {
+  int first, tokens, len, keys;  // keys: cached and new ones, 0 where the request is not served
+};
+__device__ __forceinline__ Request request_at(const fb_paged_params& p, int b) {
+  Request r;
+  if (b >= p.B) {
+    const int at = cu_at(p, b == p.B ? p.B : 0);
+    r.first = b == p.B ? at : 0;
+    r.tokens = b == p.B ? p.N - at : at;
+    r.len = -1;
+    r.keys = 0;
+    return r;
+  }
+  const int c0 = p.cu_tokens[b], c1 = p.cu_tokens[b + 1];
+  r.first = min(max(c0, 0), p.N);
+  r.tokens = max(min(max(c1, 0), p.N) - r.first, 0);
+  r.len = p.lens[b];
+  if (c0 < 0 || c1 > p.N || c1 < c0) paged_bad_index(p);
+  int64_t keys = r.len < 0 ? 0 : (int64_t)r.len + r.tokens;
+  const int64_t room = (int64_t)p.table_width * p.page_size;
+  if (keys > room) {
+    paged_bad_index(p);
+    keys = room;
+  }
+  r.keys = (int)keys;
+  return r;
+}
+
+// One item of a request, and the part of its key tiles that a CTA takes.
+struct Segment {
+  int b, rt, hg;     // request, row tile, head group
+  int t0, t1, tiles;  // key tiles [t0, t1) of `tiles`
+  int last_cta;      // the CTA that holds the item's last tile
+  Request r;
+};
+
+// Walks the segments of one CTA.  Every thread of the block calls it alike.
+template <int KT, int MT, int THREADS>
+struct PagedWalk {
+  int64_t u, u1, pre;  // next number, end of the CTA's range, first number of request b
+  int64_t total;
+  int b, ngroups, ctas;
+  Request r;
+
+  __device__ __forceinline__ static int row_tiles(const PagedArgs& a, const Request& r) { return (int)(((int64_t)r.tokens * a.G + MT - 1) / MT); }
+  __device__ __forceinline__ static int key_tiles(const Request& r) { return max((int)(((int64_t)r.keys + KT - 1) / KT), 1); }
+  __device__ __forceinline__ static int64_t units(const PagedArgs& a, const Request& r, int ngroups) {
+    return r.tokens ? (int64_t)row_tiles(a, r) * key_tiles(r) * ngroups : 0;
+  }
+
+  // Finds the request in which the CTA's range begins: each thread adds up a run of requests, a scan over the threads.
+  __device__ __forceinline__ void start(const PagedArgs& a, int groups) {
+    __shared__ int64_t s_sum[THREADS / 32], s_pre;
+    __shared__ int s_b;
+    ngroups = groups;
+    const int n = a.p.B + 2, per = (n + THREADS - 1) / THREADS, b0 = threadIdx.x * per, b1 = min(b0 + per, n);
+    int64_t mine = 0;
+    for (int i = b0; i < b1; ++i) mine += units(a, request_at(a.p, i), groups);
+    int64_t x = mine;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_sum[warp] = x;
+    if (threadIdx.x == 0) s_b = -1;
+    __syncthreads();
+    int64_t before = x - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += s_sum[w];
+      total += s_sum[w];
+    }
+    ctas = (int)min((int64_t)gridDim.x, total);  // each of these has one number at least: an item's parts leave no gap
+    u = blockIdx.x < ctas ? (int64_t)blockIdx.x * total / ctas : total;
+    u1 = blockIdx.x < ctas ? (int64_t)(blockIdx.x + 1) * total / ctas : total;
+    if (u < u1 && before <= u && u < before + mine) {
+      int64_t at = before;
+      int i = b0;
+      for (;; ++i) {
+        const int64_t k = units(a, request_at(a.p, i), groups);
+        if (u < at + k) break;
+        at += k;
+      }
+      s_b = i;
+      s_pre = at;
+    }
+    __syncthreads();
+    b = s_b;
+    pre = s_pre;
+    if (u < u1) r = request_at(a.p, b);
+  }
+
+  __device__ __forceinline__ bool next(const PagedArgs& a, Segment& s) {
+    if (u >= u1) return false;
+    int64_t k;
+    while (u >= pre + (k = units(a, r, ngroups))) {  // (ends: u lies below the sum of all)
+      pre += k;
+      r = request_at(a.p, ++b);
+    }
+    s.b = b;
+    s.r = r;
+    s.tiles = key_tiles(r);
+    const int64_t local = u - pre, item = local / s.tiles;
+    const int rts = row_tiles(a, r);
+    s.hg = (int)(item / rts);
+    s.rt = (int)(item - (int64_t)s.hg * rts);
+    s.t0 = (int)(local - item * s.tiles);
+    s.t1 = (int)min((int64_t)s.tiles, s.t0 + (u1 - u));
+    const int64_t end = pre + (item + 1) * s.tiles;  // CTA c holds number n if c U / C <= n: the last one for n = end - 1
+    s.last_cta = (int)((end * ctas - 1) / total);
+    u += s.t1 - s.t0;
+    return true;
+  }
+};
+
+// Whether drafted token td of the request is seen by token t (global token n).
+__device__ __forceinline__ bool tree_sees(const fb_paged_params& p, int n, int t, int td) {
+  if (!p.tree_mask) return td <= t;
+  const int w = td >> 6;
+  return w < p.mask_words && ((p.tree_mask[n * p.mask_stride + w] >> (td & 63)) & 1);
+}
+
+// ---- host side (fb_paged.cu, fb_paged_split_*.cu) ------------------------------------------------------------------
+struct PagedPlan {
+  int kernel;   // 0: general, 1: split
+  int TD, MT;   // columns and rows of a tile
+  int WH;       // key heads of a group
+  int ctas;
+  size_t part_bytes, ml_bytes, desc_bytes;
+};
+int launch_paged_split_d32(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
+int launch_paged_split_d64(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
+int launch_paged_split_d128(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
+
+}  // namespace fb

@@ -1,0 +1,6 @@
+// Instantiations of the split kernel of attention over pages at tile width 32.
+#include "fb_paged_split.cuh"
+
+namespace fb {
+int launch_paged_split_d32(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) { return launch_paged_split<32>(a, plan, st); }
+}  // namespace fb

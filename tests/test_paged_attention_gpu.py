@@ -186,11 +186,9 @@ def test_a_table_that_is_too_short_and_offsets_out_of_range():
     for cu in ([0, 100], [-5, 1], [7, 3]):
         d["cu_tokens"] = torch.tensor(cu, dtype=torch.int32, device="cuda")
         flash_bias_paged_func(**d)  # offsets are held within the tokens
-    torch.cuda.synchronize()
-    try:
-        check_device_status()
-    except RuntimeError:
-        pass
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="out of range"):
+            check_device_status()
 
 
 def test_strided_queries_tables_and_empty_steps():
