@@ -5,8 +5,11 @@
 //   g = rotation of dout by the opposite angle,  dw = sum over rows of g x r,  dx = r (w g - x r^2 mean(w g x))
 //
 // Bound by reading x (and dout) once and writing the result once.  The angle position * inv_freq is taken in 64 bits and
-// reduced to a fraction of a turn before its sine and cosine are taken in 32: at position 1e6 a 32-bit product is off by up to
-// 0.03 rad.  It costs one pair of functions per token and frequency, shared by the token's heads, so no table is kept.
+// reduced to a fraction of a turn before its sine and cosine are taken in 32 (by the functions of the hardware, off by 2^-21,
+// an eighth of a percent of a step of fp16): at position 1e6 a 32-bit product is off by up to 0.03 rad.  It costs one pair of
+// functions per token and frequency, shared by the token's heads, so no table is kept.
+#include <type_traits>
+
 #include "fb_common.cuh"
 #include "fb_internal.h"
 
@@ -16,6 +19,7 @@ constexpr int kRopeWarps = 4;
 constexpr int kRopeThreads = 32 * kRopeWarps;
 constexpr int kRopeMaxD = 128;
 constexpr double kInv2Pi = 0.15915494309189533576888;
+constexpr float k2Pi = 6.28318530717958647693f;
 
 __device__ __forceinline__ float load_scalar(const void* p, int dtype, int i) {
   return dtype == FB_DTYPE_F32   ? reinterpret_cast<const float*>(p)[i]
@@ -37,7 +41,7 @@ __device__ __forceinline__ float2 rope_turn(const fb_rope_params& p, int b, int 
                                                 : (double)reinterpret_cast<const float*>(p.inv_freq)[pr];
   const double turns = pos * (f * kInv2Pi);
   float2 cs;
-  sincospif(2.f * (float)(turns - rint(turns)), &cs.y, &cs.x);
+  __sincosf((float)(turns - rint(turns)) * k2Pi, &cs.y, &cs.x);  // within +-pi: off by 2^-21
   return cs;
 }
 
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_general_kernel(const __grid
   }
 }
 
-// Partial sums of the weight gradients: (CTAs, 2, D) floats, added up in the order of the CTAs by rope_weight_kernel.
+// Partial sums of the weight gradients: (CTAs, 2, D) floats.
 template <typename T>
 __global__ void __launch_bounds__(kRopeThreads) rope_bwd_general_kernel(const __grid_constant__ fb_rope_params p, int64_t tokens) {
   __shared__ float2 turn[kRopeMaxD / 2];
@@ -196,14 +200,22 @@ __global__ void __launch_bounds__(kRopeThreads) rope_bwd_general_kernel(const __
   }
 }
 
-// Block (32, 32): 32 columns of one weight, the partial sums spread over the other dimension.
-__global__ void __launch_bounds__(1024) rope_weight_kernel(const __grid_constant__ fb_rope_params p, int parts) {
+// Adds up the blocks' partial sums in their order.  Block (32, 32): 32 columns of one weight, the partial sums spread over the
+// other dimension.  Tensor t has `parts` of them, `step` floats apart, from t * first on.
+struct WeightParts {
+  int parts[2];
+  int64_t first, step;
+};
+__global__ void __launch_bounds__(1024) rope_weight_kernel(const __grid_constant__ fb_rope_params p, const WeightParts q) {
   __shared__ float s[32][33];
   grid_dep_wait();
   const int c = blockIdx.x * 32 + threadIdx.x, t = blockIdx.y;
+  const float* part = reinterpret_cast<const float*>(p.workspace) + t * q.first + c;
   float v = 0.f;
-  if (c < p.D)
-    for (int i = threadIdx.y; i < parts; i += 32) v += reinterpret_cast<const float*>(p.workspace)[((int64_t)i * 2 + t) * p.D + c];
+  if (c < p.D) {
+#pragma unroll 8
+    for (int i = threadIdx.y; i < q.parts[t]; i += 32) v += part[i * q.step];
+  }
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.y) return;
@@ -213,35 +225,47 @@ __global__ void __launch_bounds__(1024) rope_weight_kernel(const __grid_constant
   if (out && c < p.D) store_scalar(out, p.weight_dtype, c, v);
 }
 
-// ---- vector kernels: rows of whole aligned 16-byte chunks, pairs that are whole chunks apart (or inside one) -------
-// G lanes (a power of two) share a row, 8 columns each; a block takes a run of tokens, all their heads.  The columns of a lane
-// are the same in every row, so its norm weights stay in registers; the angles of the block's tokens are taken once, into
-// shared memory; the other half of a pair comes from the lane that holds it, as 16-bit words.  Two rows per lane are in flight,
-// with 8 warps and 4 blocks per SM 64 KB.
-constexpr int kRopeVThreads = 256;
-constexpr int kRopeMaxTokens = 8;  // of a block at a time
-constexpr int kRopeUnroll = 2;
+// ---- vector kernels: rows of whole aligned 16-byte chunks -----------------------------------------------------------
+// A warp takes a token (or a share of its heads): G lanes (a power of two) share a row, 8 columns each, 32 / G rows side by
+// side.  Issue slots and the latency of a row's sums are what holds the rows back, not HBM: a warp issues about 110
+// instructions per 512 bytes (forward), at 6 warps per scheduler.  So all that depends on the column and the token alone
+// (weight times cosine, weight of the partner times sine) is folded into two coefficients per column that serve all heads of
+// the token, the address is one addition per row, and four rows (backward: two) are in flight per lane.
+// A lane holds both halves of its pairs: where they are half of the rotated columns apart (PAIR 0) it reads two runs of four
+// columns, where they are neighbours (1) one of eight.  Where the halves do not begin at a multiple of four (2) the other half
+// comes through shared memory.
+// B4 S4096 H32-8 D128 bf16, fp32 weights, us forward / backward: 64 (5.2 TB/s) / 117 (4.3 TB/s); with the other half by shuffle
+// 72 / 143, with coefficients from shared memory for every row and rows found by division 329 together.  Arithmetic on packed
+// pairs of fp32 issued as many instructions and was no faster; asking for the next token's rows ahead (L2) changed nothing.
+constexpr int kRopeVWarps = 4;
+constexpr int kRopeVThreads = 32 * kRopeVWarps;
 
 struct RopeV {
   fb_rope_params p;
-  Div s_div, hq_div, hk_div;
-  int tokens;   // B S
-  int run;      // tokens of a block at a time
+  Div s_div;
+  int tokens;  // B S
+  int split;   // warps of a token
+  int q_ctas;  // backward: blocks that take rows of q, the others rows of k
 };
 
 template <typename T>
-__device__ __forceinline__ void unpack_chunk(const uint4& w, float (&x)[8]) {
-  const T* e = reinterpret_cast<const T*>(&w);
+__device__ __forceinline__ void unpack_chunk(const uint4& raw, float (&x)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+  for (int i = 0; i < 4; ++i) {
+    if (std::is_same<T, __nv_bfloat16>::value) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
 }
 template <typename T>
 __device__ __forceinline__ uint4 pack_chunk(const float (&y)[8]) {
   return make_uint4(Pack2<T>::pack(y[0], y[1]), Pack2<T>::pack(y[2], y[3]), Pack2<T>::pack(y[4], y[5]), Pack2<T>::pack(y[6], y[7]));
-}
-__device__ __forceinline__ uint4 shfl_chunk(const uint4& w, int lane) {
-  return make_uint4(__shfl_sync(0xffffffffu, w.x, lane), __shfl_sync(0xffffffffu, w.y, lane), __shfl_sync(0xffffffffu, w.z, lane),
-                    __shfl_sync(0xffffffffu, w.w, lane));
 }
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -249,248 +273,352 @@ __device__ __forceinline__ float group_sum(float v) {
   for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-
-// What a lane holds of every row: 8 columns from col on, its partner's lane, its place among the pairs.
-template <int G, bool IL>
+// What a lane holds of every row: two runs of four columns, from c0 and c1 on.  PAIR 0: the first and the second halves of four
+// pairs, or eight columns in a row behind the rotated ones.  PAIR 1, 2: eight columns in a row.
+// FULL: the lanes' columns are those of the row, and all of them are rotated.
+template <typename T, int G, int PAIR, bool FULL>
 struct RopeLane {
-  int part, col, partner, pair0;
-  float sign;  // of the partner's term: out = y c + sign * y_partner s
-  bool in, turns;
+  int c0, c1;
+  bool in, turns;  // columns that exist; some of them rotated
   __device__ __forceinline__ RopeLane(const fb_rope_params& p) {
-    const int lane = threadIdx.x & 31, hc = p.rot >> 4;
-    part = lane % G;
-    col = part * 8;
-    in = col < p.D;
-    turns = col < p.rot;
-    const bool lo = part < hc;
-    partner = IL || !turns ? lane : lo ? lane + hc : lane - hc;
-    pair0 = IL ? col / 2 : lo ? col : col - 8 * hc;
-    sign = lo ? -1.f : 1.f;
+    const int part = (threadIdx.x & 31) % G;
+    c0 = part * 8;
+    in = FULL || c0 < p.D;
+    turns = FULL || c0 < p.rot;
+    if (!in) c0 = 0;  // (such a lane reads what exists and drops it)
+    c1 = c0 + 4;
+    if (PAIR == 0 && turns) {
+      c0 = part * 4;
+      c1 = c0 + (FULL ? 4 * G : p.rot >> 1);
+    }
   }
-  __device__ __forceinline__ void weights(const void* w, int dtype, int c0, float (&out)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = w && in ? load_scalar(w, dtype, c0 + i) : 1.f;
+  __device__ __forceinline__ uint4 load(const T* row) const {
+    if (PAIR != 0) return __ldcs(reinterpret_cast<const uint4*>(row + c0));
+    const uint2 a = __ldcs(reinterpret_cast<const uint2*>(row + c0)), b = __ldcs(reinterpret_cast<const uint2*>(row + c1));
+    return make_uint4(a.x, a.y, b.x, b.y);
   }
-  __device__ __forceinline__ int partner_col() const { return (partner % G) * 8; }
-  // rotates y (and the partner's yp) by the pairs' (cos, sin); DIR -1: by the opposite angle
-  template <int DIR>
-  __device__ __forceinline__ void rotate(const float2* turn, float (&y)[8], const float (&yp)[8]) const {
-    if (!turns) return;
-    if (IL) {
-      const float4 t0 = reinterpret_cast<const float4*>(turn + pair0)[0], t1 = reinterpret_cast<const float4*>(turn + pair0)[1];
-      const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y * DIR, t0.w * DIR, t1.y * DIR, t1.w * DIR};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float lo = y[2 * i], hi = y[2 * i + 1];
-        y[2 * i] = lo * c[i] - hi * s[i];
-        y[2 * i + 1] = hi * c[i] + lo * s[i];
-      }
+  __device__ __forceinline__ void store(T* row, const uint4& w) const {
+    if (PAIR != 0) {
+      *reinterpret_cast<uint4*>(row + c0) = w;
     } else {
-      const float k = sign * DIR;
+      *reinterpret_cast<uint2*>(row + c0) = make_uint2(w.x, w.y);
+      *reinterpret_cast<uint2*>(row + c1) = make_uint2(w.z, w.w);
+    }
+  }
+  // the weights of the columns (1 without weights)
+  __device__ __forceinline__ void weights(const void* w, int dtype, float (&out)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = 1.f;
+    if (!w || !in) return;
+    if (dtype == FB_DTYPE_F32) {
+      const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + c0), v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + c1);
+      out[0] = u.x; out[1] = u.y; out[2] = u.z; out[3] = u.w; out[4] = v.x; out[5] = v.y; out[6] = v.z; out[7] = v.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(w) + c0), v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(w) + c1);
+      if (dtype == FB_DTYPE_F16) unpack_chunk<__half>(make_uint4(u.x, u.y, v.x, v.y), out);
+      else unpack_chunk<__nv_bfloat16>(make_uint4(u.x, u.y, v.x, v.y), out);
+    }
+  }
+  // Coefficients of (own, partner's) value: out = a y + b y_partner, weights folded in if w; DIR -1: the opposite angle.
+  // turn: cosines of the token's pairs, sines kRopeMaxD / 2 behind.
+  template <int DIR>
+  __device__ __forceinline__ void coefficients(const fb_rope_params& p, const void* w, const float* turn, float (&a)[8], float (&b)[8]) const {
+    float wt[8];
+    weights(w, p.weight_dtype, wt);
+    if (PAIR == 0) {
+      const float4 c4 = turns ? *reinterpret_cast<const float4*>(turn + c0) : make_float4(1.f, 1.f, 1.f, 1.f);
+      const float4 s4 = turns ? *reinterpret_cast<const float4*>(turn + kRopeMaxD / 2 + c0) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 t = reinterpret_cast<const float4*>(turn + pair0)[i];
-        y[2 * i] = y[2 * i] * t.x + yp[2 * i] * (k * t.y);
-        y[2 * i + 1] = y[2 * i + 1] * t.z + yp[2 * i + 1] * (k * t.w);
+        a[i] = wt[i] * c[i];
+        a[i + 4] = wt[i + 4] * c[i];
+        b[i] = -DIR * (wt[i + 4] * s[i]);
+        b[i + 4] = DIR * (wt[i] * s[i]);
+      }
+      return;
+    }
+    const int half = p.rot >> 1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = c0 + i;
+      a[i] = wt[i];
+      b[i] = 0.f;
+      if (c < p.rot) {
+        const bool lo = PAIR == 1 ? !(i & 1) : c < half;
+        const float* t = turn + (PAIR == 1 ? c >> 1 : lo ? c : c - half);
+        const float q = PAIR == 1 ? wt[i ^ 1] : w ? load_scalar(w, p.weight_dtype, lo ? c + half : c - half) : 1.f;
+        a[i] = wt[i] * t[0];
+        b[i] = (lo ? -DIR : DIR) * (q * t[kRopeMaxD / 2]);
       }
     }
   }
+  // The partners of the values v of a row, times r: in the lane, or (PAIR 2) from the row's words in the warp's shared memory.
+  __device__ __forceinline__ void partners(const fb_rope_params& p, const uint4& raw, const float (&v)[8], float r, uint4* stage,
+                                           float (&vp)[8]) const {
+    if (PAIR < 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vp[i] = v[PAIR == 0 ? i ^ 4 : i ^ 1];
+      return;
+    }
+    const int lane = threadIdx.x & 31, half = p.rot >> 1;
+    stage[lane] = raw;
+    __syncwarp();
+    uint32_t e[4] = {};
+    if (turns && !(half & 1)) {  // both columns of a word have their partners in one word
+      const uint32_t* row = reinterpret_cast<const uint32_t*>(stage + lane - lane % G);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + 2 * i;
+        if (c < p.rot) e[i] = row[(c < half ? c + half : c - half) >> 1];
+      }
+    } else if (turns) {
+      const uint16_t* row = reinterpret_cast<const uint16_t*>(stage + lane - lane % G);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + i;
+        if (c < p.rot) e[i >> 1] |= (uint32_t)row[c < half ? c + half : c - half] << (16 * (i & 1));
+      }
+    }
+    __syncwarp();
+    unpack_chunk<T>(make_uint4(e[0], e[1], e[2], e[3]), vp);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vp[i] *= r;
+  }
 };
 
-// (cos, sin) of the tokens tok0 .. tok0 + n - 1, by all threads of the block
-__device__ __forceinline__ void rope_turns(const RopeV& a, int tok0, int n, float2 (*turn)[kRopeMaxD / 2]) {
-  const int half = a.p.rot >> 1;
-  for (int i = threadIdx.x; i < n * half; i += kRopeVThreads) {
-    const int t = i / half, pr = i - t * half, b = a.s_div.quot32(tok0 + t);
-    turn[t][pr] = rope_turn(a.p, b, tok0 + t - b * a.p.S, pr);
+// Cosines and sines of one token's pairs, by the warp, into its shared memory.
+__device__ __forceinline__ void rope_turns(const fb_rope_params& p, int b, int s, float* turn) {
+  __syncwarp();
+  for (int pr = threadIdx.x & 31; pr < p.rot >> 1; pr += 32) {
+    const float2 t = rope_turn(p, b, s, pr);
+    turn[pr] = t.x;
+    turn[kRopeMaxD / 2 + pr] = t.y;
   }
+  __syncwarp();
 }
 
-template <typename T, int G, bool IL, bool APPEND>
-__global__ void __launch_bounds__(kRopeVThreads) rope_vector_kernel(const __grid_constant__ RopeV a) {
-  constexpr int ROWS = kRopeVThreads / G;  // side by side
-  __shared__ __align__(16) float2 turn[kRopeMaxTokens][kRopeMaxD / 2];
-  __shared__ int64_t s_page[kRopeMaxTokens];
-  __shared__ int s_place[kRopeMaxTokens];
+template <typename T, int G, int PAIR, bool FULL, bool APPEND>
+__global__ void __launch_bounds__(kRopeVThreads, 6) rope_vector_kernel(const __grid_constant__ RopeV a) {
+  constexpr int SIDE = 32 / G, U = 4;
+  __shared__ __align__(16) float turns[kRopeVWarps][kRopeMaxD];
+  __shared__ uint4 stages[kRopeVWarps][PAIR == 2 ? 32 : 1];
   const fb_rope_params& p = a.p;
-  const RopeLane<G, IL> me(p);
-  const int slot = threadIdx.x / G, tok0 = blockIdx.x * a.run, ntok = min(a.run, a.tokens - tok0);
-  if (APPEND && threadIdx.x < ntok) {
-    int64_t page = -1;
-    int place = 0;
-    if (!cache_place(p, tok0 + threadIdx.x, page, place)) page = -1;
-    s_page[threadIdx.x] = page;
-    s_place[threadIdx.x] = place;
-  }
-  rope_turns(a, tok0, ntok, turn);
-  __syncthreads();
+  const RopeLane<T, G, PAIR, FULL> me(p);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t gw = (int64_t)blockIdx.x * kRopeVWarps + warp;
+  const int tok = (int)(gw / a.split), sub = (int)(gw - (int64_t)tok * a.split);
+  if (tok >= a.tokens) return;
+  const int b = a.s_div.quot32(tok), s = tok - b * p.S;
+  int64_t page = 0;
+  int place = 0;
+  const bool cached = APPEND && cache_place(p, s, page, place);
+  rope_turns(p, b, s, turns[warp]);
+  const float inv_d = 1.f / p.D;
 
   // TENSOR 0: q, 1: k, 2: v (copied)
   auto rows_of = [&](auto tensor) {
     constexpr int X = decltype(tensor)::value;
-    const int H = X == 0 ? p.Hq : p.Hk, rows = ntok * H;
-    const Div& div = X == 0 ? a.hq_div : a.hk_div;
+    const int H = X == 0 ? p.Hq : p.Hk;
+    const int h0 = sub * SIDE + lane / G, step = a.split * SIDE;
+    if (sub * SIDE >= H) return;
     const int64_t* xs = X == 0 ? p.q_stride : X == 1 ? p.k_stride : p.v_stride;
-    const T* x = reinterpret_cast<const T*>(X == 0 ? p.q : X == 1 ? p.k : p.v);
-    const void* w = X == 0 ? p.q_weight : X == 1 ? p.k_weight : nullptr;
-    float wt[8], wp[8];
-    if (X < 2) {
-      me.weights(w, p.weight_dtype, me.col, wt);
-      me.weights(w, p.weight_dtype, me.partner_col(), wp);
+    const T* x = reinterpret_cast<const T*>(X == 0 ? p.q : X == 1 ? p.k : p.v) + b * xs[0] + s * xs[2] + h0 * xs[1];
+    const int64_t* os = X == 0 ? p.q_out_stride : p.k_out_stride;
+    T* y = reinterpret_cast<T*>(X == 0 ? p.q_out : p.k_out) + b * os[0] + s * os[2];
+    int64_t yh = os[1];
+    if (APPEND && X > 0) {
+      const int64_t* cs = X == 1 ? p.key_cache_stride : p.value_cache_stride;
+      y = reinterpret_cast<T*>(X == 1 ? p.key_cache : p.value_cache) + page * cs[0] + place * cs[1];
+      yh = cs[2];
     }
-    for (int r0 = 0; r0 < rows; r0 += ROWS * kRopeUnroll) {
-      uint4 raw[kRopeUnroll];
-      T* dst[kRopeUnroll];
-      int tk[kRopeUnroll];
+    y += h0 * yh;
+    const int64_t xstep = step * xs[1], ystep = step * yh;
+    const void* w = X == 0 ? p.q_weight : X == 1 ? p.k_weight : nullptr;
+    const bool touched = FULL || w || me.turns;  // (untouched values keep their bits)
+    float ca[8], cb[8];
+    const T* const x0 = x - (lane / G) * xs[1];  // (the warp's first row exists)
+    auto load = [&](uint4& raw, const T* src, bool live) {
+      raw = me.load(live ? src : x0);
+      if ((!FULL && !me.in) || !live) raw = make_uint4(0u, 0u, 0u, 0u);
+    };
+    auto finish = [&](const uint4& raw, T* dst, bool live) {
+      uint4 out = raw;
+      if (X < 2) {
+        float v[8], vp[8], rr = 1.f;
+        unpack_chunk<T>(raw, v);
+        if (w) {
+          float q = 0.f;
 #pragma unroll
-      for (int u = 0; u < kRopeUnroll; ++u) {
-        const int r = r0 + u * ROWS + slot;
-        dst[u] = nullptr;
-        raw[u] = make_uint4(0u, 0u, 0u, 0u);
-        tk[u] = 0;
-        if (r < rows && me.in) {
-          const int t = div.quot32(r), h = r - t * H, tok = tok0 + t, b = a.s_div.quot32(tok), s = tok - b * p.S;
-          tk[u] = t;
-          if (APPEND && X > 0) {
-            if (s_page[t] >= 0) {
-              const int64_t* cs = X == 1 ? p.key_cache_stride : p.value_cache_stride;
-              dst[u] = reinterpret_cast<T*>(X == 1 ? p.key_cache : p.value_cache) + s_page[t] * cs[0] + s_place[t] * cs[1] + h * cs[2] + me.col;
-            }
-          } else {
-            const int64_t* os = X == 0 ? p.q_out_stride : p.k_out_stride;
-            dst[u] = reinterpret_cast<T*>(X == 0 ? p.q_out : p.k_out) + b * os[0] + h * os[1] + s * os[2] + me.col;
-          }
-          if (dst[u]) raw[u] = __ldcs(reinterpret_cast<const uint4*>(x + b * xs[0] + h * xs[1] + s * xs[2] + me.col));
+          for (int i = 0; i < 8; ++i) q = fmaf(v[i], v[i], q);
+          rr = rsqrtf(fmaf(group_sum<G>(q), inv_d, p.eps));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] *= rr;
         }
-      }
+        if (FULL || p.rot) me.partners(p, raw, v, rr, stages[warp], vp);
 #pragma unroll
-      for (int u = 0; u < kRopeUnroll; ++u) {
-        uint4 out = raw[u];
-        if (X < 2) {
-          float y[8], yp[8];
-          unpack_chunk<T>(raw[u], y);
-          float rr = 1.f;
-          if (w) {
-            float ss = 0.f;
+        for (int i = 0; i < 8; ++i) v[i] *= ca[i];
+        if (me.turns) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
-            rr = rsqrtf(group_sum<G>(ss) / p.D + p.eps);
-          }
-          if (!IL && p.rot) unpack_chunk<T>(shfl_chunk(raw[u], me.partner), yp);
-          if (w) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              y[i] = y[i] * rr * wt[i];
-              if (!IL) yp[i] = yp[i] * rr * wp[i];
-            }
-          }
-          me.template rotate<1>(turn[tk[u]], y, yp);
-          if (w || me.turns) out = pack_chunk<T>(y);  // (untouched values keep their bits)
+          for (int i = 0; i < 8; ++i) v[i] = fmaf(vp[i], cb[i], v[i]);
         }
-        if (dst[u]) *reinterpret_cast<uint4*>(dst[u]) = out;
+        if (touched) out = pack_chunk<T>(v);
       }
+      if (live && me.in) me.store(dst, out);
+    };
+    int h = sub * SIDE;  // (of the warp's first row; the same in all lanes)
+    uint4 raw[U];
+    auto load_rows = [&](auto count) {
+#pragma unroll
+      for (int u = 0; u < decltype(count)::value; ++u) load(raw[u], x + u * xstep, true);
+    };
+    auto finish_rows = [&](auto count) {
+      constexpr int N = decltype(count)::value;
+      x += N * xstep;
+#pragma unroll
+      for (int u = 0; u < N; ++u) finish(raw[u], y + u * ystep, true);
+      y += N * ystep;
+      h += N * step;
+    };
+    const std::integral_constant<int, U> many;
+    const std::integral_constant<int, U / 2> some;
+    const bool whole = h + (U - 1) * step + SIDE <= H;
+    if (whole) load_rows(many);
+    if (X < 2) me.template coefficients<1>(p, w, turns[warp], ca, cb);  // under the first loads
+    if (whole) {
+      finish_rows(many);
+      while (h + (U - 1) * step + SIDE <= H) {
+        load_rows(many);
+        finish_rows(many);
+      }
+    }
+    if (h + (U / 2 - 1) * step + SIDE <= H) {
+      load_rows(some);
+      finish_rows(some);
+    }
+#pragma unroll 1
+    for (; h < H; h += step, x += xstep, y += ystep) {
+      const bool live = h + lane / G < H;
+      load(raw[0], x, live);
+      finish(raw[0], y, live);
     }
   };
   rows_of(std::integral_constant<int, 0>());
+  if (APPEND && !cached) return;
   rows_of(std::integral_constant<int, 1>());
   if constexpr (APPEND) {
     rows_of(std::integral_constant<int, 2>());
-    const int per = p.bias_heads * p.R;
-    for (int i = threadIdx.x; i < ntok * per; i += kRopeVThreads) {
-      const int t = i / per, h = (i - t * per) / p.R, c = i - t * per - h * p.R;
-      if (s_page[t] < 0) continue;
-      reinterpret_cast<T*>(p.bias_cache)[s_page[t] * p.bias_cache_stride[0] + s_place[t] * p.bias_cache_stride[1] + h * p.bias_cache_stride[2] + c] =
-          reinterpret_cast<const T*>(p.k_bias)[h * p.k_bias_stride[1] + (tok0 + t) * p.k_bias_stride[2] + c];
+    for (int i = sub * 32 + lane; i < p.bias_heads * p.R; i += a.split * 32) {
+      const int h = i / p.R, c = i - h * p.R;
+      reinterpret_cast<T*>(p.bias_cache)[page * p.bias_cache_stride[0] + place * p.bias_cache_stride[1] + h * p.bias_cache_stride[2] + c] =
+          reinterpret_cast<const T*>(p.k_bias)[h * p.k_bias_stride[1] + s * p.k_bias_stride[2] + c];
     }
   }
 }
 
-template <typename T, int G, bool IL>
-__global__ void __launch_bounds__(kRopeVThreads) rope_bwd_vector_kernel(const __grid_constant__ RopeV a) {
-  constexpr int ROWS = kRopeVThreads / G;
-  __shared__ __align__(16) float2 turn[kRopeMaxTokens][kRopeMaxD / 2];
-  __shared__ float sums[ROWS][G * 8 + 1];
+// A block takes rows of one tensor, so that a lane keeps one set of weight sums: the first a.q_ctas blocks take q.
+template <typename T, int G, int PAIR, bool FULL>
+__global__ void __launch_bounds__(kRopeVThreads, 5) rope_bwd_vector_kernel(const __grid_constant__ RopeV a) {
+  constexpr int SIDE = 32 / G, U = 2;
+  __shared__ __align__(16) float turns[kRopeVWarps][kRopeMaxD];
+  __shared__ uint4 stages[kRopeVWarps][PAIR == 2 ? 32 : 1];
+  __shared__ float sums[kRopeVWarps * SIDE][G * 8 + 1];
   const fb_rope_params& p = a.p;
-  const RopeLane<G, IL> me(p);
-  const int slot = threadIdx.x / G;
-  float dw[2][8] = {};
-  for (int tok0 = blockIdx.x * a.run; tok0 < a.tokens; tok0 += gridDim.x * a.run) {
-    const int ntok = min(a.run, a.tokens - tok0);
-    __syncthreads();
-    rope_turns(a, tok0, ntok, turn);
-    __syncthreads();
-    auto rows_of = [&](auto tensor) {
-      constexpr int X = decltype(tensor)::value;
-      const int H = X == 0 ? p.Hq : p.Hk, rows = ntok * H;
-      const Div& div = X == 0 ? a.hq_div : a.hk_div;
-      const int64_t *xs = X == 0 ? p.q_stride : p.k_stride, *gs = X == 0 ? p.dq_out_stride : p.dk_out_stride,
-                    *ds = X == 0 ? p.dq_stride : p.dk_stride;
-      const void* w = X == 0 ? p.q_weight : p.k_weight;
-      float wt[8];
-      me.weights(w, p.weight_dtype, me.col, wt);
-      for (int r0 = 0; r0 < rows; r0 += ROWS * kRopeUnroll) {
-        uint4 xr[kRopeUnroll], gr[kRopeUnroll];
-        T* dst[kRopeUnroll];
-        int tk[kRopeUnroll];
+  const RopeLane<T, G, PAIR, FULL> me(p);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool is_q = (int)blockIdx.x < a.q_ctas;
+  const int block = is_q ? blockIdx.x : blockIdx.x - a.q_ctas, blocks = is_q ? a.q_ctas : gridDim.x - a.q_ctas;
+  const int H = is_q ? p.Hq : p.Hk;
+  const int64_t *xs = is_q ? p.q_stride : p.k_stride, *gs = is_q ? p.dq_out_stride : p.dk_out_stride, *ds = is_q ? p.dq_stride : p.dk_stride;
+  const T* x0 = reinterpret_cast<const T*>(is_q ? p.q : p.k);
+  const T* g0 = reinterpret_cast<const T*>(is_q ? p.dq_out : p.dk_out);
+  T* d0 = reinterpret_cast<T*>(is_q ? p.dq : p.dk);
+  const void* w = is_q ? p.q_weight : p.k_weight;
+  const bool touched = FULL || w || me.turns;
+  float dw[8] = {}, wt[8];
+  me.weights(w, p.weight_dtype, wt);
+  const float inv_d = 1.f / p.D;
+  const int64_t nwarps = (int64_t)a.tokens * a.split;
+  for (int64_t gw = (int64_t)block * kRopeVWarps + warp; gw < nwarps; gw += (int64_t)blocks * kRopeVWarps) {
+    const int tok = (int)(gw / a.split), sub = (int)(gw - (int64_t)tok * a.split);
+    const int h0 = sub * SIDE + lane / G, step = a.split * SIDE;
+    if (sub * SIDE >= H) continue;
+    const int b = a.s_div.quot32(tok), s = tok - b * p.S;
+    const T* x = x0 + b * xs[0] + s * xs[2] + h0 * xs[1];
+    const T* g = g0 + b * gs[0] + s * gs[2] + h0 * gs[1];
+    T* d = d0 + b * ds[0] + s * ds[2] + h0 * ds[1];
+    const int64_t xstep = step * xs[1], gstep = step * gs[1], dstep = step * ds[1];
+    float ca[8], cb[8];
+    uint4 xr[U], gr[U];
+    const T *const gfirst = g - (lane / G) * gs[1], *const xfirst = x - (lane / G) * xs[1];  // (the warp's first row exists)
+    auto load = [&](int u, const T* gsrc, const T* xsrc, bool live) {
+      gr[u] = me.load(live ? gsrc : gfirst);
+      if (w) xr[u] = me.load(live ? xsrc : xfirst);
+      if ((!FULL && !me.in) || !live) xr[u] = gr[u] = make_uint4(0u, 0u, 0u, 0u);
+    };
+    auto finish = [&](int u, T* dst, bool live) {
+      uint4 out = gr[u];
+      float v[8], vp[8];
+      unpack_chunk<T>(gr[u], v);
+      if (FULL || p.rot) me.partners(p, gr[u], v, 1.f, stages[warp], vp);
+      if (me.turns) {
 #pragma unroll
-        for (int u = 0; u < kRopeUnroll; ++u) {
-          const int r = r0 + u * ROWS + slot;
-          dst[u] = nullptr;
-          tk[u] = 0;
-          xr[u] = gr[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (r < rows && me.in) {
-            const int t = div.quot32(r), h = r - t * H, tok = tok0 + t, b = a.s_div.quot32(tok), s = tok - b * p.S;
-            tk[u] = t;
-            gr[u] = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(X == 0 ? p.dq_out : p.dk_out) + b * gs[0] + h * gs[1] + s * gs[2] + me.col));
-            if (w) xr[u] = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(X == 0 ? p.q : p.k) + b * xs[0] + h * xs[1] + s * xs[2] + me.col));
-            dst[u] = reinterpret_cast<T*>(X == 0 ? p.dq : p.dk) + b * ds[0] + h * ds[1] + s * ds[2] + me.col;
-          }
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(vp[i], cb[i], v[i] * ca[i]);
+      }
+      if (w) {
+        float x8[8], q = 0.f, t = 0.f;
+        unpack_chunk<T>(xr[u], x8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          q = fmaf(x8[i], x8[i], q);
+          t = fmaf(v[i] * wt[i], x8[i], t);
         }
+        const float rr = rsqrtf(fmaf(group_sum<G>(q), inv_d, p.eps)), k = -rr * (rr * (group_sum<G>(t) * inv_d));
 #pragma unroll
-        for (int u = 0; u < kRopeUnroll; ++u) {
-          float g[8], gp[8];
-          uint4 out = gr[u];
-          unpack_chunk<T>(gr[u], g);
-          if (!IL && p.rot) unpack_chunk<T>(shfl_chunk(gr[u], me.partner), gp);
-          me.template rotate<-1>(turn[tk[u]], g, gp);
-          if (w) {
-            float x[8], ss = 0.f, sg = 0.f;
-            unpack_chunk<T>(xr[u], x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              ss = fmaf(x[i], x[i], ss);
-              sg = fmaf(x[i] * g[i], wt[i], sg);
-            }
-            const float rr = rsqrtf(group_sum<G>(ss) / p.D + p.eps), mean = rr * (group_sum<G>(sg) / p.D);
-            if (dst[u]) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float xn = x[i] * rr;
-                dw[X][i] = fmaf(g[i], xn, dw[X][i]);
-                g[i] = rr * (wt[i] * g[i] - xn * mean);
-              }
-            }
-          }
-          if (w || me.turns) out = pack_chunk<T>(g);
-          if (dst[u]) *reinterpret_cast<uint4*>(dst[u]) = out;
+        for (int i = 0; i < 8; ++i) {
+          const float xn = x8[i] * rr;
+          dw[i] = fmaf(v[i], xn, dw[i]);
+          v[i] = fmaf(xn, k, v[i] * (wt[i] * rr));
         }
       }
+      if (touched) out = pack_chunk<T>(v);
+      if (live && me.in) me.store(dst, out);
     };
-    rows_of(std::integral_constant<int, 0>());
-    rows_of(std::integral_constant<int, 1>());
+    int h = sub * SIDE;  // (of the warp's first row; the same in all lanes)
+    if (h + (U - 1) * step + SIDE <= H) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) load(u, g + u * gstep, x + u * xstep, true);
+    }
+    rope_turns(p, b, s, turns[warp]);  // under the first loads
+    me.template coefficients<-1>(p, nullptr, turns[warp], ca, cb);
+    for (bool first = true; h + (U - 1) * step + SIDE <= H; h += U * step, first = false) {
+      if (!first) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(u, g + u * gstep, x + u * xstep, true);
+      }
+      g += U * gstep;
+      x += U * xstep;
+#pragma unroll
+      for (int u = 0; u < U; ++u) finish(u, d + u * dstep, true);
+      d += U * dstep;
+    }
+#pragma unroll 1
+    for (; h < H; h += step, g += gstep, x += xstep, d += dstep) {
+      const bool live = h + lane / G < H;
+      load(0, g, x, live);
+      finish(0, d, live);
+    }
   }
   if (!p.workspace) return;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sums[slot][me.col + i] = dw[t][i];
-    __syncthreads();
-    for (int c = threadIdx.x; c < p.D; c += kRopeVThreads) {
-      float v = 0.f;
-      for (int r = 0; r < ROWS; ++r) v += sums[r][c];
-      reinterpret_cast<float*>(p.workspace)[((int64_t)blockIdx.x * 2 + t) * p.D + c] = v;
-    }
+  for (int i = 0; i < 8; ++i)
+    if (me.in) sums[warp * SIDE + lane / G][i < 4 ? me.c0 + i : me.c1 + i - 4] = dw[i];
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.D; c += kRopeVThreads) {
+    float v = 0.f;
+#pragma unroll 4
+    for (int r = 0; r < kRopeVWarps * SIDE; ++r) v += sums[r][c];
+    reinterpret_cast<float*>(p.workspace)[(int64_t)blockIdx.x * p.D + c] = v;
   }
 }
 
@@ -529,23 +657,40 @@ int sm_count() {
   return n > 0 ? n : 148;
 }
 
-// Tokens of a block at a time: enough blocks for four on every SM first, then longer runs.
-int rope_run(const fb_rope_params* p) {
-  const int64_t run = (int64_t)p->B * p->S / (4ll * sm_count());
-  return run < 1 ? 1 : run > kRopeMaxTokens ? kRopeMaxTokens : (int)run;
+// Warps of a token: few tokens are spread over more warps, up to two rows for a lane.  A share has its own angles and
+// coefficients to take, five rows' worth, so no more shares than make two full GPUs.
+int rope_split(const fb_rope_params* p) {
+  const int G = p->D <= 8 ? 1 : p->D <= 16 ? 2 : p->D <= 32 ? 4 : p->D <= 64 ? 8 : 16, H = p->Hq > p->Hk ? p->Hq : p->Hk;
+  const int64_t tokens = (int64_t)p->B * p->S, want = 48ll * sm_count();
+  int split = 1;
+  while (split * 2 * (32 / G) <= H && tokens * split < want) split *= 2;
+  return split;
 }
-int rope_bwd_ctas(const fb_rope_params* p, bool vector) {
-  const int run = vector ? rope_run(p) : 1;
-  const int64_t most = (vector ? 4ll : 8ll) * sm_count(), runs = ((int64_t)p->B * p->S + run - 1) / run;
-  return (int)(runs < most ? runs : most);
+// Blocks of the backward; vector kernels: those of q, then those of k, each by its share of the rows.
+struct BwdGrid {
+  int q, all;
+};
+BwdGrid rope_bwd_grid(const fb_rope_params* p, bool vector) {
+  const int64_t tokens = (int64_t)p->B * p->S;
+  if (!vector) {
+    const int64_t most = 8ll * sm_count();
+    return {0, (int)(tokens < most ? tokens : most)};
+  }
+  const int64_t most = 5ll * sm_count(), each = (tokens * rope_split(p) + kRopeVWarps - 1) / kRopeVWarps;
+  int64_t q = most * p->Hq / (p->Hq + p->Hk), k;
+  q = !p->Hq ? 0 : q < 1 ? 1 : !p->Hk ? most : q > most - 1 ? most - 1 : q;
+  k = p->Hk ? most - q : 0;
+  if (q > each) q = each;
+  if (k > each) k = each;
+  return {(int)q, (int)(q + k)};
 }
 bool wants_weights(const fb_rope_params* p) { return p->dq_weight || p->dk_weight; }
 
 enum { ROPE_FORWARD, ROPE_BACKWARD, ROPE_APPEND };
-// Rows of whole aligned chunks of 16 bytes in everything that the call touches, pairs inside a chunk or whole chunks apart.
+// Rows of whole aligned chunks of 16 bytes in everything that the call touches.
 bool rope_vector(const fb_rope_params* p, int what) {
-  if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 8 || p->rot % (p->interleaved ? 8 : 16)) return false;
-  uintptr_t bits = 0;
+  if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 8) return false;
+  uintptr_t bits = reinterpret_cast<uintptr_t>(p->q_weight) | reinterpret_cast<uintptr_t>(p->k_weight);
   auto add = [&](const void* ptr, const int64_t (&s)[3], bool used) {
     if (!used) return;
     bits |= reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(s[0] | s[1] | s[2]) * 2;
@@ -568,16 +713,21 @@ bool rope_vector(const fb_rope_params* p, int what) {
   return !(bits & 15);
 }
 
-template <typename T, int G, bool IL>
+template <typename T, int G, int PAIR, bool FULL>
 void launch_rope_v(const RopeV& a, int what, unsigned grid, cudaStream_t st) {
-  if (what == ROPE_FORWARD) rope_vector_kernel<T, G, IL, false><<<grid, kRopeVThreads, 0, st>>>(a);
-  else if (what == ROPE_APPEND) rope_vector_kernel<T, G, IL, true><<<grid, kRopeVThreads, 0, st>>>(a);
-  else rope_bwd_vector_kernel<T, G, IL><<<grid, kRopeVThreads, 0, st>>>(a);
+  if (what == ROPE_FORWARD) rope_vector_kernel<T, G, PAIR, FULL, false><<<grid, kRopeVThreads, 0, st>>>(a);
+  else if (what == ROPE_APPEND) rope_vector_kernel<T, G, PAIR, FULL, true><<<grid, kRopeVThreads, 0, st>>>(a);
+  else rope_bwd_vector_kernel<T, G, PAIR, FULL><<<grid, kRopeVThreads, 0, st>>>(a);
 }
 template <typename T, int G>
 void launch_rope_g(const RopeV& a, int what, unsigned grid, cudaStream_t st) {
-  if (a.p.interleaved) launch_rope_v<T, G, true>(a, what, grid, st);
-  else launch_rope_v<T, G, false>(a, what, grid, st);
+  if constexpr (G >= 8) {
+    if (a.p.D == 8 * G && a.p.rot == a.p.D)
+      return a.p.interleaved ? launch_rope_v<T, G, 1, true>(a, what, grid, st) : launch_rope_v<T, G, 0, true>(a, what, grid, st);
+  }
+  if (a.p.interleaved) launch_rope_v<T, G, 1, false>(a, what, grid, st);
+  else if (a.p.rot % 8 == 0) launch_rope_v<T, G, 0, false>(a, what, grid, st);
+  else launch_rope_v<T, G, 2, false>(a, what, grid, st);
 }
 template <typename T>
 void launch_rope_t(const RopeV& a, int what, unsigned grid, cudaStream_t st) {
@@ -591,11 +741,11 @@ void launch_rope_vector(const fb_rope_params& p, int what, cudaStream_t st) {
   RopeV a = {};
   a.p = p;
   a.s_div = Div(p.S);
-  a.hq_div = Div(p.Hq > 0 ? p.Hq : 1);
-  a.hk_div = Div(p.Hk > 0 ? p.Hk : 1);
   a.tokens = p.B * p.S;
-  a.run = rope_run(&p);
-  const unsigned grid = what == ROPE_BACKWARD ? (unsigned)rope_bwd_ctas(&p, true) : (unsigned)((a.tokens + (int64_t)a.run - 1) / a.run);
+  a.split = rope_split(&p);
+  const BwdGrid bwd = rope_bwd_grid(&p, true);
+  a.q_ctas = bwd.q;
+  const unsigned grid = what == ROPE_BACKWARD ? (unsigned)bwd.all : (unsigned)(((int64_t)a.tokens * a.split + kRopeVWarps - 1) / kRopeVWarps);
   if (p.dtype == FB_DTYPE_F16) launch_rope_t<__half>(a, what, grid, st);
   else launch_rope_t<__nv_bfloat16>(a, what, grid, st);
   note_launch();
@@ -626,7 +776,7 @@ extern "C" int fb_norm_rope(const fb_rope_params* p, void* cuda_stream) {
 
 extern "C" size_t fb_norm_rope_bwd_workspace_bytes(const fb_rope_params* p) {
   if (validate_rope(p) || !wants_weights(p)) return 0;
-  return round256((size_t)rope_bwd_ctas(p, rope_vector(p, ROPE_BACKWARD)) * 2 * p->D * 4);
+  return round256((size_t)rope_bwd_grid(p, rope_vector(p, ROPE_BACKWARD)).all * 2 * p->D * 4);
 }
 
 extern "C" int fb_norm_rope_bwd(const fb_rope_params* p, void* cuda_stream) {
@@ -640,7 +790,8 @@ extern "C" int fb_norm_rope_bwd(const fb_rope_params* p, void* cuda_stream) {
   if (!need) a.workspace = nullptr;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   const bool vector = rope_vector(p, ROPE_BACKWARD);
-  const int ctas = rope_bwd_ctas(p, vector);
+  const BwdGrid grid = rope_bwd_grid(p, vector);
+  const int ctas = grid.all;
   const int64_t tokens = (int64_t)p->B * p->S;
   if (vector) {
     launch_rope_vector(a, ROPE_BACKWARD, st);
@@ -650,7 +801,8 @@ extern "C" int fb_norm_rope_bwd(const fb_rope_params* p, void* cuda_stream) {
     note_launch();
   }
   if (need) {
-    rope_weight_kernel<<<dim3((p->D + 31) / 32, 2), dim3(32, 32), 0, st>>>(a, ctas);
+    const WeightParts parts = vector ? WeightParts{{grid.q, ctas - grid.q}, (int64_t)grid.q * p->D, p->D} : WeightParts{{ctas, ctas}, p->D, 2 * p->D};
+    rope_weight_kernel<<<dim3((p->D + 31) / 32, 2), dim3(32, 32), 0, st>>>(a, parts);
     note_launch();
   }
   return (int)cudaGetLastError();

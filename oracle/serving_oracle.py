@@ -41,9 +41,16 @@ def norm_rope(x, weight=None, angles=None, interleaved=False, eps=1e-6):
 
 
 def norm_rope_grads(x, dout, weight=None, angles=None, interleaved=False, eps=1e-6):
-    """(dx, dw, size of the terms of dx, sum of the magnitudes that make up dw): the last two scale a rounding bound."""
+    """(dx, dw, size of the terms of dx, sum of the magnitudes that make up dw): the last two scale a rounding bound.  A
+    rotated gradient g_lo c + g_hi s may cancel, and each product carries a rounding of its own and that of its cosine or
+    sine: its error is a multiple of 2^-24 (|g_lo| + |g_hi|), which is what counts in the second."""
     x, g = x.detach().double().cpu(), dout.detach().double().cpu()
+    mag = g.abs()
     if angles is not None:
+        half = angles.shape[-1]
+        for i in range(half):
+            lo, hi = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+            mag[..., lo] = mag[..., hi] = g[..., lo].abs() + g[..., hi].abs()
         g = rotate(g, -angles, interleaved)
     if weight is None:
         return g, None, g.abs(), None
@@ -51,8 +58,7 @@ def norm_rope_grads(x, dout, weight=None, angles=None, interleaved=False, eps=1e
     r = torch.rsqrt((x * x).mean(-1, keepdim=True) + eps)
     dx = r * (w * g - x * r ** 2 * (w * g * x).mean(-1, keepdim=True))
     size = r * ((w * g).abs() + x.abs() * r ** 2 * (w * g * x).abs().mean(-1, keepdim=True))
-    each = (g * x * r).flatten(0, -2)
-    return dx, each.sum(0), size, each.abs().sum(0)
+    return dx, (g * x * r).flatten(0, -2).sum(0), size, (mag * (x * r).abs()).flatten(0, -2).sum(0)
 
 
 # ---- the plan of a step ------------------------------------------------------------------------------------------
