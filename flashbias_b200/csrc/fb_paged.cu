@@ -144,17 +144,31 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
   }
   const int G = p->Hq / p->Hk;
   if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 8 || (bits & 15) || (int64_t)p->N * G > 0x7fffffffLL) return plan;
-  plan.kernel = 1;
-  plan.TD = p->D <= 32 ? 32 : p->D <= 64 ? 64 : 128;
   const int64_t rows = ((int64_t)p->N * G + p->B - 1) / p->B;  // per request on average
-  plan.MT = rows <= 16 ? 16 : 32;
   int dev = 0;
   cudaGetDevice(&dev);
-  plan.ctas = 2 * (device_sm_count(dev) > 0 ? device_sm_count(dev) : 148);
-  // The heads of a group are read side by side, whole rows of the cache; where the longest requests that the table can hold do
-  // not fill the GPU that way, one head is spread over the CTA's warps.
-  const int64_t tiles = (int64_t)p->B * (((int64_t)p->table_width * p->page_size + 63) / 64) * p->Hk;
-  plan.WH = p->Hk % 4 == 0 && tiles / 4 >= 4 * plan.ctas ? 4 : p->Hk % 2 == 0 && tiles / 2 >= 4 * plan.ctas ? 2 : 1;
+  const int sms = device_sm_count(dev) > 0 ? device_sm_count(dev) : 148;
+  // More rows than the split kernel holds side by side: 128 of them in a tcgen05 tile, if a tile of 128 keys is made of whole
+  // pages (or a page of whole tiles) that TMA can address, and the scale may be taken out of a maximum.
+  const bool tma = tma_compatible(p->key_cache, p->key_cache_stride[1], p->key_cache_stride[2], p->key_cache_stride[0], p->Hk, p->num_pages) &&
+                   tma_compatible(p->value_cache, p->value_cache_stride[1], p->value_cache_stride[2], p->value_cache_stride[0], p->Hk, p->num_pages);
+  if (rows > 32 && tma && p->R == 0 && p->softmax_scale > 0.f && p->page_size % 8 == 0 && (128 % p->page_size == 0 || p->page_size % 128 == 0) &&
+      p->num_pages < 0x7fffffffLL) {
+    plan.kernel = PAGED_TILE;
+    plan.TD = p->D <= 64 ? 64 : 128;
+    plan.MT = 128;
+    plan.WH = 1;
+    plan.ctas = sms;
+  } else {
+    plan.kernel = PAGED_SPLIT;
+    plan.TD = p->D <= 32 ? 32 : p->D <= 64 ? 64 : 128;
+    plan.MT = rows <= 16 ? 16 : 32;
+    plan.ctas = 2 * sms;
+    // The heads of a group are read side by side, whole rows of the cache; where the longest requests that the table can hold do
+    // not fill the GPU that way, one head is spread over the CTA's warps.
+    const int64_t tiles = (int64_t)p->B * (((int64_t)p->table_width * p->page_size + 63) / 64) * p->Hk;
+    plan.WH = p->Hk % 4 == 0 && tiles / 4 >= 4 * plan.ctas ? 4 : p->Hk % 2 == 0 && tiles / 2 >= 4 * plan.ctas ? 2 : 1;
+  }
   const size_t prows = (size_t)plan.ctas * 2 * plan.WH * plan.MT;
   plan.part_bytes = round256(prows * plan.TD * 4);
   plan.ml_bytes = round256(prows * 8);
@@ -178,7 +192,7 @@ extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
   if (const int rc = validate_paged(p)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   const PagedPlan plan = plan_paged(p);
-  if (plan.kernel == 1) {
+  if (plan.kernel != PAGED_GENERAL) {
     const size_t need = plan.part_bytes + plan.ml_bytes + plan.desc_bytes;
     if (!p->workspace || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255)) return FB_EINVAL_WORKSPACE;
     PagedArgs a = {};
@@ -191,6 +205,7 @@ extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
     a.part = reinterpret_cast<float*>(ws);
     a.ml = reinterpret_cast<float2*>(ws + plan.part_bytes);
     a.desc = reinterpret_cast<int4*>(ws + plan.part_bytes + plan.ml_bytes);
+    if (plan.kernel == PAGED_TILE) return plan.TD == 64 ? launch_paged_tile_d64(a, plan, st) : launch_paged_tile_d128(a, plan, st);
     return plan.TD == 32 ? launch_paged_split_d32(a, plan, st) : plan.TD == 64 ? launch_paged_split_d64(a, plan, st) : launch_paged_split_d128(a, plan, st);
   }
   const unsigned grid = (unsigned)(p->N * p->Hq);

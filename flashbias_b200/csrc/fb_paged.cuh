@@ -161,16 +161,80 @@ __device__ __forceinline__ bool tree_sees(const fb_paged_params& p, int n, int t
   return w < p.mask_words && ((p.tree_mask[n * p.mask_stride + w] >> (td & 63)) & 1);
 }
 
-// ---- host side (fb_paged.cu, fb_paged_split_*.cu) ------------------------------------------------------------------
+// ---- host side (fb_paged.cu, fb_paged_split_*.cu, fb_paged_tile_*.cu) ------------------------------------------------
+enum { PAGED_GENERAL, PAGED_SPLIT, PAGED_TILE };
 struct PagedPlan {
-  int kernel;   // 0: general, 1: split
-  int TD, MT;   // columns and rows of a tile
-  int WH;       // key heads of a group
+  int kernel;  // PAGED_*
+  int TD, MT;  // columns and rows of a tile
+  int WH;      // key heads of a group
   int ctas;
   size_t part_bytes, ml_bytes, desc_bytes;
 };
 int launch_paged_split_d32(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
 int launch_paged_split_d64(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
 int launch_paged_split_d128(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
+int launch_paged_tile_d64(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
+int launch_paged_tile_d128(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
+
+// Joins the parts of the item that begins in CTA blockIdx.x; a warp per row, the parts in the order of the CTAs.
+constexpr int kJoinRows = 16;  // of a block
+template <typename T, int TD>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a, const int WH, const int MT) {
+  constexpr int C = TD / 32;  // columns of a lane
+  grid_dep_wait();
+  const int4 d = a.desc[blockIdx.x];
+  if (d.x < 0) return;
+  const fb_paged_params& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const Request rq = request_at(p, d.x);
+  for (int idx = blockIdx.y * kJoinRows + (threadIdx.x >> 5); idx < (blockIdx.y + 1) * kJoinRows; idx += 4) {
+    const int wh = idx / MT, r = idx - wh * MT, gr = d.y * MT + r;
+    if (gr >= rq.tokens * a.G) continue;
+    const int t = a.group_div.quot32(gr), h = (d.z * WH + wh) * a.G + gr - t * a.G, n = rq.first + t;
+    const int64_t step = (int64_t)2 * WH * MT;  // rows of a CTA
+    const int64_t row0 = blockIdx.x * step + (int64_t)(WH + wh) * MT + r, row1 = (int64_t)(blockIdx.x + 1) * step + (int64_t)wh * MT + r;
+    const int parts = d.w - (int)blockIdx.x + 1;
+    auto row_of = [&](int i) { return i == 0 ? row0 : row1 + (i - 1) * step; };
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, a.ml[row_of(i)].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ms = fmaxf(m, -FLT_MAX);
+    float l = 0.f, acc[C] = {};
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const int64_t row = row_of(i);
+      const float2 s = a.ml[row];
+      const float f = fast_exp2(s.x - ms);
+      l = fmaf(s.y, f, l);
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[c] = fmaf(a.part[row * TD + c * 32 + lane], f, acc[c]);
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    T* dst = reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c * 32 + lane < p.D) dst[c * 32 + lane] = from_f32<T>(l == 0.f ? 0.f : acc[c] * inv);
+    if (p.lse && lane == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
+  }
+}
+
+// (an item may begin in any CTA and end in a later one)
+template <int TD>
+int launch_paged_join(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.ctas, plan.WH * plan.MT / kJoinRows);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = a.p.dtype == FB_DTYPE_F16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<__half, TD>, a, plan.WH, plan.MT)
+                                                  : cudaLaunchKernelEx(&cfg, paged_join_kernel<__nv_bfloat16, TD>, a, plan.WH, plan.MT);
+  if (e == cudaSuccess) note_launch();
+  return (int)e;
+}
 
 }  // namespace fb
