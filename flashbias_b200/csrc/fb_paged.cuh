@@ -17,6 +17,11 @@ namespace fb {
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kLn2P = 0.6931471805599453f;
 
+// 16 bytes to shared memory; zeros, and nothing is read, where they do not exist
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16u : 0u) : "memory");
+}
+
 struct PagedArgs {
   fb_paged_params p;
   Div page_div, group_div;  // by page_size, by the query heads of a key head
@@ -219,22 +224,29 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   }
 }
 
-// (an item may begin in any CTA and end in a later one)
-template <int TD>
-int launch_paged_join(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
+// launch_pdl (fb_internal.h) with a grid of two dimensions and no dynamic shared memory
+template <typename... P, typename... A>
+int launch_pdl_2d(void (*kern)(P...), dim3 grid, unsigned block, cudaStream_t st, A&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(plan.ctas, plan.WH * plan.MT / kJoinRows);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = a.p.dtype == FB_DTYPE_F16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<__half, TD>, a, plan.WH, plan.MT)
-                                                  : cudaLaunchKernelEx(&cfg, paged_join_kernel<__nv_bfloat16, TD>, a, plan.WH, plan.MT);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
   if (e == cudaSuccess) note_launch();
   return (int)e;
+}
+
+// (an item may begin in any CTA and end in a later one)
+template <int TD>
+int launch_paged_join(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
+  const dim3 grid(plan.ctas, plan.WH * plan.MT / kJoinRows);
+  return a.p.dtype == FB_DTYPE_F16 ? launch_pdl_2d(paged_join_kernel<__half, TD>, grid, 128, st, a, plan.WH, plan.MT)
+                                   : launch_pdl_2d(paged_join_kernel<__nv_bfloat16, TD>, grid, 128, st, a, plan.WH, plan.MT);
 }
 
 }  // namespace fb

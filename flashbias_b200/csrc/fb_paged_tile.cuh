@@ -4,11 +4,15 @@
 // Built like the dense two-stream forward (fb_fwd_s_sm100.cuh): two softmax warpgroups share a row tile and take its key tiles in
 // turn, with logits and probabilities of their own in tensor memory, one output accumulator and one running reference maximum
 // per row that they hand to one another behind each tile's row maximum.
-//   warps 0-3, 4-7  softmax of the even / odd key tiles, thread = row; queries into shared memory; epilogue
-//   warp 8          TMA producer: a copy per page (and 64 columns), a lane looks up a page
+//   warps 0-3, 4-7  softmax of the even / odd key tiles, thread = row; epilogue
+//   warp 8          walks the schedule, one segment ahead of all others; TMA producer: a copy per page (and 64 columns), a lane
+//                   looks up a page
 //   warp 9          S = Q.K^T          warp 10   O += P.V
-//   warp 11         V behind its copy: places that hold no key become zero, and so do values that are not finite where not every
-//                   row sees the key (0 x inf would reach the rows that do not): the epilogue adds them to the rows that do
+//   warp 11         the next segment's queries; V behind its copy: places that hold no key become zero, and so do values that are
+//                   not finite where not every row sees the key (0 x inf would reach the rows that do not): the epilogue adds
+//                   them to the rows that do
+// The schedule's state is registers that a softmax thread, with a row of logits in its own, does not have: the others read the
+// segments from shared memory.
 // The schedule is that of fb_paged.cuh: equal parts of all key tiles per CTA, parts of an item joined by a second launch.
 // Key tiles are taken from the newest down: a bias that falls with the distance then shows its maximum first.
 #pragma once
@@ -24,10 +28,16 @@ constexpr int kTileThreads = 384;
 template <int TD>
 struct TileCfg {
   static constexpr int Q_BYTES = tile_bytes(TD), ST = 2;
-  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + ST * Q_BYTES, OFF_BAR = OFF_V + ST * Q_BYTES, OFF_ML = OFF_BAR + 256,
-                       OFF_M = OFF_ML + 2 * 2 * 128 * 8, SMEM = OFF_M + 2 * 128 * 4 + 1024;
+  static constexpr int OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + ST * Q_BYTES, OFF_BAR = OFF_V + ST * Q_BYTES, OFF_SEG = OFF_BAR + 512,
+                       OFF_ML = OFF_SEG + 8 * 64, OFF_M = OFF_ML + 2 * 2 * 128 * 8, OFF_POS = OFF_M + 2 * 128 * 4, SMEM = OFF_POS + 8 * 128 * 4 + 1024;
   static constexpr int T_S = 0, T_P = 256, T_O = 384;  // stream x: S + 128 x, P + 64 x
 };
+
+// A segment as the other warps read it; n_kv = 0: there are no more.
+struct TileSeg {
+  int n_kv, t0, t1, tiles, b, rt, hg, last_cta, first, tokens, len, keys;
+};
+static_assert(sizeof(TileSeg) <= 64, "room in shared memory");
 
 // The 32 keys from drafted token td0 on (negative: cached ones) that a row of token t (global token n) sees, as bits.
 __device__ __forceinline__ uint32_t seen_bits(const fb_paged_params& p, int n, int t, int td0) {
@@ -47,25 +57,29 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem), sQ = sbase, sK = sbase + Cfg::OFF_K, sV = sbase + Cfg::OFF_V, bar0 = sbase + Cfg::OFF_BAR;
-  // (two slots: one per stream, or per stage)
-  const uint32_t q_ready = bar0, q_free = bar0 + 8, o_free = bar0 + 16, s_full = bar0 + 24, p_ready = bar0 + 40, pv_done = bar0 + 56,
-                 k_full = bar0 + 72, k_free = bar0 + 88, v_full = bar0 + 104, v_free = bar0 + 120, s_read = bar0 + 136, v_ok = bar0 + 152;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 168);
-  const uint32_t abort_flag = bar0 + 172;
-  // per tile, eight deep (the producer is four tiles ahead of a softmax at most): which of the tile's pages exist
-  volatile uint32_t* s_pages = reinterpret_cast<volatile uint32_t*>(smem + Cfg::OFF_BAR + 176);
-  // per segment, eight deep: its number + 1 if it has values that were taken out
-  volatile int* s_taken = reinterpret_cast<volatile int*>(smem + Cfg::OFF_BAR + 208);
+  // (two slots: one per stream, stage, or buffer of queries)
+  const uint32_t q_ready = bar0, q_free = bar0 + 16, o_free = bar0 + 32, s_full = bar0 + 40, p_ready = bar0 + 56, pv_done = bar0 + 72,
+                 k_full = bar0 + 88, k_free = bar0 + 104, v_full = bar0 + 120, v_free = bar0 + 136, s_read = bar0 + 152, v_ok = bar0 + 168,
+                 seg_full = bar0 + 184;  // eight
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 248);
+  const uint32_t abort_flag = bar0 + 252;
+  // per tile, eight deep (the producer is four tiles ahead of a softmax at most): which of the tile's pages exist, and the
+  // positions of its keys where they are not their places
+  volatile uint32_t* s_pages = reinterpret_cast<volatile uint32_t*>(smem + Cfg::OFF_BAR + 256);
+  int* s_pos = reinterpret_cast<int*>(smem + Cfg::OFF_POS);
+  // per segment, eight deep: its number + 1 if it has values that were taken out; the segment
+  volatile int* s_taken = reinterpret_cast<volatile int*>(smem + Cfg::OFF_BAR + 288);
+  volatile TileSeg* s_seg = reinterpret_cast<volatile TileSeg*>(smem + Cfg::OFF_SEG);
 
   const fb_paged_params& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 8) {
     if (lane == 0) {
       st_shared_flag(abort_flag, 0u);
-      mbar_init(q_ready, 8);
-      mbar_init(q_free, 1);
       mbar_init(o_free, 8);
       for (int i = 0; i < 2; ++i) {
+        mbar_init(q_ready + 8 * i, 1);
+        mbar_init(q_free + 8 * i, 1);
         mbar_init(s_full + 8 * i, 1);
         mbar_init(p_ready + 8 * i, 4);
         mbar_init(pv_done + 8 * i, 1);
@@ -76,7 +90,10 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         mbar_init(v_free + 8 * i, 1);
         mbar_init(v_ok + 8 * i, 1);
       }
-      for (int i = 0; i < 8; ++i) s_taken[i] = 0;
+      for (int i = 0; i < 8; ++i) {
+        mbar_init(seg_full + 8 * i, 1);
+        s_taken[i] = 0;
+      }
       mbar_fence_init();
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
@@ -93,21 +110,47 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  Segment seg;
-  auto key0 = [](const Segment& s, int j) { return (s.t1 - 1 - j) * 128; };  // first key of the j-th tile visited
+  // Segment n, once it is known; false if there is none.
+  auto segment = [&](int n) -> const volatile TileSeg* {
+    const volatile TileSeg* sg = s_seg + (n & 7);
+    return mbar_wait(seg_full + 8 * (n & 7), (n >> 3) & 1, abort_flag) && sg->n_kv > 0 ? sg : nullptr;
+  };
 
   if (warp >= 8) {
     setmaxnreg_dec<88>();
     if (warp == 8) {
-      // ------------------------------------------------------------------ TMA producer
+      // ------------------------------------------------------------------ schedule, TMA producer
       const int rows = min(p.page_size, 128), pieces = 128 / rows;  // copies of a tile
       auto wait_all = [&](uint32_t bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)); };  // (the warp leaves together)
+      auto publish = [&](const Segment& sg, bool there, int n) {
+        if (lane == 0) {
+          volatile TileSeg* d = s_seg + (n & 7);
+          d->n_kv = there ? sg.t1 - sg.t0 : 0;
+          d->t0 = sg.t0;
+          d->t1 = sg.t1;
+          d->tiles = sg.tiles;
+          d->b = sg.b;
+          d->rt = sg.rt;
+          d->hg = sg.hg;
+          d->last_cta = sg.last_cta;
+          d->first = sg.r.first;
+          d->tokens = sg.r.tokens;
+          d->len = sg.r.len;
+          d->keys = sg.r.keys;
+          mbar_arrive(seg_full + 8 * (n & 7));
+        }
+      };
       auto produce = [&] {
-        int t = 0;
-        while (walk.next(a, seg)) {
+        Segment seg, nxt = {};
+        bool more = walk.next(a, nxt);
+        publish(nxt, more, 0);
+        for (int t = 0, n = 0; more; ++n) {
+          seg = nxt;
+          more = walk.next(a, nxt);
+          publish(nxt, more, n + 1);
           const int32_t* table = p.block_table + (int64_t)min(seg.b, p.B - 1) * p.table_stride;
           for (int j = 0; j < seg.t1 - seg.t0; ++j, ++t) {
-            const int st = t % ST, key = key0(seg, j) + lane * rows;
+            const int st = t % ST, k0 = (seg.t1 - 1 - j) * 128, key = k0 + lane * rows;
             int page = (int)p.num_pages, place = 0;  // behind the cache: the copy fills in zeros
             bool bad = false;
             if (lane < pieces && key < seg.r.keys) {
@@ -122,10 +165,16 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             }
             const uint32_t there = ~__ballot_sync(0xffffffffu, bad);
             if (t >= ST && !wait_all(k_free + 8 * st, (t / ST - 1) & 1)) return;
-            if (lane == 0) {
-              s_pages[t & 7] = there;
-              mbar_expect_tx(k_full + 8 * st, Cfg::Q_BYTES);
+            if (SLOPES && k0 + 128 > seg.r.len) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int k = k0 + e * 32 + lane;
+                s_pos[(t & 7) * 128 + e * 32 + lane] = p.positions && k >= seg.r.len && k < seg.r.keys ? p.positions[seg.r.first + k - seg.r.len] : k;
+              }
             }
+            if (lane == 0) s_pages[t & 7] = there;
+            __syncwarp();
+            if (lane == 0) mbar_expect_tx(k_full + 8 * st, Cfg::Q_BYTES);
             __syncwarp();
             if (lane < pieces) {
 #pragma unroll
@@ -150,21 +199,22 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         constexpr uint32_t idS = instr_desc(kBf16, false, false, 128, 128);
         const DescBase dQ = kmajor_base<TD>(sQ), dK = kmajor_base<TD>(sK);
         int t = 0, n = 0, c0 = 0, c1 = 0;  // key tiles, segments; key tiles of either stream
-        for (; walk.next(a, seg); ++n) {
-          mbar_wait(q_ready, n & 1, abort_flag);
+        for (const volatile TileSeg* sg; (sg = segment(n)); ++n) {
+          const int n_kv = sg->n_kv, qo = (n & 1) * Cfg::Q_BYTES;
+          mbar_wait(q_ready + 8 * (n & 1), (n >> 1) & 1, abort_flag);
           tc_fence_after_sync();
-          for (int j = 0; j < seg.t1 - seg.t0; ++j, ++t) {
+          for (int j = 0; j < n_kv; ++j, ++t) {
             const int x = j & 1, c = x ? c1++ : c0++, st = t % ST;
             if (c > 0) mbar_wait(s_read + 8 * x, (c - 1) & 1, abort_flag);
             mbar_wait(k_full + 8 * st, (t / ST) & 1, abort_flag);
             tc_fence_after_sync();
 #pragma unroll
             for (int s = 0; s < TD / 16; ++s)
-              umma_ss(tmem + Cfg::T_S + 128 * x, desc_at(dQ, kmajor_step<TD>(s)), desc_at(dK, st * Cfg::Q_BYTES + kmajor_step<TD>(s)), idS, s > 0);
+              umma_ss(tmem + Cfg::T_S + 128 * x, desc_at(dQ, qo + kmajor_step<TD>(s)), desc_at(dK, st * Cfg::Q_BYTES + kmajor_step<TD>(s)), idS, s > 0);
             umma_commit(s_full + 8 * x);
             umma_commit(k_free + 8 * st);
           }
-          umma_commit(q_free);  // Q of this segment is no longer read
+          umma_commit(q_free + 8 * (n & 1));  // the segment's queries are no longer read
         }
       }
     } else if (warp == 10) {
@@ -173,8 +223,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         constexpr uint32_t idO = instr_desc(kBf16, false, true, 128, TD);
         const DescBase dV = mnmajor_base<TD>(sV);
         int t = 0, n = 0, c0 = 0, c1 = 0;
-        for (; walk.next(a, seg); ++n) {
-          for (int j = 0; j < seg.t1 - seg.t0; ++j, ++t) {
+        for (const volatile TileSeg* sg; (sg = segment(n)); ++n) {
+          const int n_kv = sg->n_kv;
+          for (int j = 0; j < n_kv; ++j, ++t) {
             const int x = j & 1, c = x ? c1++ : c0++, st = t % ST;
             mbar_wait(v_ok + 8 * st, (t / ST) & 1, abort_flag);
             mbar_wait(p_ready + 8 * x, c & 1, abort_flag);
@@ -189,13 +240,48 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
       }
     } else {
-      // ------------------------------------------------------------------ V behind its copy
+      // ------------------------------------------------------------------ queries; V behind its copy
+      constexpr int STEP = 8 * (32 / CH);  // rows of a step: eight copies of a lane
+      auto load_q = [&](const volatile TileSeg* sg, int n, int r0) {
+        if (r0 == 0 && n > 1) mbar_wait(q_free + 8 * (n & 1), (n / 2 - 1) & 1, abort_flag);
+        const int rt = sg->rt, hg = sg->hg, first = sg->first, rows = min(sg->tokens * a.G - rt * 128, 128);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int r = r0 + u * (32 / CH) + lane / CH, col = (lane % CH) * 8, gr = rt * 128 + r;
+          const bool live = r < rows && col < p.D;
+          const int tok = live ? a.group_div.quot32(gr) : 0, head = hg * a.G + (live ? gr - tok * a.G : 0);
+          const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(first + tok) * p.q_stride[0] + head * p.q_stride[1] + col;
+          cp_async16_zfill(sQ + (n & 1) * Cfg::Q_BYTES + tile_chunk_offset<TD>(r, col), live ? src : reinterpret_cast<const T*>(p.q), live);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      auto q_landed = [&](int n) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_ready + 8 * (n & 1));
+      };
+      auto segment_warp = [&](int n) {  // (the warp leaves together)
+        const volatile TileSeg* sg = segment(n);
+        return __all_sync(0xffffffffu, sg != nullptr) ? sg : nullptr;
+      };
       int t = 0, n = 0;
-      for (; walk.next(a, seg); ++n) {
-        for (int j = 0; j < seg.t1 - seg.t0; ++j, ++t) {
-          const int st = t % ST, k0 = key0(seg, j);
+      const volatile TileSeg *sg = segment_warp(0), *nx = nullptr;
+      for (int r0 = 0; sg && r0 < 128; r0 += STEP) load_q(sg, 0, r0);
+      if (sg) q_landed(0);
+      for (; sg; sg = nx, ++n) {
+        const int n_kv = sg->n_kv, t1 = sg->t1, len = sg->len, keys = sg->keys;
+        nx = nullptr;
+        int qrow = 128 + STEP;  // the next segment's queries: a step behind every tile, then the wait for them
+        auto next_q = [&] {
+          if (qrow < 128) load_q(nx, n + 1, qrow);
+          else if (qrow < 128 + STEP) q_landed(n + 1);
+          qrow += STEP;
+        };
+        for (int j = 0; j < n_kv; ++j, ++t) {
+          const int st = t % ST, k0 = (t1 - 1 - j) * 128;
           mbar_wait(v_full + 8 * st, (t / ST) & 1, abort_flag);
-          const int r0 = max(seg.r.len - k0, 0), live = seg.r.keys - k0;  // first row that not all see; rows that hold keys
+          const int r0 = max(len - k0, 0), live = keys - k0;  // first row that not all see; rows that hold keys
           if (r0 < 128) {
             bool taken = false;
             for (int i = r0 * CH + lane; i < 128 * CH; i += 32) {
@@ -222,7 +308,10 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(v_ok + 8 * st);
+          if (j == 0 && (nx = segment_warp(n + 1))) qrow = 0;  // (known before the first copy of this one)
+          next_q();
         }
+        while (qrow < 128 + STEP) next_q();
       }
     }
   } else {
@@ -236,64 +325,53 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const uint64_t sl2p = f2(sl2, sl2);
     int c = 0, co = 0, n = 0, t0 = 0;  // key tiles of this stream and of the other, segments and key tiles so far
     uint32_t s[4][32];                 // the thread's row of the logit tile
-    int tok, head;                     // the row's token (of the request) and query head; -1: padding
-    // Half a row of queries per thread; ahead of the last segment's epilogue.
-    auto load_q = [&](const Segment& sg, int nth) {
-      const int gr = sg.rt * 128 + row;
-      tok = -1;
-      head = 0;
-      if (gr < sg.r.tokens * a.G) {
-        tok = a.group_div.quot32(gr);
-        head = sg.hg * a.G + gr - tok * a.G;
-      }
-      const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(sg.r.first + max(tok, 0)) * p.q_stride[0] + head * p.q_stride[1];
-      if (nth > 0) mbar_wait(q_free, (nth - 1) & 1, abort_flag);
-#pragma unroll
-      for (int ch = 0; ch < CH / 2; ++ch) {
-        const int col = (x * CH / 2 + ch) * 8;
-        const uint4 w = tok >= 0 && col < p.D ? *reinterpret_cast<const uint4*>(src + col) : make_uint4(0u, 0u, 0u, 0u);
-        st_shared_v4(sQ + tile_chunk_offset<TD>(row, col), w.x, w.y, w.z, w.w);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive_warp(q_ready);
+    auto segment_both = [&](int n) {  // (the warpgroups leave together: behind an expired wait, too)
+      const volatile TileSeg* sg = segment(n);
+      uint32_t all;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.b32 p, %1, 0;\n\t"
+          "barrier.cta.red.and.pred q, 1, 256, p;\n\t"
+          "selp.b32 %0, 1, 0, q;\n\t}"
+          : "=r"(all)
+          : "r"(sg ? 1u : 0u)
+          : "memory");
+      return all ? sg : nullptr;
     };
-    Segment nxt;
-    bool more = walk.next(a, nxt);
-    if (more) load_q(nxt, 0);
-    for (; more; ++n) {
-      seg = nxt;
-      const int n_kv = seg.t1 - seg.t0, tk = tok, hd = head, gn = seg.r.first + max(tk, 0);
+    for (const volatile TileSeg* sg; (sg = segment_both(n)); ++n) {
+      const int n_kv = sg->n_kv, t1 = sg->t1, len = sg->len, keys = sg->keys;
+      // the row's token (of the request, -1: padding) and query head
+      const int gr = sg->rt * 128 + row, tk = gr < sg->tokens * a.G ? a.group_div.quot32(gr) : -1, gn = sg->first + max(tk, 0);
+      const int hd = sg->hg * a.G + (tk >= 0 ? gr - tk * a.G : 0);
       float m_used = -INFINITY, l = 0.f;  // reference maximum (log2 units: logit * log2 e); row sum of this stream's tiles, relative to it
       const int c0 = c, co0 = co;
       const float slope2 = SLOPES && tk >= 0 ? p.slopes[hd] * kLog2eP : 0.f;
-      const int my_pos = SLOPES && tk >= 0 ? (p.positions ? p.positions[gn] : seg.r.len + tk) : 0;
+      const int my_pos = SLOPES && tk >= 0 ? (p.positions ? p.positions[gn] : len + tk) : 0;
       for (int j = x; j < n_kv; j += 2, ++c) {
-        const int k0 = key0(seg, j);
+        const int k0 = (t1 - 1 - j) * 128;
         mbar_wait(s_full + 8 * x, c & 1, abort_flag);
         tc_fence_after_sync();
         const uint32_t there = s_pages[(t0 + j) & 7];
-        const bool dead = there != 0xffffffffu || k0 + 128 > seg.r.len;
+        const bool dead = there != 0xffffffffu || k0 + 128 > len;
+        const int* pos = s_pos + ((t0 + j) & 7) * 128;
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         const float abase = SLOPES ? slope2 * (float)(k0 - my_pos) : 0.f;
         auto complete = [&](int ch) {
           if (dead) {
-            const int j0 = k0 + ch * 32, left = seg.r.keys - j0;
+            const int j0 = k0 + ch * 32, left = keys - j0;
             uint32_t bits = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
-            if (tk >= 0 && bits && j0 + 32 > seg.r.len) bits &= seen_bits(p, gn, tk, j0 - seg.r.len);
+            if (tk >= 0 && bits && j0 + 32 > len) bits &= seen_bits(p, gn, tk, j0 - len);
             if (there != 0xffffffffu) {  // (rare)
               const int rows = min(p.page_size, 128);
+#pragma unroll 1
               for (int i = 0; i < 32; ++i)
                 if (!(there >> ((ch * 32 + i) / rows) & 1)) bits &= ~(1u << i);
             }
-            if (SLOPES && p.positions) {
+            if (SLOPES) {
+              const bool own = k0 + 128 > len;  // (a tile of cached keys has no table of positions)
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const int key = j0 + i, pos = key >= seg.r.len && key < seg.r.keys ? p.positions[seg.r.first + key - seg.r.len] : key;
-                s[ch][i] = __float_as_uint(fmaf(slope2, (float)(pos - my_pos), __uint_as_float(s[ch][i]) * sl2));
-              }
-            } else if (SLOPES) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) s[ch][i] = __float_as_uint(fmaf(slope2, (float)(j0 + i - my_pos), __uint_as_float(s[ch][i]) * sl2));
+              for (int i = 0; i < 32; ++i)
+                s[ch][i] = __float_as_uint(fmaf(slope2, (float)((own ? pos[ch * 32 + i] : j0 + i) - my_pos), __uint_as_float(s[ch][i]) * sl2));
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -395,8 +473,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         mbar_arrive_warp(p_ready + 8 * x);
       }
       t0 += n_kv;
-      more = walk.next(a, nxt);
-      if (more) load_q(nxt, n + 1);
       // ---- epilogue, this warpgroup's half of the columns.  The stream of the last tile knows its product to have completed (its
       // commit covers the ones before it, which the same thread issued); the other learns it from the warpgroups' barrier.
       c = c0 + ((n_kv + 1 - x) >> 1);
@@ -410,9 +486,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const float2 other = ml[(x ^ 1) * 128 + row];
       const float m = fmaxf(m_used, other.x), ms = m == -INFINITY ? 0.f : m;  // the last reference is the largest
       const float ls = l * fast_exp2(m_used - ms) + other.y * fast_exp2(other.x - ms);
-      const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles, taken = s_taken[n & 7] == n + 1;
+      const bool begins = sg->t0 == 0, whole = begins && t1 == sg->tiles, taken = s_taken[n & 7] == n + 1;
       const float inv = !whole ? 1.f : ls > 0.f ? 1.f / ls : ls == 0.f ? 0.f : ls;
-      const int64_t prow = ((int64_t)blockIdx.x * 2 + (seg.t0 == 0 ? 1 : 0)) * 128 + row;  // slot 1: the CTA in which the item begins
+      const int64_t slot = (int64_t)blockIdx.x * 2 + (begins ? 1 : 0);  // slot 1: the CTA in which the item begins
 #pragma unroll 1
       for (int ch = 0; ch < TD / 64; ++ch) {
         const int col0 = x * (TD / 2) + ch * 32;
@@ -421,12 +497,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         tmem_wait_ld(r);
         if (tk >= 0) {
           if (taken) {  // (rare) values that are not finite, for the rows that see their keys
-            const int32_t* table = p.block_table + (int64_t)seg.b * p.table_stride;
-            for (int key = max(seg.r.len, seg.t0 * 128); key < min(seg.r.keys, seg.t1 * 128); ++key) {
+            const int32_t* table = p.block_table + (int64_t)sg->b * p.table_stride;
+            for (int key = max(len, sg->t0 * 128); key < min(keys, t1 * 128); ++key) {
               const int col = a.page_div.quot32(key), pg = table[col];
-              if (pg < 0 || pg >= p.num_pages || !tree_sees(p, gn, tk, key - seg.r.len)) continue;
+              if (pg < 0 || pg >= p.num_pages || !tree_sees(p, gn, tk, key - len)) continue;
               const T* v = reinterpret_cast<const T*>(p.value_cache) + pg * p.value_cache_stride[0] + (key - col * p.page_size) * p.value_cache_stride[1] +
-                           seg.hg * p.value_cache_stride[2] + col0;
+                           sg->hg * p.value_cache_stride[2] + col0;
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 const float e = col0 + i < p.D ? to_f32(v[i]) : 0.f;
@@ -445,19 +521,19 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               *reinterpret_cast<uint4*>(orow + col0 + g * 8) = make_uint4(p2(0), p2(2), p2(4), p2(6));
             }
           } else {
-            float4* dst = reinterpret_cast<float4*>(a.part + prow * TD + col0);
+            float4* dst = reinterpret_cast<float4*>(a.part) + (slot * (TD / 4) + col0 / 4) * 128 + row;  // (columns / 4, rows, 4)
 #pragma unroll
             for (int g = 0; g < 8; ++g)
-              dst[g] = make_float4(__uint_as_float(r[4 * g]), __uint_as_float(r[4 * g + 1]), __uint_as_float(r[4 * g + 2]), __uint_as_float(r[4 * g + 3]));
+              dst[g * 128] = make_float4(__uint_as_float(r[4 * g]), __uint_as_float(r[4 * g + 1]), __uint_as_float(r[4 * g + 2]), __uint_as_float(r[4 * g + 3]));
           }
         }
         __syncwarp();
       }
       if (x == 0 && tk >= 0) {
-        if (!whole) a.ml[prow] = make_float2(m, ls);
+        if (!whole) a.ml[slot * 128 + row] = make_float2(m, ls);
         else if (p.lse) p.lse[(int64_t)gn * p.Hq + hd] = ls > 0.f ? (m + fast_log2(ls)) * kLn2P : ls == 0.f ? -INFINITY : ls;
       }
-      if (!whole && seg.t0 == 0 && threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(seg.b, seg.rt, seg.hg, seg.last_cta);
+      if (!whole && begins && threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(sg->b, sg->rt, sg->hg, sg->last_cta);
       tc_fence_before_sync();
       mbar_arrive_warp(o_free);
     }
@@ -470,6 +546,47 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     __syncwarp();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// Joins the parts of the item that begins in CTA blockIdx.x, in the order of the CTAs: thread = row, 32 columns.
+template <typename T, int TD>
+__global__ void __launch_bounds__(128) paged_join_tile_kernel(const __grid_constant__ PagedArgs a) {
+  grid_dep_wait();
+  const int4 d = a.desc[blockIdx.x];
+  if (d.x < 0) return;
+  const fb_paged_params& p = a.p;
+  const Request rq = request_at(p, d.x);
+  const int row = threadIdx.x, gr = d.y * 128 + row, col0 = blockIdx.y * 32, parts = d.w - (int)blockIdx.x + 1;
+  if (gr >= rq.tokens * a.G) return;
+  const int t = a.group_div.quot32(gr), h = d.z * a.G + gr - t * a.G, n = rq.first + t;
+  auto slot_of = [&](int i) { return (int64_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, a.ml[slot_of(i) * 128 + row].x);
+  const float ms = fmaxf(m, -FLT_MAX);
+  float l = 0.f;
+  float4 acc[8] = {};
+#pragma unroll 2
+  for (int i = 0; i < parts; ++i) {
+    const float2 s = a.ml[slot_of(i) * 128 + row];
+    const float f = fast_exp2(s.x - ms);
+    l = fmaf(s.y, f, l);
+    const float4* src = reinterpret_cast<const float4*>(a.part) + (slot_of(i) * (TD / 4) + col0 / 4) * 128 + row;
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      const float4 v = src[g * 128];
+      acc[g] = make_float4(fmaf(v.x, f, acc[g].x), fmaf(v.y, f, acc[g].y), fmaf(v.z, f, acc[g].z), fmaf(v.w, f, acc[g].w));
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  T* dst = reinterpret_cast<T*>(p.o) + (int64_t)n * p.o_stride[0] + h * p.o_stride[1] + col0;
+  auto p2 = [&](float x, float y) { return l == 0.f ? 0u : Pack2<T>::pack(x * inv, y * inv); };
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    if (col0 + g * 8 < p.D)
+      *reinterpret_cast<uint4*>(dst + g * 8) = make_uint4(p2(acc[2 * g].x, acc[2 * g].y), p2(acc[2 * g].z, acc[2 * g].w), p2(acc[2 * g + 1].x, acc[2 * g + 1].y),
+                                                          p2(acc[2 * g + 1].z, acc[2 * g + 1].w));
+  if (p.lse && blockIdx.y == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
 }
 
 template <typename T, int TD, bool SLOPES>
@@ -487,7 +604,8 @@ int launch_paged_tile_t(const PagedArgs& a, const PagedPlan& plan, const CUtenso
       attr_done[dev & 63] = true;
     }
   }
-  return launch_pdl(kern, plan.ctas, kTileThreads, TileCfg<TD>::SMEM, st, tk, tv, a);
+  if (const int rc = launch_pdl(kern, plan.ctas, kTileThreads, TileCfg<TD>::SMEM, st, tk, tv, a)) return rc;
+  return launch_pdl_2d(paged_join_tile_kernel<T, TD>, dim3(plan.ctas, TD / 32), 128, st, a);
 }
 
 template <int TD>
@@ -504,8 +622,7 @@ int launch_paged_tile(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st
     using T = decltype(t);
     return p.slopes ? launch_paged_tile_t<T, TD, true>(a, plan, tk, tv, st) : launch_paged_tile_t<T, TD, false>(a, plan, tk, tv, st);
   };
-  if ((rc = p.dtype == FB_DTYPE_F16 ? go(__half()) : go(__nv_bfloat16()))) return rc;
-  return launch_paged_join<TD>(a, plan, st);
+  return p.dtype == FB_DTYPE_F16 ? go(__half()) : go(__nv_bfloat16());
 }
 
 }  // namespace fb
