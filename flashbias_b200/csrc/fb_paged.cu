@@ -163,7 +163,7 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
     plan.kernel = PAGED_SPLIT;
     plan.TD = p->D <= 32 ? 32 : p->D <= 64 ? 64 : 128;
     plan.MT = rows <= 16 ? 16 : 32;
-    plan.ctas = 2 * sms;
+    plan.ctas = split_ctas(plan.TD, plan.MT) * sms;
     // The heads of a group are read side by side, whole rows of the cache; where the longest requests that the table can hold do
     // not fill the GPU that way, one head is spread over the CTA's warps.
     const int64_t tiles = (int64_t)p->B * (((int64_t)p->table_width * p->page_size + 63) / 64) * p->Hk;
@@ -172,7 +172,7 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
   const size_t prows = (size_t)plan.ctas * 2 * plan.WH * plan.MT;
   plan.part_bytes = round256(prows * plan.TD * 4);
   plan.ml_bytes = round256(prows * 8);
-  plan.desc_bytes = round256((size_t)plan.ctas * 16);
+  plan.desc_bytes = round256((size_t)plan.ctas * 32);
   return plan;
 }
 
@@ -200,6 +200,9 @@ extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
     a.G = p->Hq / p->Hk;
     a.page_div = Div(p->page_size);
     a.group_div = Div(a.G);
+    a.whole_tiles = p->page_size % 16 == 0;
+    a.factor_words = p->R % 2 == 0 && !(reinterpret_cast<uintptr_t>(p->bias_cache) & 3) &&
+                     !((p->bias_cache_stride[0] | p->bias_cache_stride[1] | (p->bias_heads > 1 ? p->bias_cache_stride[2] : 0)) & 1);
     a.scale_log2 = p->softmax_scale * kLog2eP;
     uint8_t* ws = reinterpret_cast<uint8_t*>(p->workspace);
     a.part = reinterpret_cast<float*>(ws);

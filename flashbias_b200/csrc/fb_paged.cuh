@@ -26,10 +26,13 @@ struct PagedArgs {
   fb_paged_params p;
   Div page_div, group_div;  // by page_size, by the query heads of a key head
   int G;                    // query heads of a key head
+  int whole_tiles;          // split kernel: pages are whole tiles of 16 keys
+  int factor_words;         // split kernel: factor rows can be read two columns at a time
   float scale_log2;
   float* part;    // (CTAs, 2, heads of a group, rows of a tile, columns): sums of items that span CTAs
   float2* ml;     // the same without columns: maximum (log2 units) and sum
-  int4* desc;     // (CTAs): the item that begins in a CTA and ends in another: request, row tile, head group, last CTA; x = -1: none
+  int4* desc;     // (CTAs, 2): the item that begins in a CTA and ends in another: row tile, head group, last CTA, -; first token,
+                  // rows of the request; a row tile of -1: none
 };
 
 __device__ __forceinline__ void paged_bad_index(const fb_paged_params& p) {
@@ -168,6 +171,8 @@ __device__ __forceinline__ bool tree_sees(const fb_paged_params& p, int n, int t
 
 // ---- host side (fb_paged.cu, fb_paged_split_*.cu, fb_paged_tile_*.cu) ------------------------------------------------
 enum { PAGED_GENERAL, PAGED_SPLIT, PAGED_TILE };
+// CTAs of the split kernel that an SM holds: three while their warps' output rows leave the registers for it
+constexpr int split_ctas(int TD, int MT) { return TD < 128 && MT == 16 ? 3 : 2; }
 struct PagedPlan {
   int kernel;  // PAGED_*
   int TD, MT;  // columns and rows of a tile
@@ -181,47 +186,59 @@ int launch_paged_split_d128(const PagedArgs& a, const PagedPlan& plan, cudaStrea
 int launch_paged_tile_d64(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
 int launch_paged_tile_d128(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
 
-// Joins the parts of the item that begins in CTA blockIdx.x; a warp per row, the parts in the order of the CTAs.
-constexpr int kJoinRows = 16;  // of a block
+// Joins the parts of the item that begins in CTA blockIdx.x; a warp per row, the parts in the order of the CTAs.  Latency is
+// all there is to it: what the rows need stands in the descriptor, and the first parts are on their way before the maximum is
+// known.
 template <typename T, int TD>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a, const int WH, const int MT) {
-  constexpr int C = TD / 32;  // columns of a lane
+  constexpr int C = TD / 32, U = 8;  // columns of a lane, parts in flight
   grid_dep_wait();
-  const int4 d = a.desc[blockIdx.x];
+  const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
   if (d.x < 0) return;
   const fb_paged_params& p = a.p;
-  const int lane = threadIdx.x & 31;
-  const Request rq = request_at(p, d.x);
-  for (int idx = blockIdx.y * kJoinRows + (threadIdx.x >> 5); idx < (blockIdx.y + 1) * kJoinRows; idx += 4) {
-    const int wh = idx / MT, r = idx - wh * MT, gr = d.y * MT + r;
-    if (gr >= rq.tokens * a.G) continue;
-    const int t = a.group_div.quot32(gr), h = (d.z * WH + wh) * a.G + gr - t * a.G, n = rq.first + t;
-    const int64_t step = (int64_t)2 * WH * MT;  // rows of a CTA
-    const int64_t row0 = blockIdx.x * step + (int64_t)(WH + wh) * MT + r, row1 = (int64_t)(blockIdx.x + 1) * step + (int64_t)wh * MT + r;
-    const int parts = d.w - (int)blockIdx.x + 1;
-    auto row_of = [&](int i) { return i == 0 ? row0 : row1 + (i - 1) * step; };
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, a.ml[row_of(i)].x);
+  const int lane = threadIdx.x & 31, idx = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const int wh = idx / MT, r = idx - wh * MT, gr = d.x * MT + r, parts = d.z - (int)blockIdx.x + 1;
+  if (gr >= e.y) return;
+  const int64_t step = (int64_t)2 * WH * MT;  // rows of a CTA
+  const int64_t row0 = blockIdx.x * step + (int64_t)(WH + wh) * MT + r, row1 = (int64_t)(blockIdx.x + 1) * step + (int64_t)wh * MT + r;
+  auto row_of = [&](int i) { return i == 0 ? row0 : row1 + (i - 1) * step; };
+  float v[U][C];
+  float2 s[U];
+  auto load = [&](int i0) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ms = fmaxf(m, -FLT_MAX);
-    float l = 0.f, acc[C] = {};
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const int64_t row = row_of(i);
-      const float2 s = a.ml[row];
-      const float f = fast_exp2(s.x - ms);
-      l = fmaf(s.y, f, l);
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = row_of(min(i0 + u, parts - 1));
+      s[u] = a.ml[row];
 #pragma unroll
-      for (int c = 0; c < C; ++c) acc[c] = fmaf(a.part[row * TD + c * 32 + lane], f, acc[c]);
+      for (int c = 0; c < C; ++c) v[u][c] = a.part[row * TD + c * 32 + lane];
     }
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-    T* dst = reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1];
+  };
+  load(0);
+  float m = -INFINITY;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, a.ml[row_of(i)].x);
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (c * 32 + lane < p.D) dst[c * 32 + lane] = from_f32<T>(l == 0.f ? 0.f : acc[c] * inv);
-    if (p.lse && lane == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float ms = fmaxf(m, -FLT_MAX);
+  float l = 0.f, acc[C] = {};
+  for (int i0 = 0;;) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u >= parts) break;
+      const float f = fast_exp2(s[u].x - ms);
+      l = fmaf(s[u].y, f, l);
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[c] = fmaf(v[u][c], f, acc[c]);
+    }
+    if ((i0 += U) >= parts) break;
+    load(i0);
   }
+  const int t = a.group_div.quot32(gr), h = (d.y * WH + wh) * a.G + gr - t * a.G, n = e.x + t;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  T* dst = reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (c * 32 + lane < p.D) dst[c * 32 + lane] = from_f32<T>(l == 0.f ? 0.f : acc[c] * inv);
+  if (p.lse && lane == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
 }
 
 // launch_pdl (fb_internal.h) with a grid of two dimensions and no dynamic shared memory
@@ -244,7 +261,7 @@ int launch_pdl_2d(void (*kern)(P...), dim3 grid, unsigned block, cudaStream_t st
 // (an item may begin in any CTA and end in a later one)
 template <int TD>
 int launch_paged_join(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
-  const dim3 grid(plan.ctas, plan.WH * plan.MT / kJoinRows);
+  const dim3 grid(plan.ctas, plan.WH * plan.MT / 4);
   return a.p.dtype == FB_DTYPE_F16 ? launch_pdl_2d(paged_join_kernel<__half, TD>, grid, 128, st, a, plan.WH, plan.MT)
                                    : launch_pdl_2d(paged_join_kernel<__nv_bfloat16, TD>, grid, 128, st, a, plan.WH, plan.MT);
 }

@@ -22,7 +22,7 @@ constexpr int kSplitKT = 64;  // keys of a scheduled tile: four sub-tiles of 16
 template <int TD>
 struct SplitCfg {
   static constexpr int ROW = TD * 2;                                     // bytes of a key's row
-  static constexpr int ST = TD == 128 ? 3 : TD == 64 ? 6 : 8;            // ring stages
+  static constexpr int ST = TD == 128 ? 3 : 4;                           // ring stages
   static constexpr int HALF = 16 * ROW, STAGE = 2 * HALF, RING = ST * STAGE;  // K, then V
   static constexpr int SMEM = kSplitWarps * RING + kSplitWarps * ST * 4;
   static constexpr int CH = TD / 8;  // 16-byte chunks of a row
@@ -57,7 +57,7 @@ __device__ __forceinline__ bool pair_not_finite(uint32_t w) {
 enum { PAGED_PLAIN = 0, PAGED_SLOPES = 1, PAGED_FACTORS = 2 };
 
 template <typename T, int TD, int MT, int BIAS>
-__global__ void __launch_bounds__(kSplitThreads, 2) paged_split_kernel(const __grid_constant__ PagedArgs a, const int WH) {
+__global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split_kernel(const __grid_constant__ PagedArgs a, const int WH) {
   using Cfg = SplitCfg<TD>;
   constexpr int NM = MT / 16, KS = TD / 16, NT = TD / 8, ST = Cfg::ST;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) paged_split_kernel(const __g
   uint32_t* ring_ok = reinterpret_cast<uint32_t*>(smem + kSplitWarps * Cfg::RING) + warp * ST;  // keys of a stage that exist, as bits
   const int qr = lane >> 2, qc = 2 * (lane & 3);  // a fragment's row (and row + 8) and first column of this lane
   grid_dep_wait();
-  if (threadIdx.x == 0) a.desc[blockIdx.x].x = -1;
+  if (threadIdx.x == 0) a.desc[2 * blockIdx.x].x = -1;
   PagedWalk<kSplitKT, MT, kSplitThreads> walk;
   walk.start(a, p.Hk / WH);
 
@@ -81,10 +81,17 @@ __global__ void __launch_bounds__(kSplitThreads, 2) paged_split_kernel(const __g
     const int32_t* table = p.block_table + (int64_t)min(seg.b, p.B - 1) * p.table_stride;
     const int tile_end = min(seg.t1 * 4, (rq.keys + 15) >> 4);
 
-    // ---- copies: the pages of a tile's keys (lane & 15 = key) are looked up one tile ahead of their use
+    // ---- copies: the pages of a tile's keys are looked up one tile ahead of their use (lane & 15 = key).  Where pages are whole
+    // tiles one page serves all lanes, and a copy's address is one addition: half of the instructions that a tile of 64 columns
+    // takes would otherwise go into addresses.
+    const int c = lane % Cfg::CH, kr = lane / Cfg::CH;  // this lane's chunk, and its key in the first of a tile's copies
+    const bool in = c * 8 < p.D;
+    const int64_t kstep = (32 / Cfg::CH) * p.key_cache_stride[1], vstep = (32 / Cfg::CH) * p.value_cache_stride[1];
+    const T *klane = kbase + kr * p.key_cache_stride[1] + (in ? c * 8 : 0), *vlane = vbase + kr * p.value_cache_stride[1] + (in ? c * 8 : 0);
+    const uint32_t dst0 = ring + Cfg::at(kr, c);
     int page_next = -1, place_next = 0;
     auto look_up = [&](int tile) {
-      const int j = tile * 16 + (lane & 15);
+      const int j = tile * 16 + (a.whole_tiles ? 0 : lane & 15);
       page_next = -1;
       if (tile < tile_end && j < rq.keys) {
         const int col = a.page_div.quot32(j);
@@ -94,55 +101,81 @@ __global__ void __launch_bounds__(kSplitThreads, 2) paged_split_kernel(const __g
     };
     auto fetch = [&](int tile, int stage) {
       if (tile < tile_end) {
-        const int page = page_next;
-        const bool there = tile * 16 + (lane & 15) < rq.keys, ok = there && page >= 0 && page < p.num_pages;
-        if (there && !ok) paged_bad_index(p);
-        const int64_t ko = ok ? page * p.key_cache_stride[0] + place_next * p.key_cache_stride[1] : 0;
-        const int64_t vo = ok ? page * p.value_cache_stride[0] + place_next * p.value_cache_stride[1] : 0;
-        const uint32_t okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-        if (lane == 0) ring_ok[stage] = okm;
-        look_up(tile + WK);
-        const int c = lane % Cfg::CH;
-        const bool in = c * 8 < p.D;
+        const int page = page_next, place = place_next;
         const uint32_t dst = ring + stage * Cfg::STAGE;
+        if (a.whole_tiles && tile * 16 + 16 <= rq.keys && (uint32_t)page < (uint32_t)min(p.num_pages, (int64_t)0x7fffffff)) {
+          look_up(tile + WK);
+          if (lane == 0) ring_ok[stage] = 0xffffu;
+          const T* k = klane + page * p.key_cache_stride[0] + place * p.key_cache_stride[1];
+          const T* v = vlane + page * p.value_cache_stride[0] + place * p.value_cache_stride[1];
 #pragma unroll
-        for (int i = 0; i < TD / 16; ++i) {
-          const int key = (i * 32 + lane) / Cfg::CH;
-          const int64_t k = __shfl_sync(0xffffffffu, ko, key), v = __shfl_sync(0xffffffffu, vo, key);
-          const bool live = in && ((okm >> key) & 1);
-          cp_async16_zfill(dst + Cfg::at(key, c), live ? kbase + k + c * 8 : kbase, live);
-          cp_async16_zfill(dst + Cfg::HALF + Cfg::at(key, c), live ? vbase + v + c * 8 : vbase, live);
+          for (int i = 0; i < TD / 16; ++i) {
+            const uint32_t at = dst + Cfg::at(kr + i * (32 / Cfg::CH), c);
+            cp_async16_zfill(at, k, in);
+            cp_async16_zfill(at + Cfg::HALF, v, in);
+            k += kstep;
+            v += vstep;
+          }
+        } else {
+          const int off = a.whole_tiles ? lane & 15 : 0;
+          const bool there = tile * 16 + (lane & 15) < rq.keys, ok = there && page >= 0 && page < p.num_pages;
+          if (there && !ok) paged_bad_index(p);
+          const int64_t ko = ok ? page * p.key_cache_stride[0] + (place + off) * p.key_cache_stride[1] : 0;
+          const int64_t vo = ok ? page * p.value_cache_stride[0] + (place + off) * p.value_cache_stride[1] : 0;
+          const uint32_t okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+          if (lane == 0) ring_ok[stage] = okm;
+          look_up(tile + WK);
+#pragma unroll
+          for (int i = 0; i < TD / 16; ++i) {
+            const int key = kr + i * (32 / Cfg::CH);
+            const int64_t k = __shfl_sync(0xffffffffu, ko, key), v = __shfl_sync(0xffffffffu, vo, key);
+            const bool live = in && ((okm >> key) & 1);
+            cp_async16_zfill(dst + Cfg::at(key, c), live ? kbase + k + c * 8 : kbase, live);
+            cp_async16_zfill(dst + Cfg::HALF + Cfg::at(key, c), live ? vbase + v + c * 8 : vbase, live);
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // factors of the keys of a tile in the layout of the product's second operand, one tile ahead
-    uint16_t kb[2][4] = {};
-    auto load_factors = [&](int tile, int r0, uint16_t (&f)[2][4]) {
+    // Factors of a tile's keys in the layout of the product's second operand (two columns a word), one tile ahead; their pages
+    // two ahead.
+    uint32_t kb[2][2] = {};
+    int fpage[2] = {-1, -1}, fplace[2] = {};
+    auto factor_pages = [&](int tile) {
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         const int j = tile * 16 + nt * 8 + qr;
-        const T* src = nullptr;
+        fpage[nt] = -1;
         if (tile < tile_end && j < rq.keys) {
-          const int col = a.page_div.quot32(j), page = table[col];
-          if (page >= 0 && page < p.num_pages) src = bbase + page * p.bias_cache_stride[0] + (j - col * p.page_size) * p.bias_cache_stride[1];
+          const int col = a.page_div.quot32(j);
+          fplace[nt] = j - col * p.page_size;
+          fpage[nt] = table[col];
         }
+      }
+    };
+    auto load_factors = [&](int r0, uint32_t (&f)[2][2]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = r0 + qc + (i & 1) + (i >> 1) * 8;
-          f[nt][i] = src && c < p.R ? reinterpret_cast<const uint16_t*>(src)[c] : (uint16_t)0;
+      for (int nt = 0; nt < 2; ++nt) {
+        const bool ok = fpage[nt] >= 0 && fpage[nt] < p.num_pages;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(bbase + (ok ? fpage[nt] * p.bias_cache_stride[0] + fplace[nt] * p.bias_cache_stride[1] : 0));
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int col = r0 + qc + x * 8;
+          f[nt][x] = 0u;
+          if (x == 1 && r0 + 8 >= p.R) continue;
+          if (a.factor_words) {
+            if (ok && col < p.R) f[nt][x] = *reinterpret_cast<const uint32_t*>(src + col);
+          } else {
+            if (ok && col < p.R) f[nt][x] = src[col];
+            if (ok && col + 1 < p.R) f[nt][x] |= (uint32_t)src[col + 1] << 16;
+          }
         }
       }
     };
 
     int fetched = seg.t0 * 4 + wk;
     look_up(fetched);
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) {
-      fetch(fetched, s);
-      fetched += WK;
-    }
-    if (BIAS == PAGED_FACTORS) load_factors(seg.t0 * 4 + wk, 0, kb);
+    if (BIAS == PAGED_FACTORS) factor_pages(fetched);
 
     // ---- query rows, as fragments of the products' first operand
     uint32_t q[NM][KS][4], qb[NM][4] = {};
@@ -191,6 +224,16 @@ __global__ void __launch_bounds__(kSplitThreads, 2) paged_split_kernel(const __g
     };
     if (BIAS == PAGED_FACTORS) load_qb(0);
 
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) {
+      fetch(fetched, i);
+      fetched += WK;
+    }
+    if (BIAS == PAGED_FACTORS) {
+      load_factors(0, kb);
+      factor_pages(seg.t0 * 4 + wk + WK);
+    }
+
     float o[NM][NT][4];
 #pragma unroll
     for (int im = 0; im < NM; ++im)
@@ -223,19 +266,20 @@ __global__ void __launch_bounds__(kSplitThreads, 2) paged_split_kernel(const __g
       }
       float f[NM][2][4] = {};
       if (BIAS == PAGED_FACTORS) {
-        uint16_t cur[2][4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) cur[i >> 2][i & 3] = kb[i >> 2][i & 3];
-        load_factors(tile + WK, 0, kb);
+        uint32_t cur[2][2] = {{kb[0][0], kb[0][1]}, {kb[1][0], kb[1][1]}};
+        load_factors(0, kb);
+        factor_pages(tile + 2 * WK);
         for (int r0 = 0;;) {
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const uint32_t b0 = cur[nt][0] | (uint32_t)cur[nt][1] << 16, b1 = cur[nt][2] | (uint32_t)cur[nt][3] << 16;
+          for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-            for (int im = 0; im < NM; ++im) mma16816<T>(f[im][nt], qb[im], b0, b1);
-          }
-          if (p.R <= 16 || (r0 += 16) >= p.R) break;  // (wider factors: loaded where they are used)
-          load_factors(tile, r0, cur);
+            for (int im = 0; im < NM; ++im) mma16816<T>(f[im][nt], qb[im], cur[nt][0], cur[nt][1]);
+          if (p.R <= 16 || (r0 += 16) >= p.R) break;
+          // wider factors: loaded where they are used
+          const int keep[4] = {fpage[0], fpage[1], fplace[0], fplace[1]};
+          factor_pages(tile);
+          load_factors(r0, cur);
+          fpage[0] = keep[0], fpage[1] = keep[1], fplace[0] = keep[2], fplace[1] = keep[3];
           load_qb(r0);
         }
         if (p.R > 16) load_qb(0);
@@ -439,7 +483,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2) paged_split_kernel(const __g
           }
         }
     }
-    if (!whole && seg.t0 == 0 && threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(seg.b, seg.rt, seg.hg, seg.last_cta);
+    if (!whole && seg.t0 == 0 && threadIdx.x == 0) {
+      a.desc[2 * blockIdx.x] = make_int4(seg.rt, seg.hg, seg.last_cta, 0);
+      a.desc[2 * blockIdx.x + 1] = make_int4(rq.first, rq.tokens * a.G, 0, 0);
+    }
   }
 }
 

@@ -103,7 +103,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     tmem_relinquish();
   }
   grid_dep_wait();
-  if (threadIdx.x == 0) a.desc[blockIdx.x].x = -1;
+  if (threadIdx.x == 0) a.desc[2 * blockIdx.x].x = -1;
   PagedWalk<128, 128, kTileThreads> walk;
   walk.start(a, p.Hk);
   tc_fence_before_sync();
@@ -533,7 +533,10 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!whole) a.ml[slot * 128 + row] = make_float2(m, ls);
         else if (p.lse) p.lse[(int64_t)gn * p.Hq + hd] = ls > 0.f ? (m + fast_log2(ls)) * kLn2P : ls == 0.f ? -INFINITY : ls;
       }
-      if (!whole && begins && threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(sg->b, sg->rt, sg->hg, sg->last_cta);
+      if (!whole && begins && threadIdx.x == 0) {
+        a.desc[2 * blockIdx.x] = make_int4(sg->rt, sg->hg, sg->last_cta, 0);
+        a.desc[2 * blockIdx.x + 1] = make_int4(sg->first, sg->tokens * a.G, 0, 0);
+      }
       tc_fence_before_sync();
       mbar_arrive_warp(o_free);
     }
@@ -552,13 +555,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 template <typename T, int TD>
 __global__ void __launch_bounds__(128) paged_join_tile_kernel(const __grid_constant__ PagedArgs a) {
   grid_dep_wait();
-  const int4 d = a.desc[blockIdx.x];
+  const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
   if (d.x < 0) return;
   const fb_paged_params& p = a.p;
-  const Request rq = request_at(p, d.x);
-  const int row = threadIdx.x, gr = d.y * 128 + row, col0 = blockIdx.y * 32, parts = d.w - (int)blockIdx.x + 1;
-  if (gr >= rq.tokens * a.G) return;
-  const int t = a.group_div.quot32(gr), h = d.z * a.G + gr - t * a.G, n = rq.first + t;
+  const int row = threadIdx.x, gr = d.x * 128 + row, col0 = blockIdx.y * 32, parts = d.z - (int)blockIdx.x + 1;
+  if (gr >= e.y) return;
+  const int t = a.group_div.quot32(gr), h = d.y * a.G + gr - t * a.G, n = e.x + t;
   auto slot_of = [&](int i) { return (int64_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
   float m = -INFINITY;
 #pragma unroll 4
