@@ -201,8 +201,13 @@ extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
     a.page_div = Div(p->page_size);
     a.group_div = Div(a.G);
     a.whole_tiles = p->page_size % 16 == 0;
-    a.factor_words = p->R % 2 == 0 && !(reinterpret_cast<uintptr_t>(p->bias_cache) & 3) &&
-                     !((p->bias_cache_stride[0] | p->bias_cache_stride[1] | (p->bias_heads > 1 ? p->bias_cache_stride[2] : 0)) & 1);
+    a.pages32 = (uint32_t)(p->num_pages < 0x7fffffffLL ? p->num_pages : 0x7fffffffLL);
+    if (p->R) {  // what the rows of the factors are aligned to
+      const uintptr_t bits = reinterpret_cast<uintptr_t>(p->bias_cache) |
+                             (uintptr_t)(p->bias_cache_stride[0] | p->bias_cache_stride[1] | (p->bias_heads > 1 ? p->bias_cache_stride[2] : 0) | p->R) * 2;
+      a.factor_words = !(bits & 3);
+      a.factor_bytes = p->R > 16 ? 0 : !(bits & 15) ? 16 : !(bits & 7) ? 8 : !(bits & 3) ? 4 : 0;
+    }
     a.scale_log2 = p->softmax_scale * kLog2eP;
     uint8_t* ws = reinterpret_cast<uint8_t*>(p->workspace);
     a.part = reinterpret_cast<float*>(ws);

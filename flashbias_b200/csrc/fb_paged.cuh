@@ -26,8 +26,10 @@ struct PagedArgs {
   fb_paged_params p;
   Div page_div, group_div;  // by page_size, by the query heads of a key head
   int G;                    // query heads of a key head
-  int whole_tiles;          // split kernel: pages are whole tiles of 16 keys
+  int whole_tiles;          // split kernel: pages are whole runs of 16 keys
+  uint32_t pages32;         // num_pages, within 31 bits: what a page of the table is compared with
   int factor_words;         // split kernel: factor rows can be read two columns at a time
+  int factor_bytes;         // split kernel: pieces in which a key's factors are copied; 0: not
   float scale_log2;
   float* part;    // (CTAs, 2, heads of a group, rows of a tile, columns): sums of items that span CTAs
   float2* ml;     // the same without columns: maximum (log2 units) and sum
@@ -189,14 +191,15 @@ int launch_paged_tile_d128(const PagedArgs& a, const PagedPlan& plan, cudaStream
 // Joins the parts of the item that begins in CTA blockIdx.x; a warp per row, the parts in the order of the CTAs.  Latency is
 // all there is to it: what the rows need stands in the descriptor, and the first parts are on their way before the maximum is
 // known.
+constexpr int kJoinThreads = 128;  // (of 512 an SM holds one, and most have nothing to join)
 template <typename T, int TD>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a, const int WH, const int MT) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, const int WH, const int MT) {
   constexpr int C = TD / 32, U = 8;  // columns of a lane, parts in flight
   grid_dep_wait();
   const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
   if (d.x < 0) return;
   const fb_paged_params& p = a.p;
-  const int lane = threadIdx.x & 31, idx = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, idx = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5);
   const int wh = idx / MT, r = idx - wh * MT, gr = d.x * MT + r, parts = d.z - (int)blockIdx.x + 1;
   if (gr >= e.y) return;
   const int64_t step = (int64_t)2 * WH * MT;  // rows of a CTA
@@ -261,9 +264,9 @@ int launch_pdl_2d(void (*kern)(P...), dim3 grid, unsigned block, cudaStream_t st
 // (an item may begin in any CTA and end in a later one)
 template <int TD>
 int launch_paged_join(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
-  const dim3 grid(plan.ctas, plan.WH * plan.MT / 4);
-  return a.p.dtype == FB_DTYPE_F16 ? launch_pdl_2d(paged_join_kernel<__half, TD>, grid, 128, st, a, plan.WH, plan.MT)
-                                   : launch_pdl_2d(paged_join_kernel<__nv_bfloat16, TD>, grid, 128, st, a, plan.WH, plan.MT);
+  const dim3 grid(plan.ctas, plan.WH * plan.MT / (kJoinThreads / 32));
+  return a.p.dtype == FB_DTYPE_F16 ? launch_pdl_2d(paged_join_kernel<__half, TD>, grid, kJoinThreads, st, a, plan.WH, plan.MT)
+                                   : launch_pdl_2d(paged_join_kernel<__nv_bfloat16, TD>, grid, kJoinThreads, st, a, plan.WH, plan.MT);
 }
 
 }  // namespace fb

@@ -1,6 +1,6 @@
 // Attention over pages with few rows per key head (up to 32): decoding, and small trees or runs of drafted tokens.
 //
-// Bound by reading K and V once.  A warp works alone: it owns a head of the CTA's group and every WK-th tile of 16 keys, copies
+// Bound by reading K and V once.  A warp works alone: it owns a head of the CTA's group and every WK-th tile of 16 or 32 keys, copies
 // them into a ring of its own in shared memory (cp.async, so that what is in flight is bounded by shared memory and not by
 // registers: 2 CTAs x 96 KB per SM), and keeps 16 or 32 query rows, the row maxima and sums and the output in registers.  The
 // products are mma.sync m16n8k16: a tile of 16 keys and 16 rows is one fragment wide, S stays in the registers that P is fed
@@ -17,14 +17,17 @@ namespace fb {
 
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = 32 * kSplitWarps;
-constexpr int kSplitKT = 64;  // keys of a scheduled tile: four sub-tiles of 16
+constexpr int kSplitKT = 64;  // keys of a scheduled tile: several steps of a warp
 
-template <int TD>
+template <int TD, int MT>
 struct SplitCfg {
+  static constexpr int KT = TD == 128 ? 16 : 32;                         // keys of a step
   static constexpr int ROW = TD * 2;                                     // bytes of a key's row
-  static constexpr int ST = TD == 128 ? 3 : 4;                           // ring stages
-  static constexpr int HALF = 16 * ROW, STAGE = 2 * HALF, RING = ST * STAGE;  // K, then V
-  static constexpr int SMEM = kSplitWarps * RING + kSplitWarps * ST * 4;
+  static constexpr int ST = TD == 64 && MT == 16 ? 2 : 3;                // ring stages
+  static constexpr int HALF = KT * ROW, STAGE = 2 * HALF, RING = ST * STAGE;  // K, then V
+  static constexpr int F_ROW = 32, F_STAGE = KT * F_ROW;                 // factors: 16 columns, zeros behind the last
+  static constexpr int OFF_F = kSplitWarps * RING, OFF_OK = OFF_F + kSplitWarps * ST * F_STAGE;
+  static constexpr int smem(bool factors) { return factors ? OFF_OK + kSplitWarps * ST * 4 : OFF_F + kSplitWarps * ST * 4; }
   static constexpr int CH = TD / 8;  // 16-byte chunks of a row
   // chunk c of key r: XOR-swizzled so that eight rows of one column of chunks fall on different banks
   __device__ static __forceinline__ uint32_t at(int r, int c) {
@@ -54,17 +57,26 @@ __device__ __forceinline__ bool pair_not_finite(uint32_t w) {
   return (w & E) == E || ((w >> 16) & E) == E;
 }
 
-enum { PAGED_PLAIN = 0, PAGED_SLOPES = 1, PAGED_FACTORS = 2 };
+// PAGED_FACTORS: up to 16 columns in rows that can be copied in pieces of 4, 8 or 16 bytes, beside the keys in the ring;
+// PAGED_FACTORS_ANY: any others, read into registers.
+enum { PAGED_PLAIN, PAGED_SLOPES, PAGED_FACTORS, PAGED_FACTORS_ANY };
 
 template <typename T, int TD, int MT, int BIAS>
 __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split_kernel(const __grid_constant__ PagedArgs a, const int WH) {
-  using Cfg = SplitCfg<TD>;
-  constexpr int NM = MT / 16, KS = TD / 16, NT = TD / 8, ST = Cfg::ST;
+  using Cfg = SplitCfg<TD, MT>;
+  constexpr int NM = MT / 16, KS = TD / 16, NT = TD / 8, ST = Cfg::ST, KT = Cfg::KT, NK = KT / 16, PER = kSplitKT / KT;
+  constexpr uint32_t ALL = KT == 32 ? 0xffffffffu : 0xffffu;
   extern __shared__ __align__(1024) uint8_t smem[];
   const fb_paged_params& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, WK = kSplitWarps / WH, wh = warp / WK, wk = warp % WK;
   const uint32_t ring = smem_u32(smem) + warp * Cfg::RING;
-  uint32_t* ring_ok = reinterpret_cast<uint32_t*>(smem + kSplitWarps * Cfg::RING) + warp * ST;  // keys of a stage that exist, as bits
+  // keys of a stage that exist, as bits; the factors' ring
+  uint32_t* ring_ok = reinterpret_cast<uint32_t*>(smem + (BIAS == PAGED_FACTORS ? Cfg::OFF_OK : Cfg::OFF_F)) + warp * ST;
+  const uint32_t fring = smem_u32(smem) + Cfg::OFF_F + warp * ST * Cfg::F_STAGE;
+  if (BIAS == PAGED_FACTORS) {
+    for (int i = lane; i < ST * Cfg::F_STAGE / 16; i += 32) st_shared_v4(fring + i * 16, 0u, 0u, 0u, 0u);
+    __syncwarp();
+  }
   const int qr = lane >> 2, qc = 2 * (lane & 3);  // a fragment's row (and row + 8) and first column of this lane
   grid_dep_wait();
   if (threadIdx.x == 0) a.desc[2 * blockIdx.x].x = -1;
@@ -79,19 +91,18 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
     const T* vbase = reinterpret_cast<const T*>(p.value_cache) + hk * p.value_cache_stride[2];
     const T* bbase = reinterpret_cast<const T*>(p.bias_cache) + (p.bias_heads > 1 ? hk * p.bias_cache_stride[2] : 0);
     const int32_t* table = p.block_table + (int64_t)min(seg.b, p.B - 1) * p.table_stride;
-    const int tile_end = min(seg.t1 * 4, (rq.keys + 15) >> 4);
+    const int tile_end = min(seg.t1 * PER, (rq.keys + KT - 1) / KT);
 
-    // ---- copies: the pages of a tile's keys are looked up one tile ahead of their use (lane & 15 = key).  Where pages are whole
-    // tiles one page serves all lanes, and a copy's address is one addition: half of the instructions that a tile of 64 columns
-    // takes would otherwise go into addresses.
+    // ---- copies: the pages of a tile's keys are looked up one tile ahead of their use (lane % KT = key).  Where pages are whole
+    // runs of 16 keys one page serves a run, and a copy's address is one addition: half of the instructions that a tile of 64
+    // columns takes would otherwise go into addresses.
     const int c = lane % Cfg::CH, kr = lane / Cfg::CH;  // this lane's chunk, and its key in the first of a tile's copies
     const bool in = c * 8 < p.D;
     const int64_t kstep = (32 / Cfg::CH) * p.key_cache_stride[1], vstep = (32 / Cfg::CH) * p.value_cache_stride[1];
     const T *klane = kbase + kr * p.key_cache_stride[1] + (in ? c * 8 : 0), *vlane = vbase + kr * p.value_cache_stride[1] + (in ? c * 8 : 0);
-    const uint32_t dst0 = ring + Cfg::at(kr, c);
     int page_next = -1, place_next = 0;
     auto look_up = [&](int tile) {
-      const int j = tile * 16 + (a.whole_tiles ? 0 : lane & 15);
+      const int j = tile * KT + (a.whole_tiles ? lane & (KT - 16) : lane & (KT - 1));
       page_next = -1;
       if (tile < tile_end && j < rq.keys) {
         const int col = a.page_div.quot32(j);
@@ -99,34 +110,53 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
         page_next = table[col];
       }
     };
+    // the factors of the key lane % KT, whose page and place (or those of its run) this lane holds
+    auto fetch_factors = [&](int stage, bool ok, int page, int place) {
+      const char* src = reinterpret_cast<const char*>(bbase + (ok ? page * p.bias_cache_stride[0] + place * p.bias_cache_stride[1] : 0));
+      const uint32_t dst = fring + stage * Cfg::F_STAGE + (lane & (KT - 1)) * Cfg::F_ROW, live = ok ? 0xffffffffu : 0u;
+      if (KT == 16 && lane >= 16) return;
+      if (a.factor_bytes == 16) {
+        for (int i = 0; i < 2 * p.R; i += 16) asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i), "l"(src + i), "r"(live & 16u) : "memory");
+      } else if (a.factor_bytes == 8) {
+        for (int i = 0; i < 2 * p.R; i += 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + i), "l"(src + i), "r"(live & 8u) : "memory");
+      } else {
+        for (int i = 0; i < 2 * p.R; i += 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + i), "l"(src + i), "r"(live & 4u) : "memory");
+      }
+    };
     auto fetch = [&](int tile, int stage) {
       if (tile < tile_end) {
         const int page = page_next, place = place_next;
         const uint32_t dst = ring + stage * Cfg::STAGE;
-        if (a.whole_tiles && tile * 16 + 16 <= rq.keys && (uint32_t)page < (uint32_t)min(p.num_pages, (int64_t)0x7fffffff)) {
+        if (a.whole_tiles && tile * KT + KT <= rq.keys && __all_sync(0xffffffffu, (uint32_t)page < a.pages32)) {
           look_up(tile + WK);
-          if (lane == 0) ring_ok[stage] = 0xffffu;
-          const T* k = klane + page * p.key_cache_stride[0] + place * p.key_cache_stride[1];
-          const T* v = vlane + page * p.value_cache_stride[0] + place * p.value_cache_stride[1];
+          if (lane == 0) ring_ok[stage] = ALL;
+          if (BIAS == PAGED_FACTORS) fetch_factors(stage, true, page, place + (lane & 15));
 #pragma unroll
-          for (int i = 0; i < TD / 16; ++i) {
-            const uint32_t at = dst + Cfg::at(kr + i * (32 / Cfg::CH), c);
-            cp_async16_zfill(at, k, in);
-            cp_async16_zfill(at + Cfg::HALF, v, in);
-            k += kstep;
-            v += vstep;
+          for (int h = 0; h < NK; ++h) {
+            const int pg = NK > 1 ? __shfl_sync(0xffffffffu, page, h * 16) : page, pl = NK > 1 ? __shfl_sync(0xffffffffu, place, h * 16) : place;
+            const T* k = klane + pg * p.key_cache_stride[0] + pl * p.key_cache_stride[1];
+            const T* v = vlane + pg * p.value_cache_stride[0] + pl * p.value_cache_stride[1];
+#pragma unroll
+            for (int i = 0; i < TD / 16; ++i) {
+              const uint32_t at = dst + Cfg::at(kr + i * (32 / Cfg::CH), c) + h * 16 * Cfg::ROW;
+              cp_async16_zfill(at, k, in);
+              cp_async16_zfill(at + Cfg::HALF, v, in);
+              k += kstep;
+              v += vstep;
+            }
           }
         } else {
           const int off = a.whole_tiles ? lane & 15 : 0;
-          const bool there = tile * 16 + (lane & 15) < rq.keys, ok = there && page >= 0 && page < p.num_pages;
+          const bool there = tile * KT + (lane & (KT - 1)) < rq.keys, ok = there && (uint32_t)page < a.pages32;
           if (there && !ok) paged_bad_index(p);
           const int64_t ko = ok ? page * p.key_cache_stride[0] + (place + off) * p.key_cache_stride[1] : 0;
           const int64_t vo = ok ? page * p.value_cache_stride[0] + (place + off) * p.value_cache_stride[1] : 0;
-          const uint32_t okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+          const uint32_t okm = __ballot_sync(0xffffffffu, ok) & ALL;
           if (lane == 0) ring_ok[stage] = okm;
           look_up(tile + WK);
+          if (BIAS == PAGED_FACTORS) fetch_factors(stage, ok, page, place + off);
 #pragma unroll
-          for (int i = 0; i < TD / 16; ++i) {
+          for (int i = 0; i < TD * NK / 16; ++i) {
             const int key = kr + i * (32 / Cfg::CH);
             const int64_t k = __shfl_sync(0xffffffffu, ko, key), v = __shfl_sync(0xffffffffu, vo, key);
             const bool live = in && ((okm >> key) & 1);
@@ -139,13 +169,21 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
     };
     // Factors of a tile's keys in the layout of the product's second operand (two columns a word), one tile ahead; their pages
     // two ahead.
-    uint32_t kb[2][2] = {};
-    int fpage[2] = {-1, -1}, fplace[2] = {};
+    uint32_t kb[2 * NK][2] = {};
+    int fpage[2 * NK], fplace[2 * NK];  // (of eight keys each)
+    const uint16_t* const blane = reinterpret_cast<const uint16_t*>(bbase) + qc;
     auto factor_pages = [&](int tile) {
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const int j = tile * 16 + nt * 8 + qr;
+      for (int nt = 0; nt < 2 * NK; ++nt) {
+        const int j = tile * KT + nt * 8 + qr;
+        if ((nt & 1) && a.whole_tiles) {  // the run's other eight
+          fpage[nt] = fpage[nt - 1];
+          fplace[nt] = fplace[nt - 1] + 8;
+          if (j >= rq.keys) fpage[nt] = -1;
+          continue;
+        }
         fpage[nt] = -1;
+        fplace[nt] = 0;
         if (tile < tile_end && j < rq.keys) {
           const int col = a.page_div.quot32(j);
           fplace[nt] = j - col * p.page_size;
@@ -153,29 +191,29 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
         }
       }
     };
-    auto load_factors = [&](int r0, uint32_t (&f)[2][2]) {
+    auto load_factors = [&](int r0, uint32_t (&f)[2 * NK][2]) {
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const bool ok = fpage[nt] >= 0 && fpage[nt] < p.num_pages;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(bbase + (ok ? fpage[nt] * p.bias_cache_stride[0] + fplace[nt] * p.bias_cache_stride[1] : 0));
+      for (int nt = 0; nt < 2 * NK; ++nt) {
+        const bool ok = (uint32_t)fpage[nt] < a.pages32;
+        const uint16_t* src = blane + r0 + (ok ? fpage[nt] * p.bias_cache_stride[0] + fplace[nt] * p.bias_cache_stride[1] : 0);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int col = r0 + qc + x * 8;
           f[nt][x] = 0u;
           if (x == 1 && r0 + 8 >= p.R) continue;
           if (a.factor_words) {
-            if (ok && col < p.R) f[nt][x] = *reinterpret_cast<const uint32_t*>(src + col);
+            if (ok && col < p.R) f[nt][x] = *reinterpret_cast<const uint32_t*>(src + x * 8);
           } else {
-            if (ok && col < p.R) f[nt][x] = src[col];
-            if (ok && col + 1 < p.R) f[nt][x] |= (uint32_t)src[col + 1] << 16;
+            if (ok && col < p.R) f[nt][x] = src[x * 8];
+            if (ok && col + 1 < p.R) f[nt][x] |= (uint32_t)src[x * 8 + 1] << 16;
           }
         }
       }
     };
 
-    int fetched = seg.t0 * 4 + wk;
+    int fetched = seg.t0 * PER + wk;
     look_up(fetched);
-    if (BIAS == PAGED_FACTORS) factor_pages(fetched);
+    if (BIAS == PAGED_FACTORS_ANY) factor_pages(fetched);
 
     // ---- query rows, as fragments of the products' first operand
     uint32_t q[NM][KS][4], qb[NM][4] = {};
@@ -203,7 +241,7 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
           slope2[im][e] = p.slopes[h] * kLog2eP;
           my_pos[im][e] = p.positions ? p.positions[n] : rq.len + t;
         }
-        if (BIAS == PAGED_FACTORS) {
+        if (BIAS >= PAGED_FACTORS) {
           qbrow[im][e] = live ? reinterpret_cast<const T*>(p.q_bias) + n * p.q_bias_stride[0] + h * p.q_bias_stride[1] : nullptr;
         }
       }
@@ -222,16 +260,16 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
             qb[im][e + 2 * x] = w;
           }
     };
-    if (BIAS == PAGED_FACTORS) load_qb(0);
+    if (BIAS >= PAGED_FACTORS) load_qb(0);
 
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) {
       fetch(fetched, i);
       fetched += WK;
     }
-    if (BIAS == PAGED_FACTORS) {
+    if (BIAS == PAGED_FACTORS_ANY) {
       load_factors(0, kb);
-      factor_pages(seg.t0 * 4 + wk + WK);
+      factor_pages(seg.t0 * PER + wk + WK);
     }
 
     float o[NM][NT][4];
@@ -240,8 +278,11 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[im][i][0] = o[im][i][1] = o[im][i][2] = o[im][i][3] = 0.f;
 
+    // lanes' addresses in a stage; the k-step or pair of column blocks i is an XOR of i << 5 away (rows begin at multiples of it)
+    const uint32_t k_at = Cfg::at((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1), v_at = Cfg::at(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
+    const uint32_t f_at = ((lane >> 4) * 8 + (lane & 7)) * Cfg::F_ROW + ((lane >> 3) & 1) * 16;
     int stage = 0, fill = ST - 1;
-    for (int tile = seg.t0 * 4 + wk; tile < tile_end; tile += WK) {
+    for (int tile = seg.t0 * PER + wk; tile < tile_end; tile += WK) {
       asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
       __syncwarp();  // every lane's copies have landed, and the stage read last has been read by all
       const uint32_t okm = ring_ok[stage];
@@ -251,87 +292,111 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
       const uint32_t ks_base = ring + stage * Cfg::STAGE, vs_base = ks_base + Cfg::HALF;
       stage = stage + 1 == ST ? 0 : stage + 1;
 
-      // ---- S = Q K^T
-      float s[NM][2][4] = {};
+      // ---- S = Q K^T (columns beyond D hold zeros)
+      float s[NM][2 * NK][4] = {};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        if (TD > 32 && ks * 16 >= p.D) break;
-        uint32_t b[4];
-        ldsm4(ks_base + Cfg::at((lane >> 4) * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)), b);
+      for (int h = 0; h < NK; ++h)
 #pragma unroll
-        for (int im = 0; im < NM; ++im) {
-          mma16816<T>(s[im][0], q[im][ks], b[0], b[1]);
-          mma16816<T>(s[im][1], q[im][ks], b[2], b[3]);
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t b[4];
+          ldsm4((ks_base + h * 16 * Cfg::ROW + k_at) ^ (ks << 5), b);
+#pragma unroll
+          for (int im = 0; im < NM; ++im) {
+            mma16816<T>(s[im][2 * h], q[im][ks], b[0], b[1]);
+            mma16816<T>(s[im][2 * h + 1], q[im][ks], b[2], b[3]);
+          }
+        }
+      float f[NM][2 * NK][4] = {};
+      if (BIAS == PAGED_FACTORS) {
+        const uint32_t fb = fring + (ks_base - ring) / Cfg::STAGE * Cfg::F_STAGE;
+#pragma unroll
+        for (int h = 0; h < NK; ++h) {
+          uint32_t b[4];
+          ldsm4(fb + h * 16 * Cfg::F_ROW + f_at, b);
+#pragma unroll
+          for (int im = 0; im < NM; ++im) {
+            mma16816<T>(f[im][2 * h], qb[im], b[0], b[1]);
+            mma16816<T>(f[im][2 * h + 1], qb[im], b[2], b[3]);
+          }
         }
       }
-      float f[NM][2][4] = {};
-      if (BIAS == PAGED_FACTORS) {
-        uint32_t cur[2][2] = {{kb[0][0], kb[0][1]}, {kb[1][0], kb[1][1]}};
+      if (BIAS == PAGED_FACTORS_ANY) {
+        uint32_t cur[2 * NK][2];
+#pragma unroll
+        for (int i = 0; i < 2 * NK; ++i) cur[i][0] = kb[i][0], cur[i][1] = kb[i][1];
         load_factors(0, kb);
-        factor_pages(tile + 2 * WK);
         for (int r0 = 0;;) {
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
+          for (int nt = 0; nt < 2 * NK; ++nt)
 #pragma unroll
             for (int im = 0; im < NM; ++im) mma16816<T>(f[im][nt], qb[im], cur[nt][0], cur[nt][1]);
           if (p.R <= 16 || (r0 += 16) >= p.R) break;
-          // wider factors: loaded where they are used
-          const int keep[4] = {fpage[0], fpage[1], fplace[0], fplace[1]};
-          factor_pages(tile);
+          factor_pages(tile);  // wider factors: loaded where they are used
           load_factors(r0, cur);
-          fpage[0] = keep[0], fpage[1] = keep[1], fplace[0] = keep[2], fplace[1] = keep[3];
           load_qb(r0);
         }
         if (p.R > 16) load_qb(0);
+        factor_pages(tile + 2 * WK);
       }
 
       // ---- logits in log2 units; masks where the tile holds new tokens' keys or keys that do not exist
-      const int j0 = tile * 16 + qc;
-      const bool masked = okm != 0xffffu || tile * 16 + 16 > rq.len;
+      const int j0 = tile * KT + qc;
+      const bool masked = okm != ALL || tile * KT + KT > rq.len;
 #pragma unroll
       for (int im = 0; im < NM; ++im)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int nt = 0; nt < 2 * NK; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int e = i >> 1, j = j0 + nt * 8 + (i & 1);
             float v = s[im][nt][i] * a.scale_log2;
-            if (BIAS == PAGED_SLOPES) {
-              int pos = j;
-              if (masked && p.positions && j >= rq.len && j < rq.keys) pos = p.positions[rq.first + j - rq.len];
-              v = fmaf(slope2[im][e], (float)(pos - my_pos[im][e]), v);
-            }
-            if (BIAS == PAGED_FACTORS) v = fmaf(f[im][nt][i], kLog2eP, v);
-            if (masked) {
-              bool seen = (okm >> (j - tile * 16)) & 1;
-              if (seen && j >= rq.len) seen = row_tok[im][e] >= 0 && tree_sees(p, rq.first + row_tok[im][e], row_tok[im][e], j - rq.len);
-              if (!seen) v = -INFINITY;
-            }
+            if (BIAS == PAGED_SLOPES) v = fmaf(slope2[im][i >> 1], (float)(j0 + nt * 8 + (i & 1) - my_pos[im][i >> 1]), v);
+            if (BIAS >= PAGED_FACTORS) v = fmaf(f[im][nt][i], kLog2eP, v);
             s[im][nt][i] = v;
           }
+      if (masked) {
+#pragma unroll
+        for (int im = 0; im < NM; ++im)
+#pragma unroll
+          for (int nt = 0; nt < 2 * NK; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int e = i >> 1, j = j0 + nt * 8 + (i & 1);
+              bool seen = (okm >> (j - tile * KT)) & 1;
+              if (seen && j >= rq.len) {
+                seen = row_tok[im][e] >= 0 && tree_sees(p, rq.first + row_tok[im][e], row_tok[im][e], j - rq.len);
+                if (BIAS == PAGED_SLOPES && p.positions)  // the key's position instead of its place
+                  s[im][nt][i] = fmaf(slope2[im][e], (float)(p.positions[rq.first + j - rq.len] - j), s[im][nt][i]);
+              }
+              if (!seen) s[im][nt][i] = -INFINITY;
+            }
+      }
 
       // ---- running maximum and sum, P as fragments
-      uint32_t pf[NM][4];
+      uint32_t pf[NM][NK][4];
       bool grown = false;
       float alpha[NM][2];
 #pragma unroll
       for (int im = 0; im < NM; ++im)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(s[im][0][2 * e], s[im][0][2 * e + 1]), fmaxf(s[im][1][2 * e], s[im][1][2 * e + 1]));
+          float mx = m[im][e];
+#pragma unroll
+          for (int nt = 0; nt < 2 * NK; ++nt) mx = fmax3(mx, s[im][nt][2 * e], s[im][nt][2 * e + 1]);
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          mx = fmaxf(mx, m[im][e]);
           grown |= mx > m[im][e];
           const float msub = fmaxf(mx, -FLT_MAX);  // no visible key yet: every exponential is zero
           alpha[im][e] = fast_exp2(m[im][e] - msub);
           m[im][e] = mx;
-          const float p0 = fast_exp2(s[im][0][2 * e] - msub), p1 = fast_exp2(s[im][0][2 * e + 1] - msub);
-          const float p2 = fast_exp2(s[im][1][2 * e] - msub), p3 = fast_exp2(s[im][1][2 * e + 1] - msub);
-          l[im][e] = fmaf(l[im][e], alpha[im][e], (p0 + p1) + (p2 + p3));
-          // the probabilities are rounded to the 16 bits of V: half a step of relative error each, what the result is rounded by
-          pf[im][e] = Pack2<T>::pack(p0, p1);
-          pf[im][2 + e] = Pack2<T>::pack(p2, p3);
+          float sum = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < 2 * NK; ++nt) {
+            const float p0 = fast_exp2(s[im][nt][2 * e] - msub), p1 = fast_exp2(s[im][nt][2 * e + 1] - msub);
+            sum += p0 + p1;
+            // the probabilities are rounded to the 16 bits of V: half a step of relative error each, what the result is rounded by
+            pf[im][nt >> 1][2 * (nt & 1) + e] = Pack2<T>::pack(p0, p1);
+          }
+          l[im][e] = fmaf(l[im][e], alpha[im][e], sum);
         }
       if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -350,8 +415,8 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
       bool odd = false;
       if (masked) {
         bool mine = false;
-#pragma unroll
-        for (int i = 0; i < TD / 16; ++i) {
+#pragma unroll 1
+        for (int i = 0; i < Cfg::HALF / 512; ++i) {
           const uint4 w = *reinterpret_cast<const uint4*>(smem + warp * Cfg::RING + (vs_base - ring) + (i * 32 + lane) * 16);
           mine |= pair_not_finite<T>(w.x) || pair_not_finite<T>(w.y) || pair_not_finite<T>(w.z) || pair_not_finite<T>(w.w);
         }
@@ -359,26 +424,31 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
       }
       if (!odd) {
 #pragma unroll
-        for (int np = 0; np < KS; ++np) {
-          if (TD > 32 && np * 16 >= p.D) break;
-          uint32_t b[4];
-          ldsm4t(vs_base + Cfg::at(((lane >> 3) & 1) * 8 + (lane & 7), np * 2 + (lane >> 4)), b);
+        for (int h = 0; h < NK; ++h)
 #pragma unroll
-          for (int im = 0; im < NM; ++im) {
-            mma16816<T>(o[im][2 * np], pf[im], b[0], b[1]);
-            mma16816<T>(o[im][2 * np + 1], pf[im], b[2], b[3]);
+          for (int np = 0; np < KS; ++np) {
+            uint32_t b[4];
+            ldsm4t((vs_base + h * 16 * Cfg::ROW + v_at) ^ (np << 5), b);
+#pragma unroll
+            for (int im = 0; im < NM; ++im) {
+              mma16816<T>(o[im][2 * np], pf[im][h], b[0], b[1]);
+              mma16816<T>(o[im][2 * np + 1], pf[im][h], b[2], b[3]);
+            }
           }
-        }
       } else {
 #pragma unroll 1
-        for (int k = 0; k < 16; ++k) {
-          const int src = (lane & ~3) | ((k & 7) >> 1);
+        for (int k = 0; k < KT; ++k) {
+          const int src = (lane & ~3) | ((k & 7) >> 1), at = k >> 3;  // the fragment's lane and half
           float pk[NM][2];
 #pragma unroll
           for (int im = 0; im < NM; ++im)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint32_t w = __shfl_sync(0xffffffffu, k < 8 ? pf[im][e] : pf[im][2 + e], src);
+              uint32_t w = pf[im][0][e];
+#pragma unroll
+              for (int x = 1; x < 2 * NK; ++x)
+                if (at == x) w = pf[im][x >> 1][2 * (x & 1) + e];
+              w = __shfl_sync(0xffffffffu, w, src);
               const uint16_t h = (uint16_t)(k & 1 ? w >> 16 : w);
               pk[im][e] = to_f32(*reinterpret_cast<const T*>(&h));
             }
@@ -493,6 +563,7 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
 template <typename T, int TD, int MT, int BIAS>
 int launch_paged_split_t(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
   auto kern = paged_split_kernel<T, TD, MT, BIAS>;
+  constexpr int SMEM = SplitCfg<TD, MT>::smem(BIAS == PAGED_FACTORS);
   static std::mutex mu;
   static bool attr_done[64] = {};
   int dev = 0;
@@ -500,12 +571,12 @@ int launch_paged_split_t(const PagedArgs& a, const PagedPlan& plan, cudaStream_t
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!attr_done[dev & 63]) {
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<TD>::SMEM);
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
       if (e != cudaSuccess) return (int)e;
       attr_done[dev & 63] = true;
     }
   }
-  if (const int rc = launch_pdl(kern, plan.ctas, kSplitThreads, SplitCfg<TD>::SMEM, st, a, plan.WH)) return rc;
+  if (const int rc = launch_pdl(kern, plan.ctas, kSplitThreads, SMEM, st, a, plan.WH)) return rc;
   return launch_paged_join<TD>(a, plan, st);
 }
 
@@ -515,8 +586,9 @@ int launch_paged_split(const PagedArgs& a, const PagedPlan& plan, cudaStream_t s
     using T = decltype(t);
     constexpr int MT = decltype(mt)::value;
     return a.p.slopes ? launch_paged_split_t<T, TD, MT, PAGED_SLOPES>(a, plan, st)
-           : a.p.R    ? launch_paged_split_t<T, TD, MT, PAGED_FACTORS>(a, plan, st)
-                      : launch_paged_split_t<T, TD, MT, PAGED_PLAIN>(a, plan, st);
+           : a.p.R && a.factor_bytes ? launch_paged_split_t<T, TD, MT, PAGED_FACTORS>(a, plan, st)
+           : a.p.R                   ? launch_paged_split_t<T, TD, MT, PAGED_FACTORS_ANY>(a, plan, st)
+                                     : launch_paged_split_t<T, TD, MT, PAGED_PLAIN>(a, plan, st);
   };
   auto by_rows = [&](auto t) {
     return plan.MT == 16 ? by_bias(t, std::integral_constant<int, 16>()) : by_bias(t, std::integral_constant<int, 32>());
