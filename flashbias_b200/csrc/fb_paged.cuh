@@ -82,6 +82,11 @@ struct Segment {
   Request r;
 };
 
+// 64-bit numbers that are 32 bits long almost always: their division is four times as long otherwise.
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+  return ((n | d) >> 32) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
+}
+
 // Walks the segments of one CTA.  Every thread of the block calls it alike.
 template <int KT, int MT, int THREADS>
 struct PagedWalk {
@@ -100,10 +105,12 @@ struct PagedWalk {
   __device__ __forceinline__ void start(const PagedArgs& a, int groups) {
     __shared__ int64_t s_sum[THREADS / 32], s_pre;
     __shared__ int s_b;
+    __shared__ Request s_r;
     ngroups = groups;
     const int n = a.p.B + 2, per = (n + THREADS - 1) / THREADS, b0 = threadIdx.x * per, b1 = min(b0 + per, n);
     int64_t mine = 0;
-    for (int i = b0; i < b1; ++i) mine += units(a, request_at(a.p, i), groups);
+    Request mr = {0, 0, -1, 0};  // the last of the run: all of it while there are fewer requests than threads
+    for (int i = b0; i < b1; ++i) mine += units(a, mr = request_at(a.p, i), groups);
     int64_t x = mine;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -122,23 +129,24 @@ struct PagedWalk {
       total += s_sum[w];
     }
     ctas = (int)min((int64_t)gridDim.x, total);  // each of these has one number at least: an item's parts leave no gap
-    u = blockIdx.x < ctas ? (int64_t)blockIdx.x * total / ctas : total;
-    u1 = blockIdx.x < ctas ? (int64_t)(blockIdx.x + 1) * total / ctas : total;
+    u = blockIdx.x < ctas ? quotient(blockIdx.x * total, ctas) : total;
+    u1 = blockIdx.x < ctas ? quotient((blockIdx.x + 1) * total, ctas) : total;
     if (u < u1 && before <= u && u < before + mine) {
       int64_t at = before;
       int i = b0;
-      for (;; ++i) {
-        const int64_t k = units(a, request_at(a.p, i), groups);
+      for (; per > 1; ++i) {
+        const int64_t k = units(a, mr = request_at(a.p, i), groups);
         if (u < at + k) break;
         at += k;
       }
       s_b = i;
       s_pre = at;
+      s_r = mr;
     }
     __syncthreads();
     b = s_b;
     pre = s_pre;
-    if (u < u1) r = request_at(a.p, b);
+    r = s_r;
   }
 
   __device__ __forceinline__ bool next(const PagedArgs& a, Segment& s) {
@@ -151,14 +159,14 @@ struct PagedWalk {
     s.b = b;
     s.r = r;
     s.tiles = key_tiles(r);
-    const int64_t local = u - pre, item = local / s.tiles;
+    const int64_t local = u - pre, item = quotient(local, s.tiles);
     const int rts = row_tiles(a, r);
-    s.hg = (int)(item / rts);
+    s.hg = (int)quotient(item, rts);
     s.rt = (int)(item - (int64_t)s.hg * rts);
     s.t0 = (int)(local - item * s.tiles);
     s.t1 = (int)min((int64_t)s.tiles, s.t0 + (u1 - u));
     const int64_t end = pre + (item + 1) * s.tiles;  // CTA c holds number n if c U / C <= n: the last one for n = end - 1
-    s.last_cta = (int)((end * ctas - 1) / total);
+    s.last_cta = (int)quotient(end * ctas - 1, total);
     u += s.t1 - s.t0;
     return true;
   }

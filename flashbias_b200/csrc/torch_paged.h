@@ -448,7 +448,10 @@ std::tuple<Tensor, OptTensor> paged_forward(const Tensor& q_, const Tensor& key_
   }
   if (slopes_) {
     FB_ASSERT(!q_bias_, "slopes and factors exclude each other");
-    slopes = slopes_->detach().to(q.device(), at::kFloat).reshape({-1}).contiguous();
+    // (as it is in the common case: the conversions, which do nothing then, cost three trips through the dispatcher)
+    slopes = slopes_->scalar_type() == at::kFloat && slopes_->device() == q.device() && slopes_->is_contiguous()
+                 ? *slopes_
+                 : slopes_->detach().to(q.device(), at::kFloat).reshape({-1}).contiguous();
     FB_ASSERT(slopes.numel() == Hq, "one slope per head");
     p.slopes = slopes.data_ptr<float>();
   }
