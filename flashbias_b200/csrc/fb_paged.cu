@@ -152,7 +152,7 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
   // pages (or a page of whole tiles) that TMA can address, and the scale may be taken out of a maximum.
   const bool tma = tma_compatible(p->key_cache, p->key_cache_stride[1], p->key_cache_stride[2], p->key_cache_stride[0], p->Hk, p->num_pages) &&
                    tma_compatible(p->value_cache, p->value_cache_stride[1], p->value_cache_stride[2], p->value_cache_stride[0], p->Hk, p->num_pages);
-  if (rows > 32 && tma && p->R == 0 && p->softmax_scale > 0.f && p->page_size % 8 == 0 && (128 % p->page_size == 0 || p->page_size % 128 == 0) &&
+  if (rows > 32 && tma && p->R == 0 && p->softmax_scale > 1e-20f && p->page_size % 8 == 0 && (128 % p->page_size == 0 || p->page_size % 128 == 0) &&
       p->num_pages < 0x7fffffffLL) {
     plan.kernel = PAGED_TILE;
     plan.TD = p->D <= 64 ? 64 : 128;

@@ -5,12 +5,12 @@
 // turn, with logits and probabilities of their own in tensor memory, one output accumulator and one running reference maximum
 // per row that they hand to one another behind each tile's row maximum.
 //   warps 0-3, 4-7  softmax of the even / odd key tiles, thread = row; epilogue
-//   warp 8          walks the schedule, one segment ahead of all others; TMA producer: a copy per page (and 64 columns), a lane
-//                   looks up a page
+//   warp 8          walks the schedule, one segment ahead of all others; copies of K: TMA, one per page (and 64 columns), a lane
+//                   looks up a page.  K does not wait for V's ring: the logits run ahead of the products P.V
 //   warp 9          S = Q.K^T          warp 10   O += P.V
-//   warp 11         the next segment's queries; V behind its copy: places that hold no key become zero, and so do values that are
-//                   not finite where not every row sees the key (0 x inf would reach the rows that do not): the epilogue adds
-//                   them to the rows that do
+//   warp 11         copies of V, and V behind its copy: places that hold no key become zero, and so do values that are not finite
+//                   where not every row sees the key (0 x inf would reach the rows that do not): the epilogue adds them to the
+//                   rows that do; the next segment's queries
 // The schedule's state is registers that a softmax thread, with a row of logits in its own, does not have: the others read the
 // segments from shared memory.
 // The schedule is that of fb_paged.cuh: equal parts of all key tiles per CTA, parts of an item joined by a second launch.
@@ -58,7 +58,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem), sQ = sbase, sK = sbase + Cfg::OFF_K, sV = sbase + Cfg::OFF_V, bar0 = sbase + Cfg::OFF_BAR;
   // (two slots: one per stream, stage, or buffer of queries)
-  const uint32_t q_ready = bar0, q_free = bar0 + 16, o_free = bar0 + 32, s_full = bar0 + 40, p_ready = bar0 + 56, pv_done = bar0 + 72,
+  const uint32_t q_ready = bar0, q_free = bar0 + 16, o_free = bar0 + 32, s_full = bar0 + 40, p_ready = bar0 + 56, pv_done = bar0 + 320,
                  k_full = bar0 + 88, k_free = bar0 + 104, v_full = bar0 + 120, v_free = bar0 + 136, s_read = bar0 + 152, v_ok = bar0 + 168,
                  seg_full = bar0 + 184;  // eight
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 248);
@@ -83,6 +83,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         mbar_init(s_full + 8 * i, 1);
         mbar_init(p_ready + 8 * i, 4);
         mbar_init(pv_done + 8 * i, 1);
+        mbar_init(pv_done + 16 + 8 * i, 1);
         mbar_init(s_read + 8 * i, 4);
         mbar_init(k_full + 8 * i, 1);
         mbar_init(k_free + 8 * i, 1);
@@ -110,7 +111,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  // Segment n, once it is known; false if there is none.
+  // Product number c of stream x: two barriers in turn, so that a wait cannot take the product before it for its own.
+  auto pv_bar = [&](int x, int c) { return pv_done + 16 * x + 8 * (c & 1); };
+  // Segment n, once it is known; none if there is none.
   auto segment = [&](int n) -> const volatile TileSeg* {
     const volatile TileSeg* sg = s_seg + (n & 7);
     return mbar_wait(seg_full + 8 * (n & 7), (n >> 3) & 1, abort_flag) && sg->n_kv > 0 ? sg : nullptr;
@@ -119,7 +122,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (warp >= 8) {
     setmaxnreg_dec<88>();
     if (warp == 8) {
-      // ------------------------------------------------------------------ schedule, TMA producer
+      // ------------------------------------------------------------------ schedule, copies of K
       const int rows = min(p.page_size, 128), pieces = 128 / rows;  // copies of a tile
       auto wait_all = [&](uint32_t bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)); };  // (the warp leaves together)
       auto publish = [&](const Segment& sg, bool there, int n) {
@@ -181,14 +184,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               for (int c = 0; c < NB; ++c)
                 tma_load_4d(sK + st * Cfg::Q_BYTES + c * 128 * 128 + lane * rows * 128, &tmK, k_full + 8 * st, c * 64, place, seg.hg, page);
             }
-            if (t >= ST && !wait_all(v_free + 8 * st, (t / ST - 1) & 1)) return;
-            if (lane == 0) mbar_expect_tx(v_full + 8 * st, Cfg::Q_BYTES);
-            __syncwarp();
-            if (lane < pieces) {
-#pragma unroll
-              for (int c = 0; c < NB; ++c)
-                tma_load_4d(sV + st * Cfg::Q_BYTES + c * 128 * 128 + lane * rows * 128, &tmV, v_full + 8 * st, c * 64, place, seg.hg, page);
-            }
           }
         }
       };
@@ -234,7 +229,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
             for (int s = 0; s < 8; ++s)
               umma_ts(tmem + Cfg::T_O, tmem + Cfg::T_P + 64 * x + s * 8, desc_at(dV, st * Cfg::Q_BYTES + mnmajor_step<TD>(s)), idO, (j > 0 || s > 0) ? 1u : 0u);
-            umma_commit(pv_done + 8 * x);
+            umma_commit(pv_bar(x, c));
             umma_commit(v_free + 8 * st);
           }
         }
@@ -265,14 +260,36 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const volatile TileSeg* sg = segment(n);
         return __all_sync(0xffffffffu, sg != nullptr) ? sg : nullptr;
       };
+      // V of tile number t (of the CTA), the j-th of a segment
+      const int rows = min(p.page_size, 128), pieces = 128 / rows;
+      auto load_v = [&](const volatile TileSeg* sg, int j, int t) {
+        const int st = t % ST, key = (sg->t1 - 1 - j) * 128 + lane * rows;
+        int page = (int)p.num_pages, place = 0;  // behind the cache: the copy fills in zeros
+        if (lane < pieces && key < sg->keys) {
+          const int col = a.page_div.quot32(key), pg = p.block_table[(int64_t)min(sg->b, p.B - 1) * p.table_stride + col];
+          if (pg >= 0 && pg < p.num_pages) {
+            page = pg;
+            place = key - col * p.page_size;
+          }
+        }
+        if (t >= ST && !__all_sync(0xffffffffu, mbar_wait(v_free + 8 * st, (t / ST - 1) & 1, abort_flag))) return;
+        if (lane == 0) mbar_expect_tx(v_full + 8 * st, Cfg::Q_BYTES);
+        __syncwarp();
+        if (lane < pieces) {
+#pragma unroll
+          for (int c = 0; c < NB; ++c)
+            tma_load_4d(sV + st * Cfg::Q_BYTES + c * 128 * 128 + lane * rows * 128, &tmV, v_full + 8 * st, c * 64, place, sg->hg, page);
+        }
+      };
       int t = 0, n = 0;
       const volatile TileSeg *sg = segment_warp(0), *nx = nullptr;
+      if (sg) load_v(sg, 0, 0);
       for (int r0 = 0; sg && r0 < 128; r0 += STEP) load_q(sg, 0, r0);
       if (sg) q_landed(0);
       for (; sg; sg = nx, ++n) {
         const int n_kv = sg->n_kv, t1 = sg->t1, len = sg->len, keys = sg->keys;
-        nx = nullptr;
-        int qrow = 128 + STEP;  // the next segment's queries: a step behind every tile, then the wait for them
+        nx = segment_warp(n + 1);  // (known before the first copy of this one)
+        int qrow = nx ? 0 : 128 + STEP;  // its queries: a step behind every tile, then the wait for them
         auto next_q = [&] {
           if (qrow < 128) load_q(nx, n + 1, qrow);
           else if (qrow < 128 + STEP) q_landed(n + 1);
@@ -280,6 +297,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         };
         for (int j = 0; j < n_kv; ++j, ++t) {
           const int st = t % ST, k0 = (t1 - 1 - j) * 128;
+          if (j + 1 < n_kv) load_v(sg, j + 1, t + 1);
+          else if (nx) load_v(nx, 0, t + 1);
           mbar_wait(v_full + 8 * st, (t / ST) & 1, abort_flag);
           const int r0 = max(len - k0, 0), live = keys - k0;  // first row that not all see; rows that hold keys
           if (r0 < 128) {
@@ -308,7 +327,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(v_ok + 8 * st);
-          if (j == 0 && (nx = segment_warp(n + 1))) qrow = 0;  // (known before the first copy of this one)
           next_q();
         }
         while (qrow < 128 + STEP) next_q();
@@ -345,7 +363,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const int hd = sg->hg * a.G + (tk >= 0 ? gr - tk * a.G : 0);
       float m_used = -INFINITY, l = 0.f;  // reference maximum (log2 units: logit * log2 e); row sum of this stream's tiles, relative to it
       const int c0 = c, co0 = co;
-      const float slope2 = SLOPES && tk >= 0 ? p.slopes[hd] * kLog2eP : 0.f;
+      // the bias in units of q.k, so that a logit costs one product more: s + slope_r (pos - k0), times sl2, plus abase
+      const float slope2 = SLOPES && tk >= 0 ? p.slopes[hd] * kLog2eP : 0.f, slope_r = slope2 / sl2;
       const int my_pos = SLOPES && tk >= 0 ? (p.positions ? p.positions[gn] : len + tk) : 0;
       for (int j = x; j < n_kv; j += 2, ++c) {
         const int k0 = (t1 - 1 - j) * 128;
@@ -371,7 +390,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               const bool own = k0 + 128 > len;  // (a tile of cached keys has no table of positions)
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                s[ch][i] = __float_as_uint(fmaf(slope2, (float)((own ? pos[ch * 32 + i] : j0 + i) - my_pos), __uint_as_float(s[ch][i]) * sl2));
+                s[ch][i] = __float_as_uint(fmaf(slope_r, (float)((own ? pos[ch * 32 + i] : j0 + i) - k0), __uint_as_float(s[ch][i])));
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -385,7 +404,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           for (int i = 0; i < 32; i += 2) {
             float v0 = __uint_as_float(s[ch][i]), v1 = __uint_as_float(s[ch][i + 1]);
             if (SLOPES) {
-              f2_unpack(f2_fma(f2(v0, v1), sl2p, f2(fmaf((float)(ch * 32 + i), slope2, abase), fmaf((float)(ch * 32 + i + 1), slope2, abase))), v0, v1);
+              v0 = fmaf((float)(ch * 32 + i), slope_r, v0);
+              v1 = fmaf((float)(ch * 32 + i + 1), slope_r, v1);
               s[ch][i] = __float_as_uint(v0);
               s[ch][i + 1] = __float_as_uint(v1);
             }
@@ -406,8 +426,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         tc_fence_before_sync();
         mbar_arrive_warp(s_read + 8 * x);  // the tensor core may start on the stream's next tile
         complete(3);
-        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        if (!SLOPES) mx *= sl2;  // sl2 > 0
+        const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sl2, abase);  // sl2 > 0
         // ---- the reference maximum, from tile to tile: it moves only when the maximum has grown by more than 2^8 (exact: the row
         // sums carry the same reference)
         const float m_last = m_used;
@@ -416,11 +435,10 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           m_used = __uint_as_float(ld_shared_flag(m_other));
           const float m_new = fmaxf(m_used, mx);
           if (__any_sync(0xffffffffu, m_new - m_used > 8.f)) {  // (from -inf: the difference is +inf, or NaN where both are)
-            // O is stable behind the product of tile j - 1.  The wait tests a parity, so the other stream's product before it, tile
-            // j - 3, must be known to have completed: tile j's logits are here, K(j) was loaded behind V(j - 1), and V(j - 1), in a
-            // ring of two, where V(j - 3) had been, behind that product.
-            static_assert(ST == 2, "a deeper ring does not order the products of tiles j - 3 and j");
-            mbar_wait(pv_done + 8 * (x ^ 1), (co0 + ((j - 1) >> 1)) & 1, abort_flag);
+            // O is stable behind the product of tile j - 1, which is the other stream's.  (The one two before it on that barrier,
+            // tile j - 5, has completed: the other stream has waited for it ahead of its P of tile j - 3.)
+            const int cp = co0 + ((j - 1) >> 1);
+            mbar_wait(pv_bar(x ^ 1, cp), (cp >> 1) & 1, abort_flag);
             tc_fence_after_sync();
             const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
             m_used = m_new;
@@ -442,12 +460,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           st_shared_f32(m_own, m_used);
           asm volatile("bar.arrive %0, 256;" ::"r"(2 + x) : "memory");
         }
-        if (c > 0) mbar_wait(pv_done + 8 * x, (c - 1) & 1, abort_flag);  // P has been read
+        if (c > 0) mbar_wait(pv_bar(x, c - 1), ((c - 1) >> 1) & 1, abort_flag);  // P has been read
         // ---- p = exp2(logit2 - m), row sum, P -> tensor memory (the A operand of O += P.V), rounded to the 16 bits of V
         const float msub = m_used == -INFINITY ? 0.f : m_used;
         l *= fast_exp2(m_last - msub);  // (0 at the stream's first tile, where l is 0)
         uint64_t l2a = f2(0.f, 0.f), l2b = f2(0.f, 0.f);
-        const uint64_t nm = f2(-msub, -msub);
+        const uint64_t nm = f2(abase - msub, abase - msub);
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
           uint32_t pw[16];  // 32 keys = 16 packed words
@@ -455,7 +473,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           for (int i = 0; i < 32; i += 2) {
             const uint64_t v = f2(__uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1]));
             float a0, a1;
-            f2_unpack(!SLOPES ? f2_fma(v, sl2p, nm) : f2_add(v, nm), a0, a1);
+            f2_unpack(f2_fma(v, sl2p, nm), a0, a1);
             const float p0 = fast_exp2(a0), p1 = fast_exp2(a1);
             if (i & 2) l2b = f2_add(l2b, f2(p0, p1)); else l2a = f2_add(l2a, f2(p0, p1));
             pw[i / 2] = Pack2<T>::pack(p0, p1);
@@ -478,7 +496,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       c = c0 + ((n_kv + 1 - x) >> 1);
       co = co0 + ((n_kv + x) >> 1);
       const int xl = (n_kv - 1) & 1;  // stream of the last tile
-      if (xl == x) mbar_wait(pv_done + 8 * x, (c - 1) & 1, abort_flag);
+      if (xl == x) mbar_wait(pv_bar(x, c - 1), ((c - 1) >> 1) & 1, abort_flag);
       float2* ml = reinterpret_cast<float2*>(smem + Cfg::OFF_ML) + (n & 1) * 256;
       ml[x * 128 + row] = make_float2(m_used, l);
       asm volatile("bar.sync 1, 256;" ::: "memory");  // both warpgroups
