@@ -27,8 +27,11 @@ constexpr int kTileThreads = 384;
 
 template <int TD>
 struct TileCfg {
-  static constexpr int Q_BYTES = tile_bytes(TD), ST = 2;
-  static constexpr int OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + ST * Q_BYTES, OFF_BAR = OFF_V + ST * Q_BYTES, OFF_SEG = OFF_BAR + 512,
+  static constexpr int Q_BYTES = tile_bytes(TD);
+  // Stages of K and V.  A copy from HBM takes about as long as two tiles' work, and V's stage is held until its product is done:
+  // with two the products wait for V (2200 clk a tile).
+  static constexpr int KST = TD == 128 ? 2 : 3, VST = TD == 128 ? 3 : 4;
+  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + KST * Q_BYTES, OFF_BAR = OFF_V + VST * Q_BYTES, OFF_SEG = OFF_BAR + 512,
                        OFF_ML = OFF_SEG + 8 * 64, OFF_M = OFF_ML + 2 * 2 * 128 * 8, OFF_POS = OFF_M + 2 * 128 * 4, SMEM = OFF_POS + 8 * 128 * 4 + 1024;
   static constexpr int T_S = 0, T_P = 256, T_O = 384;  // stream x: S + 128 x, P + 64 x
 };
@@ -52,23 +55,23 @@ template <typename T, int TD, bool SLOPES>
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedArgs a) {
   using Cfg = TileCfg<TD>;
-  constexpr int ST = Cfg::ST, NB = TD / 64, CH = TD / 8;
+  constexpr int KST = Cfg::KST, VST = Cfg::VST, NB = TD / 64, CH = TD / 8;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem), sQ = sbase, sK = sbase + Cfg::OFF_K, sV = sbase + Cfg::OFF_V, bar0 = sbase + Cfg::OFF_BAR;
-  // (two slots: one per stream, stage, or buffer of queries)
-  const uint32_t q_ready = bar0, q_free = bar0 + 16, o_free = bar0 + 32, s_full = bar0 + 40, p_ready = bar0 + 56, pv_done = bar0 + 320,
-                 k_full = bar0 + 88, k_free = bar0 + 104, v_full = bar0 + 120, v_free = bar0 + 136, s_read = bar0 + 152, v_ok = bar0 + 168,
-                 seg_full = bar0 + 184;  // eight
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 248);
-  const uint32_t abort_flag = bar0 + 252;
+  // one slot per stream, stage (up to four), product in turn and stream, segment (eight)
+  const uint32_t q_ready = bar0, q_free = bar0 + 8, o_free = bar0 + 16, s_full = bar0 + 24, p_ready = bar0 + 40, s_read = bar0 + 56,
+                 k_full = bar0 + 72, k_free = bar0 + 104, v_full = bar0 + 136, v_free = bar0 + 168, v_ok = bar0 + 320, pv_done = bar0 + 352,
+                 seg_full = bar0 + 384;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 200);
+  const uint32_t abort_flag = bar0 + 204;
   // per tile, eight deep (the producer is four tiles ahead of a softmax at most): which of the tile's pages exist, and the
-  // positions of its keys where they are not their places
-  volatile uint32_t* s_pages = reinterpret_cast<volatile uint32_t*>(smem + Cfg::OFF_BAR + 256);
-  int* s_pos = reinterpret_cast<int*>(smem + Cfg::OFF_POS);
+  // positions of its keys behind its first place, where they are not their places
+  volatile uint32_t* s_pages = reinterpret_cast<volatile uint32_t*>(smem + Cfg::OFF_BAR + 208);
+  float* s_pos = reinterpret_cast<float*>(smem + Cfg::OFF_POS);
   // per segment, eight deep: its number + 1 if it has values that were taken out; the segment
-  volatile int* s_taken = reinterpret_cast<volatile int*>(smem + Cfg::OFF_BAR + 288);
+  volatile int* s_taken = reinterpret_cast<volatile int*>(smem + Cfg::OFF_BAR + 240);
   volatile TileSeg* s_seg = reinterpret_cast<volatile TileSeg*>(smem + Cfg::OFF_SEG);
 
   const fb_paged_params& p = a.p;
@@ -76,20 +79,21 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (warp == 8) {
     if (lane == 0) {
       st_shared_flag(abort_flag, 0u);
-      mbar_init(o_free, 8);
+      mbar_init(q_ready, 1);
+      mbar_init(q_free, 1);
+      mbar_init(o_free, 8);  // every softmax warp has read the accumulator of the segment
       for (int i = 0; i < 2; ++i) {
-        mbar_init(q_ready + 8 * i, 1);
-        mbar_init(q_free + 8 * i, 1);
         mbar_init(s_full + 8 * i, 1);
-        mbar_init(p_ready + 8 * i, 4);
-        mbar_init(pv_done + 8 * i, 1);
-        mbar_init(pv_done + 16 + 8 * i, 1);
-        mbar_init(s_read + 8 * i, 4);
+        mbar_init(p_ready + 8 * i, 4);  // the stream's warps
+        mbar_init(s_read + 8 * i, 4);   // the logits of the tile are in registers
+      }
+      for (int i = 0; i < 4; ++i) {
         mbar_init(k_full + 8 * i, 1);
         mbar_init(k_free + 8 * i, 1);
         mbar_init(v_full + 8 * i, 1);
         mbar_init(v_free + 8 * i, 1);
         mbar_init(v_ok + 8 * i, 1);
+        mbar_init(pv_done + 8 * i, 1);
       }
       for (int i = 0; i < 8; ++i) {
         mbar_init(seg_full + 8 * i, 1);
@@ -143,6 +147,22 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           mbar_arrive(seg_full + 8 * (n & 7));
         }
       };
+      auto load_q = [&](const Segment& sg, int n) {
+        if (n > 0 && !wait_all(q_free, (n - 1) & 1)) return false;
+        const int live_rows = min(sg.r.tokens * a.G - sg.rt * 128, 128), col = (lane % CH) * 8;
+#pragma unroll 4
+        for (int r = lane / CH; r < 128; r += 32 / CH) {
+          const bool live = r < live_rows && col < p.D;
+          const int gr = sg.rt * 128 + r, tok = live ? a.group_div.quot32(gr) : 0, head = sg.hg * a.G + (live ? gr - tok * a.G : 0);
+          const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(sg.r.first + tok) * p.q_stride[0] + head * p.q_stride[1] + col;
+          cp_async16_zfill(sQ + tile_chunk_offset<TD>(r, col), live ? src : reinterpret_cast<const T*>(p.q), live);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_ready);
+        return true;
+      };
       auto produce = [&] {
         Segment seg, nxt = {};
         bool more = walk.next(a, nxt);
@@ -153,7 +173,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           publish(nxt, more, n + 1);
           const int32_t* table = p.block_table + (int64_t)min(seg.b, p.B - 1) * p.table_stride;
           for (int j = 0; j < seg.t1 - seg.t0; ++j, ++t) {
-            const int st = t % ST, k0 = (seg.t1 - 1 - j) * 128, key = k0 + lane * rows;
+            const int st = t % KST, k0 = (seg.t1 - 1 - j) * 128, key = k0 + lane * rows;
             int page = (int)p.num_pages, place = 0;  // behind the cache: the copy fills in zeros
             bool bad = false;
             if (lane < pieces && key < seg.r.keys) {
@@ -167,12 +187,13 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               }
             }
             const uint32_t there = ~__ballot_sync(0xffffffffu, bad);
-            if (t >= ST && !wait_all(k_free + 8 * st, (t / ST - 1) & 1)) return;
+            if (t >= KST && !wait_all(k_free + 8 * st, (t / KST - 1) & 1)) return;
             if (SLOPES && k0 + 128 > seg.r.len) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int k = k0 + e * 32 + lane;
-                s_pos[(t & 7) * 128 + e * 32 + lane] = p.positions && k >= seg.r.len && k < seg.r.keys ? p.positions[seg.r.first + k - seg.r.len] : k;
+                s_pos[(t & 7) * 128 + e * 32 + lane] =
+                    (float)((p.positions && k >= seg.r.len && k < seg.r.keys ? p.positions[seg.r.first + k - seg.r.len] : k) - k0);
               }
             }
             if (lane == 0) s_pages[t & 7] = there;
@@ -184,6 +205,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               for (int c = 0; c < NB; ++c)
                 tma_load_4d(sK + st * Cfg::Q_BYTES + c * 128 * 128 + lane * rows * 128, &tmK, k_full + 8 * st, c * 64, place, seg.hg, page);
             }
+            if (j == 0 && !load_q(seg, n)) return;  // (behind the first copy of K, which need not wait for the last segment's end)
           }
         }
       };
@@ -195,21 +217,21 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const DescBase dQ = kmajor_base<TD>(sQ), dK = kmajor_base<TD>(sK);
         int t = 0, n = 0, c0 = 0, c1 = 0;  // key tiles, segments; key tiles of either stream
         for (const volatile TileSeg* sg; (sg = segment(n)); ++n) {
-          const int n_kv = sg->n_kv, qo = (n & 1) * Cfg::Q_BYTES;
-          mbar_wait(q_ready + 8 * (n & 1), (n >> 1) & 1, abort_flag);
+          const int n_kv = sg->n_kv;
+          mbar_wait(q_ready, n & 1, abort_flag);
           tc_fence_after_sync();
           for (int j = 0; j < n_kv; ++j, ++t) {
-            const int x = j & 1, c = x ? c1++ : c0++, st = t % ST;
+            const int x = j & 1, c = x ? c1++ : c0++, st = t % KST;
             if (c > 0) mbar_wait(s_read + 8 * x, (c - 1) & 1, abort_flag);
-            mbar_wait(k_full + 8 * st, (t / ST) & 1, abort_flag);
+            mbar_wait(k_full + 8 * st, (t / KST) & 1, abort_flag);
             tc_fence_after_sync();
 #pragma unroll
             for (int s = 0; s < TD / 16; ++s)
-              umma_ss(tmem + Cfg::T_S + 128 * x, desc_at(dQ, qo + kmajor_step<TD>(s)), desc_at(dK, st * Cfg::Q_BYTES + kmajor_step<TD>(s)), idS, s > 0);
+              umma_ss(tmem + Cfg::T_S + 128 * x, desc_at(dQ, kmajor_step<TD>(s)), desc_at(dK, st * Cfg::Q_BYTES + kmajor_step<TD>(s)), idS, s > 0);
             umma_commit(s_full + 8 * x);
             umma_commit(k_free + 8 * st);
           }
-          umma_commit(q_free + 8 * (n & 1));  // the segment's queries are no longer read
+          umma_commit(q_free);  // the segment's queries are no longer read
         }
       }
     } else if (warp == 10) {
@@ -221,8 +243,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         for (const volatile TileSeg* sg; (sg = segment(n)); ++n) {
           const int n_kv = sg->n_kv;
           for (int j = 0; j < n_kv; ++j, ++t) {
-            const int x = j & 1, c = x ? c1++ : c0++, st = t % ST;
-            mbar_wait(v_ok + 8 * st, (t / ST) & 1, abort_flag);
+            const int x = j & 1, c = x ? c1++ : c0++, st = t % VST;
+            mbar_wait(v_ok + 8 * st, (t / VST) & 1, abort_flag);
             mbar_wait(p_ready + 8 * x, c & 1, abort_flag);
             if (j == 0 && n > 0) mbar_wait(o_free, (n - 1) & 1, abort_flag);  // the accumulator of the last segment has been read
             tc_fence_after_sync();
@@ -235,27 +257,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
       }
     } else {
-      // ------------------------------------------------------------------ queries; V behind its copy
-      constexpr int STEP = 8 * (32 / CH);  // rows of a step: eight copies of a lane
-      auto load_q = [&](const volatile TileSeg* sg, int n, int r0) {
-        if (r0 == 0 && n > 1) mbar_wait(q_free + 8 * (n & 1), (n / 2 - 1) & 1, abort_flag);
-        const int rt = sg->rt, hg = sg->hg, first = sg->first, rows = min(sg->tokens * a.G - rt * 128, 128);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int r = r0 + u * (32 / CH) + lane / CH, col = (lane % CH) * 8, gr = rt * 128 + r;
-          const bool live = r < rows && col < p.D;
-          const int tok = live ? a.group_div.quot32(gr) : 0, head = hg * a.G + (live ? gr - tok * a.G : 0);
-          const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(first + tok) * p.q_stride[0] + head * p.q_stride[1] + col;
-          cp_async16_zfill(sQ + (n & 1) * Cfg::Q_BYTES + tile_chunk_offset<TD>(r, col), live ? src : reinterpret_cast<const T*>(p.q), live);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
-      auto q_landed = [&](int n) {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_ready + 8 * (n & 1));
-      };
+      // ------------------------------------------------------------------ copies of V, and V behind them
       auto segment_warp = [&](int n) {  // (the warp leaves together)
         const volatile TileSeg* sg = segment(n);
         return __all_sync(0xffffffffu, sg != nullptr) ? sg : nullptr;
@@ -263,7 +265,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       // V of tile number t (of the CTA), the j-th of a segment
       const int rows = min(p.page_size, 128), pieces = 128 / rows;
       auto load_v = [&](const volatile TileSeg* sg, int j, int t) {
-        const int st = t % ST, key = (sg->t1 - 1 - j) * 128 + lane * rows;
+        const int st = t % VST, key = (sg->t1 - 1 - j) * 128 + lane * rows;
         int page = (int)p.num_pages, place = 0;  // behind the cache: the copy fills in zeros
         if (lane < pieces && key < sg->keys) {
           const int col = a.page_div.quot32(key), pg = p.block_table[(int64_t)min(sg->b, p.B - 1) * p.table_stride + col];
@@ -272,7 +274,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             place = key - col * p.page_size;
           }
         }
-        if (t >= ST && !__all_sync(0xffffffffu, mbar_wait(v_free + 8 * st, (t / ST - 1) & 1, abort_flag))) return;
+        if (t >= VST && !__all_sync(0xffffffffu, mbar_wait(v_free + 8 * st, (t / VST - 1) & 1, abort_flag))) return;
         if (lane == 0) mbar_expect_tx(v_full + 8 * st, Cfg::Q_BYTES);
         __syncwarp();
         if (lane < pieces) {
@@ -283,23 +285,24 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       };
       int t = 0, n = 0;
       const volatile TileSeg *sg = segment_warp(0), *nx = nullptr;
-      if (sg) load_v(sg, 0, 0);
-      for (int r0 = 0; sg && r0 < 128; r0 += STEP) load_q(sg, 0, r0);
-      if (sg) q_landed(0);
+      // The copies run VST - 1 tiles ahead, across segments: tile lj of segment ls is copied next.
+      const volatile TileSeg* ls = sg;
+      int lj = 0, lt = 0, ln = 0;
+      auto load_next = [&] {
+        if (!ls) return;
+        load_v(ls, lj, lt++);
+        if (++lj == ls->n_kv) {
+          ls = segment_warp(++ln);  // (known before the first copy of K of the one before)
+          lj = 0;
+        }
+      };
+      for (int i = 0; i < VST - 1; ++i) load_next();
       for (; sg; sg = nx, ++n) {
         const int n_kv = sg->n_kv, t1 = sg->t1, len = sg->len, keys = sg->keys;
-        nx = segment_warp(n + 1);  // (known before the first copy of this one)
-        int qrow = nx ? 0 : 128 + STEP;  // its queries: a step behind every tile, then the wait for them
-        auto next_q = [&] {
-          if (qrow < 128) load_q(nx, n + 1, qrow);
-          else if (qrow < 128 + STEP) q_landed(n + 1);
-          qrow += STEP;
-        };
         for (int j = 0; j < n_kv; ++j, ++t) {
-          const int st = t % ST, k0 = (t1 - 1 - j) * 128;
-          if (j + 1 < n_kv) load_v(sg, j + 1, t + 1);
-          else if (nx) load_v(nx, 0, t + 1);
-          mbar_wait(v_full + 8 * st, (t / ST) & 1, abort_flag);
+          const int st = t % VST, k0 = (t1 - 1 - j) * 128;
+          load_next();
+          mbar_wait(v_full + 8 * st, (t / VST) & 1, abort_flag);
           const int r0 = max(len - k0, 0), live = keys - k0;  // first row that not all see; rows that hold keys
           if (r0 < 128) {
             bool taken = false;
@@ -327,9 +330,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(v_ok + 8 * st);
-          next_q();
         }
-        while (qrow < 128 + STEP) next_q();
+        nx = segment_warp(n + 1);
       }
     }
   } else {
@@ -368,33 +370,49 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const int my_pos = SLOPES && tk >= 0 ? (p.positions ? p.positions[gn] : len + tk) : 0;
       for (int j = x; j < n_kv; j += 2, ++c) {
         const int k0 = (t1 - 1 - j) * 128;
+        const bool own = k0 + 128 > len;  // the tile holds new tokens' keys, or places behind them
+        uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (own) {  // the row's view of them, ahead of the wait
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) {
+            const int j0 = k0 + ch * 32, left = keys - j0;
+            bits[ch] = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
+            if (tk >= 0 && j0 + 32 > len) bits[ch] &= seen_bits(p, gn, tk, j0 - len);
+          }
+        }
         mbar_wait(s_full + 8 * x, c & 1, abort_flag);
         tc_fence_after_sync();
         const uint32_t there = s_pages[(t0 + j) & 7];
-        const bool dead = there != 0xffffffffu || k0 + 128 > len;
-        const int* pos = s_pos + ((t0 + j) & 7) * 128;
+        const bool dead = there != 0xffffffffu || own;
+        const float* pos = s_pos + ((t0 + j) & 7) * 128;
+        if (there != 0xffffffffu) {  // (rare) pages that do not exist
+          const int rows = min(p.page_size, 128);
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+#pragma unroll 1
+            for (int i = 0; i < 32; ++i)
+              if (!(there >> ((ch * 32 + i) / rows) & 1)) bits[ch] &= ~(1u << i);
+        }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         const float abase = SLOPES ? slope2 * (float)(k0 - my_pos) : 0.f;
         auto complete = [&](int ch) {
           if (dead) {
-            const int j0 = k0 + ch * 32, left = keys - j0;
-            uint32_t bits = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
-            if (tk >= 0 && bits && j0 + 32 > len) bits &= seen_bits(p, gn, tk, j0 - len);
-            if (there != 0xffffffffu) {  // (rare)
-              const int rows = min(p.page_size, 128);
-#pragma unroll 1
-              for (int i = 0; i < 32; ++i)
-                if (!(there >> ((ch * 32 + i) / rows) & 1)) bits &= ~(1u << i);
-            }
             if (SLOPES) {
-              const bool own = k0 + 128 > len;  // (a tile of cached keys has no table of positions)
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 f = own ? *reinterpret_cast<const float4*>(pos + ch * 32 + i)
+                                     : make_float4((float)(ch * 32 + i), (float)(ch * 32 + i + 1), (float)(ch * 32 + i + 2), (float)(ch * 32 + i + 3));
+                s[ch][i] = __float_as_uint(fmaf(slope_r, f.x, __uint_as_float(s[ch][i])));
+                s[ch][i + 1] = __float_as_uint(fmaf(slope_r, f.y, __uint_as_float(s[ch][i + 1])));
+                s[ch][i + 2] = __float_as_uint(fmaf(slope_r, f.z, __uint_as_float(s[ch][i + 2])));
+                s[ch][i + 3] = __float_as_uint(fmaf(slope_r, f.w, __uint_as_float(s[ch][i + 3])));
+              }
+            }
+            if (__any_sync(0xffffffffu, bits[ch] != 0xffffffffu)) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                s[ch][i] = __float_as_uint(fmaf(slope_r, (float)((own ? pos[ch * 32 + i] : j0 + i) - k0), __uint_as_float(s[ch][i])));
+                if (!(bits[ch] >> i & 1)) s[ch][i] = __float_as_uint(-INFINITY);
             }
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(bits >> i & 1)) s[ch][i] = __float_as_uint(-INFINITY);
 #pragma unroll
             for (int i = 0; i < 32; i += 2) mx4[(i >> 1) & 3] = fmax3(mx4[(i >> 1) & 3], __uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1]));
             __syncwarp();  // (the loads from tensor memory want the warp together)
