@@ -196,59 +196,58 @@ int launch_paged_split_d128(const PagedArgs& a, const PagedPlan& plan, cudaStrea
 int launch_paged_tile_d64(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
 int launch_paged_tile_d128(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
 
-// Joins the parts of the item that begins in CTA blockIdx.x; a warp per row, the parts in the order of the CTAs.  Latency is
-// all there is to it: what the rows need stands in the descriptor, and the first parts are on their way before the maximum is
-// known.
+// Joins the parts of the item that begins in CTA blockIdx.x; TD / 4 lanes per row, the parts in the order of the CTAs.  Latency
+// is all there is to it: what the rows need stands in the descriptor, and the first parts are on their way before the maximum
+// is known.
 constexpr int kJoinThreads = 128;  // (of 512 an SM holds one, and most have nothing to join)
 template <typename T, int TD>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, const int WH, const int MT) {
-  constexpr int C = TD / 32, U = 8;  // columns of a lane, parts in flight
+  constexpr int LANES = TD / 4, U = 8;  // lanes of a row, parts in flight
   grid_dep_wait();
   const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
   if (d.x < 0) return;
   const fb_paged_params& p = a.p;
-  const int lane = threadIdx.x & 31, idx = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x % LANES, idx = blockIdx.y * (kJoinThreads / LANES) + threadIdx.x / LANES;
   const int wh = idx / MT, r = idx - wh * MT, gr = d.x * MT + r, parts = d.z - (int)blockIdx.x + 1;
   if (gr >= e.y) return;
   const int64_t step = (int64_t)2 * WH * MT;  // rows of a CTA
   const int64_t row0 = blockIdx.x * step + (int64_t)(WH + wh) * MT + r, row1 = (int64_t)(blockIdx.x + 1) * step + (int64_t)wh * MT + r;
   auto row_of = [&](int i) { return i == 0 ? row0 : row1 + (i - 1) * step; };
-  float v[U][C];
+  float4 v[U];
   float2 s[U];
   auto load = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = row_of(min(i0 + u, parts - 1));
       s[u] = a.ml[row];
-#pragma unroll
-      for (int c = 0; c < C; ++c) v[u][c] = a.part[row * TD + c * 32 + lane];
+      v[u] = reinterpret_cast<const float4*>(a.part + row * TD)[lane];
     }
   };
   load(0);
   float m = -INFINITY;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, a.ml[row_of(i)].x);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int u = 0; u < U; ++u) m = fmaxf(m, s[u].x);
+#pragma unroll 4
+  for (int i = U; i < parts; ++i) m = fmaxf(m, a.ml[row_of(i)].x);
   const float ms = fmaxf(m, -FLT_MAX);
-  float l = 0.f, acc[C] = {};
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i0 + u >= parts) break;
       const float f = fast_exp2(s[u].x - ms);
       l = fmaf(s[u].y, f, l);
-#pragma unroll
-      for (int c = 0; c < C; ++c) acc[c] = fmaf(v[u][c], f, acc[c]);
+      acc = make_float4(fmaf(v[u].x, f, acc.x), fmaf(v[u].y, f, acc.y), fmaf(v[u].z, f, acc.z), fmaf(v[u].w, f, acc.w));
     }
     if ((i0 += U) >= parts) break;
     load(i0);
   }
   const int t = a.group_div.quot32(gr), h = (d.y * WH + wh) * a.G + gr - t * a.G, n = e.x + t;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-  T* dst = reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1];
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-    if (c * 32 + lane < p.D) dst[c * 32 + lane] = from_f32<T>(l == 0.f ? 0.f : acc[c] * inv);
+  if (lane * 4 < p.D)  // D is a multiple of 8
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1] + lane * 4) =
+        l == 0.f ? make_uint2(0u, 0u) : make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
   if (p.lse && lane == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
 }
 
@@ -272,7 +271,7 @@ int launch_pdl_2d(void (*kern)(P...), dim3 grid, unsigned block, cudaStream_t st
 // (an item may begin in any CTA and end in a later one)
 template <int TD>
 int launch_paged_join(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
-  const dim3 grid(plan.ctas, plan.WH * plan.MT / (kJoinThreads / 32));
+  const dim3 grid(plan.ctas, plan.WH * plan.MT / (kJoinThreads / (TD / 4)));
   return a.p.dtype == FB_DTYPE_F16 ? launch_pdl_2d(paged_join_kernel<__half, TD>, grid, kJoinThreads, st, a, plan.WH, plan.MT)
                                    : launch_pdl_2d(paged_join_kernel<__nv_bfloat16, TD>, grid, kJoinThreads, st, a, plan.WH, plan.MT);
 }

@@ -301,7 +301,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const int n_kv = sg->n_kv, t1 = sg->t1, len = sg->len, keys = sg->keys;
         for (int j = 0; j < n_kv; ++j, ++t) {
           const int st = t % VST, k0 = (t1 - 1 - j) * 128;
-          load_next();
           mbar_wait(v_full + 8 * st, (t / VST) & 1, abort_flag);
           const int r0 = max(len - k0, 0), live = keys - k0;  // first row that not all see; rows that hold keys
           if (r0 < 128) {
@@ -330,6 +329,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(v_ok + 8 * st);
+          load_next();  // (behind the product of tile t - 1; ahead of the arrival it would hold up the next product)
         }
         nx = segment_warp(n + 1);
       }
