@@ -19,6 +19,8 @@ FB_FLAG_BWD_QUERY_MAJOR = 2
 FB_FLAG_BWD_ONE_ITEM = 4
 FB_FLAG_BWD_PERSISTENT = 8
 FB_FLAG_BWD_FUSED_DELTA = 16
+FB_FLAG_PAGED_SPLIT = 32
+PAGED_KERNELS = ("general", "split", "tile")  # FB_PAGED_*
 KERNELS = ("general", "fwd_tiled", "fwd_one_query", "bwd_query_major", "bwd_persistent", "bwd_key_major", "bwd_two_stream",
            "fwd_two_stream")  # FB_KERNEL_*
 
@@ -125,6 +127,7 @@ EXPORTS = {
     "fb_paged_append": (C.c_int, [C.POINTER(FbRopeParams), C.c_void_p]),
     "fb_plan_params_size": (C.c_size_t, []),
     "fb_paged_plan": (C.c_int, [C.POINTER(FbPlanParams), C.c_void_p]),
+    "fb_paged_kernel": (C.c_int, [C.POINTER(FbPagedParams)]),
     "fb_paged_params_size": (C.c_size_t, []),
     "fb_paged_workspace_bytes": (C.c_size_t, [C.POINTER(FbPagedParams)]),
     "fb_paged_fwd": (C.c_int, [C.POINTER(FbPagedParams), C.c_void_p]),

@@ -152,15 +152,15 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
   // pages (or a page of whole tiles) that TMA can address, and the scale may be taken out of a maximum.
   const bool tma = tma_compatible(p->key_cache, p->key_cache_stride[1], p->key_cache_stride[2], p->key_cache_stride[0], p->Hk, p->num_pages) &&
                    tma_compatible(p->value_cache, p->value_cache_stride[1], p->value_cache_stride[2], p->value_cache_stride[0], p->Hk, p->num_pages);
-  if (rows > 32 && tma && p->R == 0 && p->softmax_scale > 1e-20f && p->page_size % 8 == 0 && (128 % p->page_size == 0 || p->page_size % 128 == 0) &&
+  if (rows > 32 && !(p->flags & FB_FLAG_PAGED_SPLIT) && tma && p->R == 0 && p->softmax_scale > 1e-20f && p->page_size % 8 == 0 && (128 % p->page_size == 0 || p->page_size % 128 == 0) &&
       p->num_pages < 0x7fffffffLL) {
-    plan.kernel = PAGED_TILE;
+    plan.kernel = FB_PAGED_TILE;
     plan.TD = p->D <= 64 ? 64 : 128;
     plan.MT = 128;
     plan.WH = 1;
     plan.ctas = sms;
   } else {
-    plan.kernel = PAGED_SPLIT;
+    plan.kernel = FB_PAGED_SPLIT;
     plan.TD = p->D <= 32 ? 32 : p->D <= 64 ? 64 : 128;
     plan.MT = rows <= 16 ? 16 : 32;
     plan.ctas = split_ctas(plan.TD, plan.MT) * sms;
@@ -182,6 +182,11 @@ using namespace fb;
 
 extern "C" size_t fb_paged_params_size(void) { return sizeof(fb_paged_params); }
 
+extern "C" int fb_paged_kernel(const fb_paged_params* p) {
+  const int rc = validate_paged(p);
+  return rc ? rc : plan_paged(p).kernel;
+}
+
 extern "C" size_t fb_paged_workspace_bytes(const fb_paged_params* p) {
   if (validate_paged(p)) return 0;
   const PagedPlan plan = plan_paged(p);
@@ -192,7 +197,7 @@ extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
   if (const int rc = validate_paged(p)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   const PagedPlan plan = plan_paged(p);
-  if (plan.kernel != PAGED_GENERAL) {
+  if (plan.kernel != FB_PAGED_GENERAL) {
     const size_t need = plan.part_bytes + plan.ml_bytes + plan.desc_bytes;
     if (!p->workspace || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255)) return FB_EINVAL_WORKSPACE;
     PagedArgs a = {};
@@ -213,7 +218,7 @@ extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
     a.part = reinterpret_cast<float*>(ws);
     a.ml = reinterpret_cast<float2*>(ws + plan.part_bytes);
     a.desc = reinterpret_cast<int4*>(ws + plan.part_bytes + plan.ml_bytes);
-    if (plan.kernel == PAGED_TILE) return plan.TD == 64 ? launch_paged_tile_d64(a, plan, st) : launch_paged_tile_d128(a, plan, st);
+    if (plan.kernel == FB_PAGED_TILE) return plan.TD == 64 ? launch_paged_tile_d64(a, plan, st) : launch_paged_tile_d128(a, plan, st);
     return plan.TD == 32 ? launch_paged_split_d32(a, plan, st) : plan.TD == 64 ? launch_paged_split_d64(a, plan, st) : launch_paged_split_d128(a, plan, st);
   }
   const unsigned grid = (unsigned)(p->N * p->Hq);

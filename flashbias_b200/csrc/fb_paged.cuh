@@ -180,11 +180,10 @@ __device__ __forceinline__ bool tree_sees(const fb_paged_params& p, int n, int t
 }
 
 // ---- host side (fb_paged.cu, fb_paged_split_*.cu, fb_paged_tile_*.cu) ------------------------------------------------
-enum { PAGED_GENERAL, PAGED_SPLIT, PAGED_TILE };
 // CTAs of the split kernel that an SM holds: three while their warps' output rows leave the registers for it
 constexpr int split_ctas(int TD, int MT) { return TD < 128 && MT == 16 ? 3 : 2; }
 struct PagedPlan {
-  int kernel;  // PAGED_*
+  int kernel;  // FB_PAGED_*
   int TD, MT;  // columns and rows of a tile
   int WH;      // key heads of a group
   int ctas;

@@ -47,6 +47,7 @@ extern "C" {
                                      head)) per CTA, thread = query row, whatever the shape */
 #define FB_FLAG_BWD_PERSISTENT 8 /* ... one persistent CTA per SM walking the work items, whatever the shape (by
                                      default: chosen when a work item has few query tiles) */
+#define FB_FLAG_PAGED_SPLIT 32     /* fb_paged_fwd: the split kernel where the tile kernel would be taken (cross-checks) */
 #define FB_FLAG_BWD_FUSED_DELTA 16 /* fb_bwd takes delta itself, in the launch that prepares its operands: no
                                       fb_bwd_preprocess call is needed before it (p->delta is written either way) */
 
@@ -297,7 +298,7 @@ typedef struct fb_paged_params {
   int32_t N, B, Hq, Hk, D, R;
   int32_t dtype;
   int32_t page_size, table_width, mask_words, bias_heads; /* bias_heads: heads of bias_cache, 1 or Hk */
-  int32_t flags;                                          /* FB_FLAG_FORCE_GENERAL */
+  int32_t flags;                                          /* FB_FLAG_FORCE_GENERAL, FB_FLAG_PAGED_SPLIT */
   int64_t num_pages;
   float softmax_scale;
   const void *q, *q_bias, *key_cache, *value_cache, *bias_cache;
@@ -316,6 +317,13 @@ typedef struct fb_paged_params {
   size_t workspace_bytes;
   int32_t *status; /* optional, as in fb_params */
 } fb_paged_params;
+
+/* The kernel that fb_paged_fwd takes (FB_PAGED_*), or <0 on invalid arguments.  Fill in every pointer and stride of the call. */
+#define FB_PAGED_GENERAL 0 /* CUDA cores: head_dim not a multiple of 8, rows that are not whole aligned 16-byte chunks */
+#define FB_PAGED_SPLIT 1   /* mma.sync, up to 32 rows (tokens times heads per key head) of a request side by side */
+#define FB_PAGED_TILE 2    /* tcgen05 tiles of 128 rows: more than 32 rows per request on average, no factors, a positive scale,
+                              page_size a multiple of 8 that divides 128 or a multiple of 128 */
+int fb_paged_kernel(const fb_paged_params *p);
 
 size_t fb_paged_params_size(void);
 size_t fb_paged_workspace_bytes(const fb_paged_params *p);

@@ -279,3 +279,133 @@ def test_refusals(bad):
         flash_bias_paged_func(**dev({**args, **bad}))
     with pytest.raises(RuntimeError, match="together"):
         flash_bias_paged_func(**dev(args), q_bias=torch.zeros(2, 4, 2).half().cuda())
+
+
+def kernel_of(kw, flags=0):
+    """The kernel (flashbias_b200._lib.PAGED_KERNELS) of a call with contiguous tensors like these."""
+    import ctypes as C
+
+    from flashbias_b200 import _lib
+    p = _lib.FbPagedParams()
+    q, kc, bc = kw["q"], kw["key_cache"], kw.get("bias_cache")
+    p.N, p.Hq, p.D, p.B, p.Hk, p.page_size, p.num_pages = *q.shape, kw["lens"].numel(), kc.shape[2], kc.shape[1], kc.shape[0]
+    p.dtype, p.table_width, p.softmax_scale, p.flags = _lib.FB_DTYPE_BF16, kw["block_table"].shape[1], kw.get("softmax_scale", 1.0), flags
+    for n in ("q", "key_cache", "value_cache", "block_table", "lens", "cu_tokens", "o"):
+        setattr(p, n, 0x1000)
+    p.q_stride = p.o_stride = _lib.I64x2(q.shape[1] * q.shape[2], q.shape[2])
+    p.key_cache_stride = p.value_cache_stride = _lib.I64x3(kc.stride(0), kc.stride(1), kc.stride(2))
+    if bc is not None:
+        p.R, p.bias_heads, p.q_bias, p.bias_cache = bc.shape[3], bc.shape[2], 0x1000, 0x1000
+    return _lib.PAGED_KERNELS[_lib.load().fb_paged_kernel(C.byref(p))]
+
+
+@pytest.mark.parametrize("R,heads", [(1, 2), (2, 2), (4, 1), (5, 2), (6, 2), (7, 1), (10, 2), (12, 2), (16, 1), (17, 2), (20, 2), (40, 1)])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 16), (32, 8), (96, 7)])
+def test_ranks(R, heads, D, page):
+    """Every way of reading factors: copied in pieces of 4, 8 or 16 bytes, odd ranks, and ranks beyond one product."""
+    kw = paged_inputs([75, 0, 33], [1, 5, 3], 4, 2, D, page, torch.float16, R, R, heads)
+    assert kernel_of(kw) == "split"
+    check(kw)
+
+
+def test_factors_at_an_odd_offset():
+    kw = paged_inputs([75, 3], [1, 5], 4, 2, 64, 16, torch.float16, 1, 4)
+    want = check(kw)
+    d = dev(kw)
+    d["bias_cache"] = torch.cat([d["bias_cache"][..., :1], d["bias_cache"]], -1)[..., 1:]
+    assert torch.equal(flash_bias_paged_func(**d), want)
+
+
+@pytest.mark.parametrize("Hq,D,page", [(4, 128, 32), (8, 64, 16), (3, 96, 128), (2, 40, 8), (6, 128, 256)])
+@pytest.mark.parametrize("bias", ["none", "slopes"])
+def test_tile_and_split_kernels_agree(Hq, D, page, bias):
+    """The same call through both kernels: requests that end anywhere in a tile of 128 keys or rows, none cached, refused ones."""
+    from flashbias_b200 import _lib
+    from flashbias_b200.flash_bias import _op
+    lens, new = [127, 128, 129, 0, -1, 513, 1000], [60, 1, 130, 97, 20, 33, 64]
+    kw = paged_inputs(lens, new, Hq, 1 if Hq == 3 else 2, D, page, torch.bfloat16, D)
+    _, mask, depth = tree(new, 23, 3)
+    kw["tree_mask"] = mask
+    if bias == "slopes":
+        kw["slopes"] = torch.linspace(0.5, 0.02, Hq)
+        kw["positions"] = (torch.repeat_interleave(kw["lens"], torch.tensor(new)) + depth).int()
+    assert kernel_of(kw) == "tile" and kernel_of(kw, _lib.FB_FLAG_PAGED_SPLIT) == "split"
+    check(kw)
+    d = dev(kw)
+    args = [d["q"], d["key_cache"], d["value_cache"], d["block_table"], d["lens"], d["cu_tokens"], d["tree_mask"], d.get("positions"), d.get("slopes")]
+    got, lse = _op().paged_forward(*args, None, None, None, True, _lib.FB_FLAG_PAGED_SPLIT)
+    gen, gl = _op().paged_forward(*args, None, None, None, True, _lib.FB_FLAG_FORCE_GENERAL)
+    want, l64, weight, size = orc.paged_attention(kw["q"], kw["key_cache"], kw["value_cache"], kw["block_table"], kw["lens"], kw["cu_tokens"], mask,
+                                                  kw.get("positions"), kw.get("slopes"))
+    b = bounds(want, weight, size, D, torch.bfloat16)[0]
+    assert_within("split", got, want, b)
+    assert_within("general", gen, want, b)
+    live = l64 > -math.inf
+    assert (lse.cpu()[~live] == -math.inf).all() and (lse.cpu()[live] - l64[live]).abs().max() < 1e-3 and (gl.cpu()[live] - l64[live]).abs().max() < 1e-3
+
+
+@pytest.mark.parametrize("T,Hq", [(1, 2), (40, 2), (20, 6)])
+def test_many_requests(T, Hq):
+    """More requests than a block of the schedule has threads, most of them short, some empty."""
+    g = torch.Generator().manual_seed(T)
+    B = 900 if T == 1 else 450
+    lens, new = torch.randint(0, 40, (B,), generator=g).tolist(), torch.randint(0, T + 1, (B,), generator=g).tolist()
+    new[0] = T
+    kw = paged_inputs(lens, new, Hq, 2, 64, 16, torch.float16, 24)
+    assert kernel_of(kw) == ("tile" if T * Hq / 4 > 32 else "split")
+    check(kw)
+
+
+def test_long_request_among_short_ones():
+    """One request holds nearly all keys: its key tiles are spread over the GPU, and joined."""
+    for T, Hq in ((1, 8), (2, 4), (24, 8)):
+        kw = paged_inputs([20000, 1, 30, 0], [T, 1, T, T], Hq, 4, 64, 64, torch.bfloat16, 25)
+        check(kw, slopes=torch.full((Hq,), 0.003))
+
+
+def test_non_finite_values_in_a_tile_of_many_rows():
+    """As test_values_of_unseen_keys_do_not_count, at every kernel, with values in the cached part as well."""
+    from flashbias_b200 import _lib
+    from flashbias_b200.flash_bias import _op
+    new = [50, 40]
+    kw = paged_inputs([200, 3], new, 4, 2, 128, 16, torch.bfloat16, 26)
+    _, mask, _ = tree(new, 27)
+    d = dev(kw)
+    args = lambda d: [d["q"], d["key_cache"], d["value_cache"], d["block_table"], d["lens"], d["cu_tokens"], mask.cuda(), None, None, None, None, None, False]  # noqa: E731
+    flags = (0, _lib.FB_FLAG_PAGED_SPLIT, _lib.FB_FLAG_FORCE_GENERAL)
+    assert kernel_of(kw) == "tile"
+    clean = [_op().paged_forward(*args(d), f)[0].cpu() for f in flags]
+    for b, t, what in ((0, 4, float("nan")), (1, 20, -float("inf"))):
+        place = int(kw["lens"][b]) + t
+        kw["value_cache"][int(kw["block_table"][b, place // 16]), place % 16, :, 3:70] = what
+    d = dev(kw)
+    seen = torch.tensor([bool(mask[n, 0] >> (4 if n < 50 else 20) & 1) for n in range(90)])
+    for f, c in zip(flags, clean):
+        o = _op().paged_forward(*args(d), f)[0].cpu()
+        assert torch.equal(o[~seen], c[~seen])
+        assert not o[seen][:, :, 3:70].isfinite().any() and torch.equal(o[seen][:, :, :3], c[seen][:, :, :3])
+    d["value_cache"][int(kw["block_table"][1, 0]), 1, 0, 5] = float("inf")  # a cached key that all of request 1 see
+    for f in flags:
+        o = _op().paged_forward(*args(d), f)[0].cpu()
+        assert not o[50:, :2, 5].isfinite().any()
+
+
+def test_two_graphs_and_an_eager_call_do_not_share_their_scratch():
+    kw = [paged_inputs([3000, 70], [T, 1], 8, 2, 128, 16, torch.bfloat16, 28 + T) for T in (1, 30)]
+    ds = [dev(k) for k in kw]
+    want = [flash_bias_paged_func(**d) for d in ds]
+    graphs, outs = [], []
+    for d in ds:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(flash_bias_paged_func(**d))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in ds]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        eager = flash_bias_paged_func(**ds[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)) and torch.equal(eager, want[0])

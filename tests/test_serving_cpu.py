@@ -98,7 +98,8 @@ def test_paged_plan_refuses(change, code):
                                          (dict(table_width=1 << 30), -13), (dict(q=None), -1), (dict(cu_tokens=None), -1), (dict(o=None), -1),
                                          (dict(R=4), -7), (dict(q_bias=0x1000), -7), (dict(R=4, q_bias=0x1000, bias_cache=0x1000, bias_heads=3), -7),
                                          (dict(R=4, q_bias=0x1000, bias_cache=0x1000, bias_heads=2, slopes=0x1000), -7),
-                                         (dict(tree_mask=0x1000), -5), (dict(key_cache_stride=BAD_STRIDE), -4), (dict(q_stride=_lib.I64x2(-1, 1)), -4)],
+                                         (dict(tree_mask=0x1000), -5), (dict(key_cache_stride=BAD_STRIDE), -4), (dict(q_stride=_lib.I64x2(-1, 1)), -4),
+                                         (dict(workspace=None), -6), (dict(workspace=0x1000, workspace_bytes=64), -6)],
                          ids=str)
 def test_paged_attention_refuses(change, code):
     assert refused("fb_paged_fwd", paged_params, change) == code
@@ -163,3 +164,18 @@ def test_oracle_gradients_against_differences(norm, interleaved):
         e[i] = h
         num = ((orc.norm_rope(x, w + e, ang, interleaved) - orc.norm_rope(x, w - e, ang, interleaved)) * d).sum() / (2 * h)
         assert abs(float(num - dw[i])) < 1e-7
+
+
+@pytest.mark.parametrize("change,kernel", [
+    (dict(), "split"), (dict(N=2 * 16), "split"), (dict(N=2 * 17), "tile"), (dict(N=34, Hq=2), "split"), (dict(N=66, Hq=2), "tile"),
+    (dict(N=34, page_size=8), "tile"), (dict(N=34, page_size=24), "split"), (dict(N=34, page_size=4), "split"), (dict(N=34, page_size=256), "tile"),
+    (dict(N=34, softmax_scale=-1.0), "split"), (dict(N=34, flags=_lib.FB_FLAG_PAGED_SPLIT), "split"), (dict(D=20), "general"),
+    (dict(N=34, D=128, o_stride=_lib.I64x2(512, 128)), "tile"), (dict(key_cache=0x1008), "general"), (dict(key_cache_stride=_lib.I64x3(4096, 64, 257)), "general"),
+    (dict(N=34, key_cache_stride=_lib.I64x3(4096, 0, 256)), "split"), (dict(flags=_lib.FB_FLAG_FORCE_GENERAL), "general"),
+    (dict(N=34, R=4, q_bias=0x1000, bias_cache=0x1000, bias_heads=2), "split")], ids=str)
+def test_the_query_names_the_kernel_of_paged_attention(change, kernel):
+    p = paged_params()
+    for n, v in change.items():
+        setattr(p, n, v)
+    assert _lib.PAGED_KERNELS[_lib.load().fb_paged_kernel(C.byref(p))] == kernel
+    assert (_lib.load().fb_paged_workspace_bytes(C.byref(p)) > 0) == (kernel != "general")
