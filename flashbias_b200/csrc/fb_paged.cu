@@ -149,7 +149,9 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
   cudaGetDevice(&dev);
   const int sms = device_sm_count(dev) > 0 ? device_sm_count(dev) : 148;
   // More rows than the split kernel holds side by side: 128 of them in a tcgen05 tile, if a tile of 128 keys is made of whole
-  // pages (or a page of whole tiles) that TMA can address, and the scale may be taken out of a maximum.
+  // pages (or a page of whole tiles) that TMA can address, and the scale may be taken out of a maximum.  Tile / split kernel, us:
+  // 33 rows (B26 T11 H16-4 D128, 747 keys) 27.6 / 32.0, 45 rows (B16 T30 H16-8 D64) over 400 keys 24.7 / 28.9, over 1600 28.1 /
+  // 25.4, 120 rows (B26 T40 H16-4 D128, 747 keys) 31 / 68.
   const bool tma = tma_compatible(p->key_cache, p->key_cache_stride[1], p->key_cache_stride[2], p->key_cache_stride[0], p->Hk, p->num_pages) &&
                    tma_compatible(p->value_cache, p->value_cache_stride[1], p->value_cache_stride[2], p->value_cache_stride[0], p->Hk, p->num_pages);
   if (rows > 32 && !(p->flags & FB_FLAG_PAGED_SPLIT) && tma && p->R == 0 && p->softmax_scale > 1e-20f && p->page_size % 8 == 0 && (128 % p->page_size == 0 || p->page_size % 128 == 0) &&
@@ -169,6 +171,9 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
     const int64_t tiles = (int64_t)p->B * (((int64_t)p->table_width * p->page_size + 63) / 64) * p->Hk;
     plan.WH = p->Hk % 4 == 0 && tiles / 4 >= 4 * plan.ctas ? 4 : p->Hk % 2 == 0 && tiles / 2 >= 4 * plan.ctas ? 2 : 1;
   }
+  // items: row tiles (of every request at least one) times head groups
+  const int64_t items = (int64_t)p->B * ((rows + plan.MT - 1) / plan.MT) * (p->Hk / plan.WH);
+  plan.many_parts = items * 8 < plan.ctas;
   const size_t prows = (size_t)plan.ctas * 2 * plan.WH * plan.MT;
   plan.part_bytes = round256(prows * plan.TD * 4);
   plan.ml_bytes = round256(prows * 8);

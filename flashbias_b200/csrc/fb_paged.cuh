@@ -9,6 +9,8 @@
 
 #include <float.h>
 
+#include <type_traits>
+
 #include "fb_common.cuh"
 #include "fb_internal.h"
 
@@ -187,6 +189,7 @@ struct PagedPlan {
   int TD, MT;  // columns and rows of a tile
   int WH;      // key heads of a group
   int ctas;
+  bool many_parts;  // items are spread over more than eight CTAs on average, if they are as long as the table can hold
   size_t part_bytes, ml_bytes, desc_bytes;
 };
 int launch_paged_split_d32(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st);
@@ -197,50 +200,73 @@ int launch_paged_tile_d128(const PagedArgs& a, const PagedPlan& plan, cudaStream
 
 // Joins the parts of the item that begins in CTA blockIdx.x; TD / 4 lanes per row, the parts in the order of the CTAs.  Latency
 // is all there is to it: what the rows need stands in the descriptor, and the first parts are on their way before the maximum
-// is known.
+// is known.  ROWS: rows of a block; where few items are spread over many CTAs one, whose parts the block's lanes share (12 rows
+// over 11772 keys, two heads, 148 parts each: 34 us a call with four rows per block).
 constexpr int kJoinThreads = 128;  // (of 512 an SM holds one, and most have nothing to join)
-template <typename T, int TD>
+template <typename T, int TD, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, const int WH, const int MT) {
-  constexpr int LANES = TD / 4, U = 8;  // lanes of a row, parts in flight
+  constexpr int LANES = TD / 4, U = 8, SHARE = kJoinThreads / LANES / ROWS;  // lanes of a row, parts in flight, groups of lanes of a row
+  __shared__ float4 s_acc[SHARE > 1 ? kJoinThreads : 1];
+  __shared__ float2 s_ml[SHARE > 1 ? SHARE : 1];
   grid_dep_wait();
   const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
   if (d.x < 0) return;
   const fb_paged_params& p = a.p;
-  const int lane = threadIdx.x % LANES, idx = blockIdx.y * (kJoinThreads / LANES) + threadIdx.x / LANES;
-  const int wh = idx / MT, r = idx - wh * MT, gr = d.x * MT + r, parts = d.z - (int)blockIdx.x + 1;
-  if (gr >= e.y) return;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, share = SHARE > 1 ? group : 0;
+  const int idx = blockIdx.y * ROWS + (SHARE > 1 ? 0 : group);
+  const int wh = idx / MT, r = idx - wh * MT, gr = d.x * MT + r, all = d.z - (int)blockIdx.x + 1;
+  if (gr >= e.y) return;  // (SHARE > 1: the whole block)
   const int64_t step = (int64_t)2 * WH * MT;  // rows of a CTA
   const int64_t row0 = blockIdx.x * step + (int64_t)(WH + wh) * MT + r, row1 = (int64_t)(blockIdx.x + 1) * step + (int64_t)wh * MT + r;
-  auto row_of = [&](int i) { return i == 0 ? row0 : row1 + (i - 1) * step; };
-  float4 v[U];
-  float2 s[U];
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t row = row_of(min(i0 + u, parts - 1));
-      s[u] = a.ml[row];
-      v[u] = reinterpret_cast<const float4*>(a.part + row * TD)[lane];
-    }
-  };
-  load(0);
-  float m = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < U; ++u) m = fmaxf(m, s[u].x);
-#pragma unroll 4
-  for (int i = U; i < parts; ++i) m = fmaxf(m, a.ml[row_of(i)].x);
-  const float ms = fmaxf(m, -FLT_MAX);
-  float l = 0.f;
+  // this group's parts: share, share + SHARE, ...
+  const int parts = (all - share + SHARE - 1) / SHARE;
+  auto row_of = [&](int i) { return i * SHARE + share == 0 ? row0 : row1 + (i * SHARE + share - 1) * step; };
+  float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0;;) {
+  if (parts > 0) {
+    float4 v[U];
+    float2 s[U];
+    auto load = [&](int i0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i0 + u >= parts) break;
-      const float f = fast_exp2(s[u].x - ms);
-      l = fmaf(s[u].y, f, l);
-      acc = make_float4(fmaf(v[u].x, f, acc.x), fmaf(v[u].y, f, acc.y), fmaf(v[u].z, f, acc.z), fmaf(v[u].w, f, acc.w));
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = row_of(min(i0 + u, parts - 1));
+        s[u] = a.ml[row];
+        v[u] = reinterpret_cast<const float4*>(a.part + row * TD)[lane];
+      }
+    };
+    load(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = fmaxf(m, s[u].x);
+#pragma unroll 4
+    for (int i = U; i < parts; ++i) m = fmaxf(m, a.ml[row_of(i)].x);
+    const float ms = fmaxf(m, -FLT_MAX);
+    for (int i0 = 0;;) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u >= parts) break;
+        const float f = fast_exp2(s[u].x - ms);
+        l = fmaf(s[u].y, f, l);
+        acc = make_float4(fmaf(v[u].x, f, acc.x), fmaf(v[u].y, f, acc.y), fmaf(v[u].z, f, acc.z), fmaf(v[u].w, f, acc.w));
+      }
+      if ((i0 += U) >= parts) break;
+      load(i0);
     }
-    if ((i0 += U) >= parts) break;
-    load(i0);
+  }
+  if (SHARE > 1) {
+    s_acc[threadIdx.x] = acc;
+    if (lane == 0) s_ml[share] = make_float2(m, l);
+    __syncthreads();
+    if (share > 0) return;
+    for (int g = 0; g < SHARE; ++g) m = fmaxf(m, s_ml[g].x);
+    const float ms = fmaxf(m, -FLT_MAX);
+    l = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g = 0; g < SHARE; ++g) {
+      const float f = fast_exp2(s_ml[g].x - ms);
+      const float4 v = s_acc[g * LANES + lane];
+      l = fmaf(s_ml[g].y, f, l);
+      acc = make_float4(fmaf(v.x, f, acc.x), fmaf(v.y, f, acc.y), fmaf(v.z, f, acc.z), fmaf(v.w, f, acc.w));
+    }
   }
   const int t = a.group_div.quot32(gr), h = (d.y * WH + wh) * a.G + gr - t * a.G, n = e.x + t;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
@@ -270,9 +296,15 @@ int launch_pdl_2d(void (*kern)(P...), dim3 grid, unsigned block, cudaStream_t st
 // (an item may begin in any CTA and end in a later one)
 template <int TD>
 int launch_paged_join(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
-  const dim3 grid(plan.ctas, plan.WH * plan.MT / (kJoinThreads / (TD / 4)));
-  return a.p.dtype == FB_DTYPE_F16 ? launch_pdl_2d(paged_join_kernel<__half, TD>, grid, kJoinThreads, st, a, plan.WH, plan.MT)
-                                   : launch_pdl_2d(paged_join_kernel<__nv_bfloat16, TD>, grid, kJoinThreads, st, a, plan.WH, plan.MT);
+  constexpr int ROWS = kJoinThreads / (TD / 4);
+  auto go = [&](auto t, auto rows) {
+    return launch_pdl_2d(paged_join_kernel<decltype(t), TD, decltype(rows)::value>, dim3(plan.ctas, plan.WH * plan.MT / decltype(rows)::value), kJoinThreads,
+                         st, a, plan.WH, plan.MT);
+  };
+  auto by_parts = [&](auto t) {
+    return plan.many_parts ? go(t, std::integral_constant<int, 1>()) : go(t, std::integral_constant<int, ROWS>());
+  };
+  return a.p.dtype == FB_DTYPE_F16 ? by_parts(__half()) : by_parts(__nv_bfloat16());
 }
 
 }  // namespace fb

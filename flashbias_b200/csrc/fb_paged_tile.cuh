@@ -587,40 +587,70 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   }
 }
 
-// Joins the parts of the item that begins in CTA blockIdx.x, in the order of the CTAs: thread = row, 32 columns.
-template <typename T, int TD>
-__global__ void __launch_bounds__(128) paged_join_tile_kernel(const __grid_constant__ PagedArgs a) {
+// Joins the parts of the item that begins in CTA blockIdx.x, in the order of the CTAs: thread = row.  32 columns per block, or
+// where few items are spread over many CTAs (SHARE = 4) 8 columns, and a quarter of the parts per thread (64 tokens over 11772
+// keys, two heads, 74 parts each: 72 us a call with one thread per row, 27 so).
+template <typename T, int TD, int SHARE>
+__global__ void __launch_bounds__(128 * SHARE) paged_join_tile_kernel(const __grid_constant__ PagedArgs a) {
+  constexpr int G = SHARE > 1 ? 2 : 8, U = SHARE > 1 ? 4 : 2;  // float4 of a thread; parts in flight
+  __shared__ float4 s_acc[SHARE > 1 ? SHARE : 1][SHARE > 1 ? G : 1][SHARE > 1 ? 128 : 1];
+  __shared__ float2 s_ml[SHARE > 1 ? SHARE : 1][SHARE > 1 ? 128 : 1];
   grid_dep_wait();
   const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
   if (d.x < 0) return;
   const fb_paged_params& p = a.p;
-  const int row = threadIdx.x, gr = d.x * 128 + row, col0 = blockIdx.y * 32, parts = d.z - (int)blockIdx.x + 1;
-  if (gr >= e.y) return;
-  const int t = a.group_div.quot32(gr), h = d.y * a.G + gr - t * a.G, n = e.x + t;
-  auto slot_of = [&](int i) { return (int64_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, a.ml[slot_of(i) * 128 + row].x);
-  const float ms = fmaxf(m, -FLT_MAX);
-  float l = 0.f;
-  float4 acc[8] = {};
-#pragma unroll 2
-  for (int i = 0; i < parts; ++i) {
-    const float2 s = a.ml[slot_of(i) * 128 + row];
-    const float f = fast_exp2(s.x - ms);
-    l = fmaf(s.y, f, l);
-    const float4* src = reinterpret_cast<const float4*>(a.part) + (slot_of(i) * (TD / 4) + col0 / 4) * 128 + row;
+  const int row = threadIdx.x & 127, share = threadIdx.x >> 7, gr = d.x * 128 + row, col0 = blockIdx.y * 4 * G, all = d.z - (int)blockIdx.x + 1;
+  const int parts = (all - share + SHARE - 1) / SHARE;  // share, share + SHARE, ...
+  auto slot_of = [&](int i) { return (int64_t)(blockIdx.x + i * SHARE + share) * 2 + (i * SHARE + share == 0 ? 1 : 0); };
+  const bool live = gr < e.y;
+  float m = -INFINITY, l = 0.f;
+  float4 acc[G] = {};
+  if (live && parts > 0) {
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, a.ml[slot_of(i) * 128 + row].x);
+    const float ms = fmaxf(m, -FLT_MAX);
+#pragma unroll U
+    for (int i = 0; i < parts; ++i) {
+      const float2 s = a.ml[slot_of(i) * 128 + row];
+      const float f = fast_exp2(s.x - ms);
+      l = fmaf(s.y, f, l);
+      const float4* src = reinterpret_cast<const float4*>(a.part) + (slot_of(i) * (TD / 4) + col0 / 4) * 128 + row;
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      const float4 v = src[g * 128];
-      acc[g] = make_float4(fmaf(v.x, f, acc[g].x), fmaf(v.y, f, acc[g].y), fmaf(v.z, f, acc[g].z), fmaf(v.w, f, acc[g].w));
+      for (int g = 0; g < G; ++g) {
+        const float4 v = src[g * 128];
+        acc[g] = make_float4(fmaf(v.x, f, acc[g].x), fmaf(v.y, f, acc[g].y), fmaf(v.z, f, acc[g].z), fmaf(v.w, f, acc[g].w));
+      }
     }
   }
+  if (SHARE > 1) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) s_acc[share][g][row] = acc[g];
+    s_ml[share][row] = make_float2(m, l);
+    __syncthreads();
+    if (share > 0) return;
+    for (int x = 1; x < SHARE; ++x) m = fmaxf(m, s_ml[x][row].x);
+    const float ms = fmaxf(m, -FLT_MAX);
+    l = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) acc[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = 0; x < SHARE; ++x) {
+      const float2 s = s_ml[x][row];
+      const float f = fast_exp2(s.x - ms);
+      l = fmaf(s.y, f, l);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float4 v = s_acc[x][g][row];
+        acc[g] = make_float4(fmaf(v.x, f, acc[g].x), fmaf(v.y, f, acc[g].y), fmaf(v.z, f, acc[g].z), fmaf(v.w, f, acc[g].w));
+      }
+    }
+  }
+  if (!live) return;
+  const int t = a.group_div.quot32(gr), h = d.y * a.G + gr - t * a.G, n = e.x + t;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   T* dst = reinterpret_cast<T*>(p.o) + (int64_t)n * p.o_stride[0] + h * p.o_stride[1] + col0;
   auto p2 = [&](float x, float y) { return l == 0.f ? 0u : Pack2<T>::pack(x * inv, y * inv); };
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
+  for (int g = 0; g < G / 2; ++g)
     if (col0 + g * 8 < p.D)
       *reinterpret_cast<uint4*>(dst + g * 8) = make_uint4(p2(acc[2 * g].x, acc[2 * g].y), p2(acc[2 * g].z, acc[2 * g].w), p2(acc[2 * g + 1].x, acc[2 * g + 1].y),
                                                           p2(acc[2 * g + 1].z, acc[2 * g + 1].w));
@@ -643,7 +673,8 @@ int launch_paged_tile_t(const PagedArgs& a, const PagedPlan& plan, const CUtenso
     }
   }
   if (const int rc = launch_pdl(kern, plan.ctas, kTileThreads, TileCfg<TD>::SMEM, st, tk, tv, a)) return rc;
-  return launch_pdl_2d(paged_join_tile_kernel<T, TD>, dim3(plan.ctas, TD / 32), 128, st, a);
+  return plan.many_parts ? launch_pdl_2d(paged_join_tile_kernel<T, TD, 4>, dim3(plan.ctas, TD / 8), 512, st, a)
+                         : launch_pdl_2d(paged_join_tile_kernel<T, TD, 1>, dim3(plan.ctas, TD / 32), 128, st, a);
 }
 
 template <int TD>
