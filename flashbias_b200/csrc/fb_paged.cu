@@ -174,6 +174,9 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
   // items: row tiles (of every request at least one) times head groups
   const int64_t items = (int64_t)p->B * ((rows + plan.MT - 1) / plan.MT) * (p->Hk / plan.WH);
   plan.many_parts = items * 8 < plan.ctas;
+  // 12 rows over 11772 keys, two heads: 18.6 us with all CTAs (184 with two tiles each), 14.5 with 92.  Where an item has no more
+  // than 32 parts it is the other way about (one token over 1000 keys, 8 heads: 10.6 us with a tile per CTA, 12.5 with four).
+  plan.spread = plan.kernel == FB_PAGED_SPLIT && items * 32 < plan.ctas ? (int)(items * 32) : plan.ctas;
   const size_t prows = (size_t)plan.ctas * 2 * plan.WH * plan.MT;
   plan.part_bytes = round256(prows * plan.TD * 4);
   plan.ml_bytes = round256(prows * 8);
@@ -210,6 +213,7 @@ extern "C" int fb_paged_fwd(const fb_paged_params* p, void* cuda_stream) {
     a.G = p->Hq / p->Hk;
     a.page_div = Div(p->page_size);
     a.group_div = Div(a.G);
+    a.spread = plan.spread;
     a.whole_tiles = p->page_size % 16 == 0;
     a.pages32 = (uint32_t)(p->num_pages < 0x7fffffffLL ? p->num_pages : 0x7fffffffLL);
     if (p->R) {  // what the rows of the factors are aligned to

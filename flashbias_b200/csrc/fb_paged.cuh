@@ -28,6 +28,7 @@ struct PagedArgs {
   fb_paged_params p;
   Div page_div, group_div;  // by page_size, by the query heads of a key head
   int G;                    // query heads of a key head
+  int spread;               // more CTAs than this only if each has four key tiles: the parts of an item have to be joined again
   int whole_tiles;          // split kernel: pages are whole runs of 16 keys
   uint32_t pages32;         // num_pages, within 31 bits: what a page of the table is compared with
   int factor_words;         // split kernel: factor rows can be read two columns at a time
@@ -130,7 +131,8 @@ struct PagedWalk {
       if (w < warp) before += s_sum[w];
       total += s_sum[w];
     }
-    ctas = (int)min((int64_t)gridDim.x, total);  // each of these has one number at least: an item's parts leave no gap
+    // each of these has one number at least: an item's parts leave no gap
+    ctas = (int)min(min((int64_t)gridDim.x, total), max((int64_t)a.spread, total / 4));
     u = blockIdx.x < ctas ? quotient(blockIdx.x * total, ctas) : total;
     u1 = blockIdx.x < ctas ? quotient((blockIdx.x + 1) * total, ctas) : total;
     if (u < u1 && before <= u && u < before + mine) {
@@ -189,6 +191,7 @@ struct PagedPlan {
   int TD, MT;  // columns and rows of a tile
   int WH;      // key heads of a group
   int ctas;
+  int spread;       // of PagedArgs
   bool many_parts;  // items are spread over more than eight CTAs on average, if they are as long as the table can hold
   size_t part_bytes, ml_bytes, desc_bytes;
 };
