@@ -104,13 +104,13 @@ struct PagedWalk {
     return r.tokens ? (int64_t)row_tiles(a, r) * key_tiles(r) * ngroups : 0;
   }
 
-  // Finds the request in which the CTA's range begins: each thread adds up a run of requests, a scan over the threads.
-  __device__ __forceinline__ void start(const PagedArgs& a, int groups) {
+  // Finds the request in which the range of CTA `me` of `n` begins: each thread adds up a run of requests, a scan over the threads.
+  __device__ __forceinline__ void start(const PagedArgs& a, int groups, int me, int n) {
     __shared__ int64_t s_sum[THREADS / 32], s_pre;
     __shared__ int s_b;
     __shared__ Request s_r;
     ngroups = groups;
-    const int n = a.p.B + 2, per = (n + THREADS - 1) / THREADS, b0 = threadIdx.x * per, b1 = min(b0 + per, n);
+    const int nr = a.p.B + 2, per = (nr + THREADS - 1) / THREADS, b0 = threadIdx.x * per, b1 = min(b0 + per, nr);
     int64_t mine = 0;
     Request mr = {0, 0, -1, 0};  // the last of the run: all of it while there are fewer requests than threads
     for (int i = b0; i < b1; ++i) mine += units(a, mr = request_at(a.p, i), groups);
@@ -132,9 +132,9 @@ struct PagedWalk {
       total += s_sum[w];
     }
     // each of these has one number at least: an item's parts leave no gap
-    ctas = (int)min(min((int64_t)gridDim.x, total), max((int64_t)a.spread, total / 4));
-    u = blockIdx.x < ctas ? quotient(blockIdx.x * total, ctas) : total;
-    u1 = blockIdx.x < ctas ? quotient((blockIdx.x + 1) * total, ctas) : total;
+    ctas = (int)min(min((int64_t)n, total), max((int64_t)a.spread, total / 4));
+    u = me < ctas ? quotient(me * total, ctas) : total;
+    u1 = me < ctas ? quotient((me + 1) * total, ctas) : total;
     if (u < u1 && before <= u && u < before + mine) {
       int64_t at = before;
       int i = b0;
@@ -183,6 +183,15 @@ __device__ __forceinline__ bool tree_sees(const fb_paged_params& p, int n, int t
   return w < p.mask_words && ((p.tree_mask[n * p.mask_stride + w] >> (td & 63)) & 1);
 }
 
+// The 32 keys from drafted token td0 on (negative: cached ones) that a row of token t (global token n) sees, as bits.
+__device__ __forceinline__ uint32_t seen_bits(const fb_paged_params& p, int n, int t, int td0) {
+  if (!p.tree_mask) return td0 > t ? 0u : t - td0 >= 31 ? 0xffffffffu : (2u << (t - td0)) - 1u;
+  const int64_t* words = p.tree_mask + n * p.mask_stride;
+  auto word = [&](int w) { return w < 0 ? ~0ull : w < p.mask_words ? (uint64_t)words[w] : 0ull; };
+  const int w = td0 >> 6, s = td0 & 63;
+  return (uint32_t)(s ? (word(w) >> s) | (word(w + 1) << (64 - s)) : word(w));
+}
+
 // ---- host side (fb_paged.cu, fb_paged_split_*.cu, fb_paged_tile_*.cu) ------------------------------------------------
 // CTAs of the split kernel that an SM holds: three while their warps' output rows leave the registers for it
 constexpr int split_ctas(int TD, int MT) { return TD < 128 && MT == 16 ? 3 : 2; }
@@ -192,6 +201,7 @@ struct PagedPlan {
   int WH;      // key heads of a group
   int ctas;
   int spread;       // of PagedArgs
+  int cluster;      // split kernel: CTAs of an item, in one cluster; 0: the schedule
   bool many_parts;  // items are spread over more than eight CTAs on average, if they are as long as the table can hold
   size_t part_bytes, ml_bytes, desc_bytes;
 };

@@ -7,7 +7,13 @@
 // from, and the tensor pipe is far from being the bound; a tcgen05 tile would spend 112 of its 128 rows on padding.  No
 // barrier is needed between warps while a segment lasts; where a group has fewer heads than the CTA has warps, the warps of a
 // head join their sums through shared memory at the segment's end.
+//
+// With few items (one or two requests of a few heads) latency is what counts, and the second launch half of it: CLUSTER gives
+// every item to the CTAs of one cluster, which cut its key tiles into equal parts and join them through distributed shared
+// memory (one token over 1000 keys, 8 heads: 10.6 us a call with the schedule and a join, 9.6 so).
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include <mutex>
 
@@ -61,7 +67,61 @@ __device__ __forceinline__ bool pair_not_finite(uint32_t w) {
 // PAGED_FACTORS_ANY: any others, read into registers.
 enum { PAGED_PLAIN, PAGED_SLOPES, PAGED_FACTORS, PAGED_FACTORS_ANY };
 
-template <typename T, int TD, int MT, int BIAS>
+// The parts of an item that the CTAs of a cluster hold (those of head wh in the registers of the warp with wk == 0), joined
+// through distributed shared memory: every CTA writes some of the rows.  The parts lie in the rings of the warps that hold them.
+template <typename T, int TD, int MT>
+__device__ __forceinline__ void join_cluster(const PagedArgs& a, const Segment& seg, int hk, uint8_t* smem, int wh, int wk, int WH,
+                                             const float (&o)[MT / 16][TD / 8][4], const float (&m)[MT / 16][2], const float (&l)[MT / 16][2]) {
+  using Cfg = SplitCfg<TD, MT>;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  constexpr int LANES = TD / 4;  // of a row
+  const fb_paged_params& p = a.p;
+  const int lane = threadIdx.x & 31, qr = lane >> 2, qc = 2 * (lane & 3), step = Cfg::RING * (kSplitWarps / WH);
+  float* mine = reinterpret_cast<float*>(smem + wh * step);  // (MT, TD), statistics behind
+  __syncthreads();
+  if (wk == 0) {
+#pragma unroll
+    for (int im = 0; im < MT / 16; ++im)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = im * 16 + e * 8 + qr;
+#pragma unroll
+        for (int i = 0; i < TD / 8; ++i) *reinterpret_cast<float2*>(mine + r * TD + i * 8 + qc) = make_float2(o[im][i][2 * e], o[im][i][2 * e + 1]);
+        if (qc == 0) reinterpret_cast<float2*>(mine + MT * TD)[r] = make_float2(m[im][e], l[im][e]);
+      }
+  }
+  cluster.sync();
+  const int csize = (int)cluster.num_blocks(), col = (threadIdx.x % LANES) * 4;
+  for (int i = (int)cluster.block_rank() * (kSplitThreads / LANES) + threadIdx.x / LANES; i < WH * MT; i += csize * (kSplitThreads / LANES)) {
+    const int h_in = i / MT, r = i - h_in * MT, gr = seg.rt * MT + r;
+    if (gr >= seg.r.tokens * a.G) continue;
+    float* part = reinterpret_cast<float*>(smem + h_in * step);
+    float mx = -INFINITY;
+    for (int c = 0; c < csize; ++c) mx = fmaxf(mx, reinterpret_cast<const float2*>(cluster.map_shared_rank(part, c) + MT * TD)[r].x);
+    const float ms = fmaxf(mx, -FLT_MAX);
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int c = 0; c < csize; ++c) {
+      const float* from = cluster.map_shared_rank(part, c);
+      const float2 s = reinterpret_cast<const float2*>(from + MT * TD)[r];
+      const float4 v = *reinterpret_cast<const float4*>(from + r * TD + col);
+      const float f = fast_exp2(s.x - ms);
+      sum = fmaf(s.y, f, sum);
+      acc = make_float4(fmaf(v.x, f, acc.x), fmaf(v.y, f, acc.y), fmaf(v.z, f, acc.z), fmaf(v.w, f, acc.w));
+    }
+    const int t = a.group_div.quot32(gr), h = (hk - wh + h_in) * a.G + gr - t * a.G, n = seg.r.first + t;
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    if (col < p.D)
+      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1] + col) =
+          sum == 0.f ? make_uint2(0u, 0u) : make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
+    if (p.lse && col == 0) p.lse[(int64_t)n * p.Hq + h] = sum > 0.f ? (mx + fast_log2(sum)) * kLn2P : sum == 0.f ? -INFINITY : sum;
+  }
+  cluster.sync();  // the parts have been read
+}
+
+template <typename T, int TD, int MT, int BIAS, bool CLUSTER>
 __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split_kernel(const __grid_constant__ PagedArgs a, const int WH) {
   using Cfg = SplitCfg<TD, MT>;
   constexpr int NM = MT / 16, KS = TD / 16, NT = TD / 8, ST = Cfg::ST, KT = Cfg::KT, NK = KT / 16, PER = kSplitKT / KT;
@@ -79,12 +139,19 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
   }
   const int qr = lane >> 2, qc = 2 * (lane & 3);  // a fragment's row (and row + 8) and first column of this lane
   grid_dep_wait();
-  if (threadIdx.x == 0) a.desc[2 * blockIdx.x].x = -1;
-  PagedWalk<kSplitKT, MT, kSplitThreads> walk;
-  walk.start(a, p.Hk / WH);
+  if (!CLUSTER && threadIdx.x == 0) a.desc[2 * blockIdx.x].x = -1;
+  // (a cluster walks whole items: one key tile each, as long as there are keys)
+  PagedWalk<CLUSTER ? 0x7fffffff : kSplitKT, MT, kSplitThreads> walk;
+  const int csize = CLUSTER ? (int)cooperative_groups::this_cluster().num_blocks() : 1, crank = CLUSTER ? (int)cooperative_groups::this_cluster().block_rank() : 0;
+  walk.start(a, p.Hk / WH, blockIdx.x / csize, gridDim.x / csize);
 
   Segment seg;
   while (walk.next(a, seg)) {
+    if (CLUSTER) {  // this CTA's part of the key tiles, possibly none
+      const int64_t tiles = ((int64_t)seg.r.keys + kSplitKT - 1) / kSplitKT;
+      seg.t0 = (int)(tiles * crank / csize);
+      seg.t1 = (int)(tiles * (crank + 1) / csize);
+    }
     const Request& rq = seg.r;
     const int hk = seg.hg * WH + wh, rows = rq.tokens * a.G - seg.rt * MT;  // rows of the request from this tile on
     const T* kbase = reinterpret_cast<const T*>(p.key_cache) + hk * p.key_cache_stride[2];
@@ -354,21 +421,23 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
             s[im][nt][i] = v;
           }
       if (masked) {
+        const int td0 = tile * KT - rq.len;
 #pragma unroll
         for (int im = 0; im < NM; ++im)
 #pragma unroll
-          for (int nt = 0; nt < 2 * NK; ++nt)
+          for (int e = 0; e < 2; ++e) {  // what the row sees of the tile
+            uint32_t bits = okm;
+            if (row_tok[im][e] >= 0 && td0 + KT > 0) bits &= seen_bits(p, rq.first + row_tok[im][e], row_tok[im][e], td0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int e = i >> 1, j = j0 + nt * 8 + (i & 1);
-              bool seen = (okm >> (j - tile * KT)) & 1;
-              if (seen && j >= rq.len) {
-                seen = row_tok[im][e] >= 0 && tree_sees(p, rq.first + row_tok[im][e], row_tok[im][e], j - rq.len);
-                if (BIAS == PAGED_SLOPES && p.positions)  // the key's position instead of its place
+            for (int nt = 0; nt < 2 * NK; ++nt)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int i = 2 * e + x, k = nt * 8 + qc + x, j = tile * KT + k;
+                if (BIAS == PAGED_SLOPES && p.positions && j >= rq.len && j < rq.keys)  // the key's position instead of its place
                   s[im][nt][i] = fmaf(slope2[im][e], (float)(p.positions[rq.first + j - rq.len] - j), s[im][nt][i]);
+                if (!(bits >> k & 1)) s[im][nt][i] = -INFINITY;
               }
-              if (!seen) s[im][nt][i] = -INFINITY;
-            }
+          }
       }
 
       // ---- running maximum and sum, P as fragments
@@ -415,7 +484,7 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
       bool odd = false;
       if (masked) {
         bool mine = false;
-#pragma unroll 1
+#pragma unroll 4
         for (int i = 0; i < Cfg::HALF / 512; ++i) {
           const uint4 w = *reinterpret_cast<const uint4*>(smem + warp * Cfg::RING + (vs_base - ring) + (i * 32 + lane) * 16);
           mine |= pair_not_finite<T>(w.x) || pair_not_finite<T>(w.y) || pair_not_finite<T>(w.z) || pair_not_finite<T>(w.w);
@@ -524,6 +593,10 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
       }
       __syncthreads();
     }
+    if constexpr (CLUSTER) {
+      join_cluster<T, TD, MT>(a, seg, hk, smem, wh, wk, WH, o, m, l);
+      continue;
+    }
     const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
     if (wk == 0) {
 #pragma unroll
@@ -560,9 +633,9 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
   }
 }
 
-template <typename T, int TD, int MT, int BIAS>
+template <typename T, int TD, int MT, int BIAS, bool CLUSTER>
 int launch_paged_split_t(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
-  auto kern = paged_split_kernel<T, TD, MT, BIAS>;
+  auto kern = paged_split_kernel<T, TD, MT, BIAS, CLUSTER>;
   constexpr int SMEM = SplitCfg<TD, MT>::smem(BIAS == PAGED_FACTORS);
   static std::mutex mu;
   static bool attr_done[64] = {};
@@ -571,13 +644,32 @@ int launch_paged_split_t(const PagedArgs& a, const PagedPlan& plan, cudaStream_t
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!attr_done[dev & 63]) {
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+      if (e == cudaSuccess && CLUSTER) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e != cudaSuccess) return (int)e;
       attr_done[dev & 63] = true;
     }
   }
-  if (const int rc = launch_pdl(kern, plan.ctas, kSplitThreads, SMEM, st, a, plan.WH)) return rc;
-  return launch_paged_join<TD>(a, plan, st);
+  if (!CLUSTER) {
+    if (const int rc = launch_pdl(kern, plan.ctas, kSplitThreads, SMEM, st, a, plan.WH)) return rc;
+    return launch_paged_join<TD>(a, plan, st);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.ctas);
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = plan.cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, plan.WH);
+  if (e == cudaSuccess) note_launch();
+  return (int)e;
 }
 
 template <int TD>
@@ -585,10 +677,14 @@ int launch_paged_split(const PagedArgs& a, const PagedPlan& plan, cudaStream_t s
   auto by_bias = [&](auto t, auto mt) {
     using T = decltype(t);
     constexpr int MT = decltype(mt)::value;
-    return a.p.slopes ? launch_paged_split_t<T, TD, MT, PAGED_SLOPES>(a, plan, st)
-           : a.p.R && a.factor_bytes ? launch_paged_split_t<T, TD, MT, PAGED_FACTORS>(a, plan, st)
-           : a.p.R                   ? launch_paged_split_t<T, TD, MT, PAGED_FACTORS_ANY>(a, plan, st)
-                                     : launch_paged_split_t<T, TD, MT, PAGED_PLAIN>(a, plan, st);
+    auto go = [&](auto bias) {
+      constexpr int BIAS = decltype(bias)::value;
+      return plan.cluster ? launch_paged_split_t<T, TD, MT, BIAS, true>(a, plan, st) : launch_paged_split_t<T, TD, MT, BIAS, false>(a, plan, st);
+    };
+    return a.p.slopes                ? go(std::integral_constant<int, PAGED_SLOPES>())
+           : a.p.R && a.factor_bytes ? go(std::integral_constant<int, PAGED_FACTORS>())
+           : a.p.R                   ? go(std::integral_constant<int, PAGED_FACTORS_ANY>())
+                                     : go(std::integral_constant<int, PAGED_PLAIN>());
   };
   auto by_rows = [&](auto t) {
     return plan.MT == 16 ? by_bias(t, std::integral_constant<int, 16>()) : by_bias(t, std::integral_constant<int, 32>());

@@ -42,15 +42,6 @@ struct TileSeg {
 };
 static_assert(sizeof(TileSeg) <= 64, "room in shared memory");
 
-// The 32 keys from drafted token td0 on (negative: cached ones) that a row of token t (global token n) sees, as bits.
-__device__ __forceinline__ uint32_t seen_bits(const fb_paged_params& p, int n, int t, int td0) {
-  if (!p.tree_mask) return td0 > t ? 0u : t - td0 >= 31 ? 0xffffffffu : (2u << (t - td0)) - 1u;
-  const int64_t* words = p.tree_mask + n * p.mask_stride;
-  auto word = [&](int w) { return w < 0 ? ~0ull : w < p.mask_words ? (uint64_t)words[w] : 0ull; };
-  const int w = td0 >> 6, s = td0 & 63;
-  return (uint32_t)(s ? (word(w) >> s) | (word(w + 1) << (64 - s)) : word(w));
-}
-
 template <typename T, int TD, bool SLOPES>
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PagedArgs a) {
@@ -110,7 +101,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   grid_dep_wait();
   if (threadIdx.x == 0) a.desc[2 * blockIdx.x].x = -1;
   PagedWalk<128, 128, kTileThreads> walk;
-  walk.start(a, p.Hk);
+  walk.start(a, p.Hk, blockIdx.x, gridDim.x);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();

@@ -409,3 +409,25 @@ def test_two_graphs_and_an_eager_call_do_not_share_their_scratch():
         eager = flash_bias_paged_func(**ds[0])
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want)) and torch.equal(eager, want[0])
+
+
+@pytest.mark.parametrize("lens,new,Hq,Hk,D", [([1000], [1], 8, 4, 128), ([5], [1], 8, 4, 64), ([40, 700], [1, 1], 4, 1, 64), ([300, 0, -1, 90], [1, 2, 1, 0], 4, 2, 128),
+                                              ([129], [2], 16, 2, 96), ([2100, 17], [2, 1], 16, 2, 32), ([33, 64, 0], [1, 6, 10], 4, 1, 128)])
+@pytest.mark.parametrize("bias", ["none", "slopes", "factors", "tree"])
+def test_few_requests_with_narrow_and_wide_tables(lens, new, Hq, Hk, D, bias):
+    """Short tables: each item is a cluster's, and the parts meet in shared memory; long ones: the schedule over the whole GPU."""
+    kw = paged_inputs(lens, new, Hq, Hk, D, 16, torch.bfloat16, 26, 4 if bias == "factors" else 0)
+    if bias == "slopes":
+        kw["slopes"] = torch.linspace(0.3, 0.01, Hq)
+    if bias == "tree":
+        kw["tree_mask"] = tree(new, 27, 1)[1]
+    # two tokens behind the last request stay unowned
+    kw["q"] = torch.cat([kw["q"], kw["q"][-1:].expand(2, -1, -1)])
+    for n in ("q_bias", "tree_mask"):
+        if kw.get(n) is not None:
+            kw[n] = torch.cat([kw[n], kw[n][-1:].expand(2, *kw[n].shape[1:])])
+    wide = torch.nn.functional.pad(kw["block_table"], (0, 600), value=-1)
+    assert kernel_of(kw) == kernel_of({**kw, "block_table": wide}) == "split"
+    a = check(kw)
+    b = check(kw, block_table=wide)
+    assert (a[-2:] == 0).all() and (b[-2:] == 0).all()

@@ -36,8 +36,8 @@ def plan_params():
 
 def paged_params():
     p = _lib.FbPagedParams()
-    p.N, p.B, p.Hq, p.Hk, p.D, p.dtype, p.page_size, p.table_width, p.num_pages = 4, 2, 4, 2, 64, _lib.FB_DTYPE_F16, 16, 4, 8
-    p.softmax_scale, p.table_stride = 0.125, 4
+    p.N, p.B, p.Hq, p.Hk, p.D, p.dtype, p.page_size, p.table_width, p.num_pages = 4, 2, 4, 2, 64, _lib.FB_DTYPE_F16, 16, 4096, 8
+    p.softmax_scale, p.table_stride = 0.125, 4096
     for n in ("q", "key_cache", "value_cache", "block_table", "lens", "cu_tokens", "o"):
         setattr(p, n, 0x1000)
     for n in ("key_cache_stride", "value_cache_stride"):
@@ -179,3 +179,13 @@ def test_the_query_names_the_kernel_of_paged_attention(change, kernel):
         setattr(p, n, v)
     assert _lib.PAGED_KERNELS[_lib.load().fb_paged_kernel(C.byref(p))] == kernel
     assert (_lib.load().fb_paged_workspace_bytes(C.byref(p)) > 0) == (kernel != "general")
+
+
+@pytest.mark.parametrize("change,workspace", [(dict(), True), (dict(table_width=512), False), (dict(table_width=513), True),
+                                              (dict(table_width=512, N=8, B=8), False), (dict(table_width=512, N=64, B=64), True)], ids=str)
+def test_few_requests_over_short_tables_need_no_workspace(change, workspace):
+    p = paged_params()
+    for n, v in change.items():
+        setattr(p, n, v)
+    assert _lib.PAGED_KERNELS[_lib.load().fb_paged_kernel(C.byref(p))] == "split"
+    assert (_lib.load().fb_paged_workspace_bytes(C.byref(p)) > 0) == workspace
