@@ -29,7 +29,7 @@ TORCH_OP = os.path.join(PKG, "_torch_op.so")  # the operators' host path (csrc/t
 SOURCES = ["fb_api.cu", "fb_tmap.cu", "fb_pack.cu", "fb_finish.cu", "fb_general.cu", "fb_selftest.cu",
            "fb_fwd_sm100.cu", "fb_fwd_inst_d32.cu", "fb_fwd_inst_d64.cu", "fb_fwd_inst_d128.cu", "fb_fwd_inst_s128.cu",
            "fb_bwd_sm100.cu", "fb_bwd_inst_d32.cu", "fb_bwd_inst_d32p.cu", "fb_bwd_inst_d64.cu", "fb_bwd_inst_d128.cu", "fb_bwd_inst_s32.cu", "fb_bwd_inst_s64.cu",
-           "fb_decode.cu", "fb_noalloc.cu", "fb_prepare.cu", "fb_rope.cu", "fb_plan.cu", "fb_paged.cu", "fb_paged_split_d32.cu", "fb_paged_split_d64.cu",
+           "fb_decode.cu", "fb_noalloc.cu", "fb_prepare.cu", "fb_rope.cu", "fb_rope_f16.cu", "fb_rope_bf16.cu", "fb_plan.cu", "fb_paged.cu", "fb_paged_split_d32.cu", "fb_paged_split_d64.cu",
            "fb_paged_split_d128.cu", "fb_paged_tile_d64.cu", "fb_paged_tile_d128.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--use_fast_math", "-Xcompiler", "-fPIC", "-I", os.path.join(ROOT, "include"), "-I", CSRC]

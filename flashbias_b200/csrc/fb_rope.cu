@@ -8,54 +8,12 @@
 // reduced to a fraction of a turn before its sine and cosine are taken in 32 (by the functions of the hardware, off by 2^-21,
 // an eighth of a percent of a step of fp16): at position 1e6 a 32-bit product is off by up to 0.03 rad.  It costs one pair of
 // functions per token and frequency, shared by the token's heads, so no table is kept.
-#include <type_traits>
-
-#include "fb_common.cuh"
-#include "fb_internal.h"
+#include "fb_rope.cuh"
 
 namespace fb {
 
 constexpr int kRopeWarps = 4;
 constexpr int kRopeThreads = 32 * kRopeWarps;
-constexpr int kRopeMaxD = 128;
-constexpr double kInv2Pi = 0.15915494309189533576888;
-constexpr float k2Pi = 6.28318530717958647693f;
-
-__device__ __forceinline__ float load_scalar(const void* p, int dtype, int i) {
-  return dtype == FB_DTYPE_F32   ? reinterpret_cast<const float*>(p)[i]
-         : dtype == FB_DTYPE_F16 ? __half2float(reinterpret_cast<const __half*>(p)[i])
-                                 : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-}
-__device__ __forceinline__ void store_scalar(void* p, int dtype, int i, float v) {
-  if (dtype == FB_DTYPE_F32) reinterpret_cast<float*>(p)[i] = v;
-  else if (dtype == FB_DTYPE_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
-  else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-}
-
-// (cos, sin) of the angle of pair `pr` at token (b, s)
-__device__ __forceinline__ float2 rope_turn(const fb_rope_params& p, int b, int s, int pr) {
-  const int64_t at = p.pair_axis[pr] * p.position_stride[0] + b * p.position_stride[1] + s * p.position_stride[2];
-  const double pos = p.position_bits == 64 ? (double)reinterpret_cast<const int64_t*>(p.positions)[at]
-                                           : (double)reinterpret_cast<const int32_t*>(p.positions)[at];
-  const double f = p.freq_dtype == FB_DTYPE_F64 ? reinterpret_cast<const double*>(p.inv_freq)[pr]
-                                                : (double)reinterpret_cast<const float*>(p.inv_freq)[pr];
-  const double turns = pos * (f * kInv2Pi);
-  float2 cs;
-  __sincosf((float)(turns - rint(turns)) * k2Pi, &cs.y, &cs.x);  // within +-pi: off by 2^-21
-  return cs;
-}
-
-// Where token s goes in the cache; false if nowhere.
-__device__ __forceinline__ bool cache_place(const fb_rope_params& p, int s, int64_t& page, int& place) {
-  const int64_t slot = p.slot_bits == 64 ? reinterpret_cast<const int64_t*>(p.slots)[s * p.slot_stride]
-                                         : (int64_t) reinterpret_cast<const int32_t*>(p.slots)[s * p.slot_stride];
-  if (slot < 0) return false;
-  page = slot / p.page_size;
-  place = (int)(slot - page * p.page_size);
-  if (page < p.num_pages) return true;
-  if (p.status) *reinterpret_cast<volatile int32_t*>(p.status) = FB_DEV_BAD_INDEX;
-  return false;
-}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -160,7 +118,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_bwd_general_kernel(const __
       }
       __syncwarp();
       if (!w) {
-        for (int c = lane; c < p.D; c += 32) dx[c] = from_f32<T>(grad[c]);
+        for (int c = lane; c < p.D; c += 32) dx[c] = c < p.rot ? from_f32<T>(grad[c]) : go[c];
         __syncwarp();
         continue;
       }
@@ -225,403 +183,6 @@ __global__ void __launch_bounds__(1024) rope_weight_kernel(const __grid_constant
   if (out && c < p.D) store_scalar(out, p.weight_dtype, c, v);
 }
 
-// ---- vector kernels: rows of whole aligned 16-byte chunks -----------------------------------------------------------
-// A warp takes a token (or a share of its heads): G lanes (a power of two) share a row, 8 columns each, 32 / G rows side by
-// side.  Issue slots and the latency of a row's sums are what holds the rows back, not HBM: a warp issues about 110
-// instructions per 512 bytes (forward), at 6 warps per scheduler.  So all that depends on the column and the token alone
-// (weight times cosine, weight of the partner times sine) is folded into two coefficients per column that serve all heads of
-// the token, the address is one addition per row, and four rows (backward: two) are in flight per lane.
-// A lane holds both halves of its pairs: where they are half of the rotated columns apart (PAIR 0) it reads two runs of four
-// columns, where they are neighbours (1) one of eight.  Where the halves do not begin at a multiple of four (2) the other half
-// comes through shared memory.
-// B4 S4096 H32-8 D128 bf16, fp32 weights, us forward / backward: 64 (5.2 TB/s) / 117 (4.3 TB/s); with the other half by shuffle
-// 72 / 143, with coefficients from shared memory for every row and rows found by division 329 together.  Arithmetic on packed
-// pairs of fp32 issued as many instructions and was no faster; asking for the next token's rows ahead (L2) changed nothing.
-constexpr int kRopeVWarps = 4;
-constexpr int kRopeVThreads = 32 * kRopeVWarps;
-
-struct RopeV {
-  fb_rope_params p;
-  Div s_div;
-  int tokens;  // B S
-  int split;   // warps of a token
-  int q_ctas;  // backward: blocks that take rows of q, the others rows of k
-};
-
-template <typename T>
-__device__ __forceinline__ void unpack_chunk(const uint4& raw, float (&x)[8]) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (std::is_same<T, __nv_bfloat16>::value) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    } else {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
-}
-template <typename T>
-__device__ __forceinline__ uint4 pack_chunk(const float (&y)[8]) {
-  return make_uint4(Pack2<T>::pack(y[0], y[1]), Pack2<T>::pack(y[2], y[3]), Pack2<T>::pack(y[4], y[5]), Pack2<T>::pack(y[6], y[7]));
-}
-template <int G>
-__device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-// What a lane holds of every row: two runs of four columns, from c0 and c1 on.  PAIR 0: the first and the second halves of four
-// pairs, or eight columns in a row behind the rotated ones.  PAIR 1, 2: eight columns in a row.
-// FULL: the lanes' columns are those of the row, and all of them are rotated.
-template <typename T, int G, int PAIR, bool FULL>
-struct RopeLane {
-  int c0, c1;
-  bool in, turns;  // columns that exist; some of them rotated
-  __device__ __forceinline__ RopeLane(const fb_rope_params& p) {
-    const int part = (threadIdx.x & 31) % G;
-    c0 = part * 8;
-    in = FULL || c0 < p.D;
-    turns = FULL || c0 < p.rot;
-    if (!in) c0 = 0;  // (such a lane reads what exists and drops it)
-    c1 = c0 + 4;
-    if (PAIR == 0 && turns) {
-      c0 = part * 4;
-      c1 = c0 + (FULL ? 4 * G : p.rot >> 1);
-    }
-  }
-  __device__ __forceinline__ uint4 load(const T* row) const {
-    if (PAIR != 0) return __ldcs(reinterpret_cast<const uint4*>(row + c0));
-    const uint2 a = __ldcs(reinterpret_cast<const uint2*>(row + c0)), b = __ldcs(reinterpret_cast<const uint2*>(row + c1));
-    return make_uint4(a.x, a.y, b.x, b.y);
-  }
-  __device__ __forceinline__ void store(T* row, const uint4& w) const {
-    if (PAIR != 0) {
-      *reinterpret_cast<uint4*>(row + c0) = w;
-    } else {
-      *reinterpret_cast<uint2*>(row + c0) = make_uint2(w.x, w.y);
-      *reinterpret_cast<uint2*>(row + c1) = make_uint2(w.z, w.w);
-    }
-  }
-  // the weights of the columns (1 without weights)
-  __device__ __forceinline__ void weights(const void* w, int dtype, float (&out)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = 1.f;
-    if (!w || !in) return;
-    if (dtype == FB_DTYPE_F32) {
-      const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + c0), v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + c1);
-      out[0] = u.x; out[1] = u.y; out[2] = u.z; out[3] = u.w; out[4] = v.x; out[5] = v.y; out[6] = v.z; out[7] = v.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(w) + c0), v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(w) + c1);
-      if (dtype == FB_DTYPE_F16) unpack_chunk<__half>(make_uint4(u.x, u.y, v.x, v.y), out);
-      else unpack_chunk<__nv_bfloat16>(make_uint4(u.x, u.y, v.x, v.y), out);
-    }
-  }
-  // Coefficients of (own, partner's) value: out = a y + b y_partner, weights folded in if w; DIR -1: the opposite angle.
-  // turn: cosines of the token's pairs, sines kRopeMaxD / 2 behind.
-  template <int DIR>
-  __device__ __forceinline__ void coefficients(const fb_rope_params& p, const void* w, const float* turn, float (&a)[8], float (&b)[8]) const {
-    float wt[8];
-    weights(w, p.weight_dtype, wt);
-    if (PAIR == 0) {
-      const float4 c4 = turns ? *reinterpret_cast<const float4*>(turn + c0) : make_float4(1.f, 1.f, 1.f, 1.f);
-      const float4 s4 = turns ? *reinterpret_cast<const float4*>(turn + kRopeMaxD / 2 + c0) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = wt[i] * c[i];
-        a[i + 4] = wt[i + 4] * c[i];
-        b[i] = -DIR * (wt[i + 4] * s[i]);
-        b[i + 4] = DIR * (wt[i] * s[i]);
-      }
-      return;
-    }
-    const int half = p.rot >> 1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = c0 + i;
-      a[i] = wt[i];
-      b[i] = 0.f;
-      if (c < p.rot) {
-        const bool lo = PAIR == 1 ? !(i & 1) : c < half;
-        const float* t = turn + (PAIR == 1 ? c >> 1 : lo ? c : c - half);
-        const float q = PAIR == 1 ? wt[i ^ 1] : w ? load_scalar(w, p.weight_dtype, lo ? c + half : c - half) : 1.f;
-        a[i] = wt[i] * t[0];
-        b[i] = (lo ? -DIR : DIR) * (q * t[kRopeMaxD / 2]);
-      }
-    }
-  }
-  // The partners of the values v of a row, times r: in the lane, or (PAIR 2) from the row's words in the warp's shared memory.
-  __device__ __forceinline__ void partners(const fb_rope_params& p, const uint4& raw, const float (&v)[8], float r, uint4* stage,
-                                           float (&vp)[8]) const {
-    if (PAIR < 2) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vp[i] = v[PAIR == 0 ? i ^ 4 : i ^ 1];
-      return;
-    }
-    const int lane = threadIdx.x & 31, half = p.rot >> 1;
-    stage[lane] = raw;
-    __syncwarp();
-    uint32_t e[4] = {};
-    if (turns && !(half & 1)) {  // both columns of a word have their partners in one word
-      const uint32_t* row = reinterpret_cast<const uint32_t*>(stage + lane - lane % G);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = c0 + 2 * i;
-        if (c < p.rot) e[i] = row[(c < half ? c + half : c - half) >> 1];
-      }
-    } else if (turns) {
-      const uint16_t* row = reinterpret_cast<const uint16_t*>(stage + lane - lane % G);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = c0 + i;
-        if (c < p.rot) e[i >> 1] |= (uint32_t)row[c < half ? c + half : c - half] << (16 * (i & 1));
-      }
-    }
-    __syncwarp();
-    unpack_chunk<T>(make_uint4(e[0], e[1], e[2], e[3]), vp);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) vp[i] *= r;
-  }
-};
-
-// Cosines and sines of one token's pairs, by the warp, into its shared memory.
-__device__ __forceinline__ void rope_turns(const fb_rope_params& p, int b, int s, float* turn) {
-  __syncwarp();
-  for (int pr = threadIdx.x & 31; pr < p.rot >> 1; pr += 32) {
-    const float2 t = rope_turn(p, b, s, pr);
-    turn[pr] = t.x;
-    turn[kRopeMaxD / 2 + pr] = t.y;
-  }
-  __syncwarp();
-}
-
-template <typename T, int G, int PAIR, bool FULL, bool APPEND>
-__global__ void __launch_bounds__(kRopeVThreads, 6) rope_vector_kernel(const __grid_constant__ RopeV a) {
-  constexpr int SIDE = 32 / G, U = 4;
-  __shared__ __align__(16) float turns[kRopeVWarps][kRopeMaxD];
-  __shared__ uint4 stages[kRopeVWarps][PAIR == 2 ? 32 : 1];
-  const fb_rope_params& p = a.p;
-  const RopeLane<T, G, PAIR, FULL> me(p);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t gw = (int64_t)blockIdx.x * kRopeVWarps + warp;
-  const int tok = (int)(gw / a.split), sub = (int)(gw - (int64_t)tok * a.split);
-  if (tok >= a.tokens) return;
-  const int b = a.s_div.quot32(tok), s = tok - b * p.S;
-  int64_t page = 0;
-  int place = 0;
-  const bool cached = APPEND && cache_place(p, s, page, place);
-  rope_turns(p, b, s, turns[warp]);
-  const float inv_d = 1.f / p.D;
-
-  // TENSOR 0: q, 1: k, 2: v (copied)
-  auto rows_of = [&](auto tensor) {
-    constexpr int X = decltype(tensor)::value;
-    const int H = X == 0 ? p.Hq : p.Hk;
-    const int h0 = sub * SIDE + lane / G, step = a.split * SIDE;
-    if (sub * SIDE >= H) return;
-    const int64_t* xs = X == 0 ? p.q_stride : X == 1 ? p.k_stride : p.v_stride;
-    const T* x = reinterpret_cast<const T*>(X == 0 ? p.q : X == 1 ? p.k : p.v) + b * xs[0] + s * xs[2] + h0 * xs[1];
-    const int64_t* os = X == 0 ? p.q_out_stride : p.k_out_stride;
-    T* y = reinterpret_cast<T*>(X == 0 ? p.q_out : p.k_out) + b * os[0] + s * os[2];
-    int64_t yh = os[1];
-    if (APPEND && X > 0) {
-      const int64_t* cs = X == 1 ? p.key_cache_stride : p.value_cache_stride;
-      y = reinterpret_cast<T*>(X == 1 ? p.key_cache : p.value_cache) + page * cs[0] + place * cs[1];
-      yh = cs[2];
-    }
-    y += h0 * yh;
-    const int64_t xstep = step * xs[1], ystep = step * yh;
-    const void* w = X == 0 ? p.q_weight : X == 1 ? p.k_weight : nullptr;
-    const bool touched = FULL || w || me.turns;  // (untouched values keep their bits)
-    float ca[8], cb[8];
-    const T* const x0 = x - (lane / G) * xs[1];  // (the warp's first row exists)
-    auto load = [&](uint4& raw, const T* src, bool live) {
-      raw = me.load(live ? src : x0);
-      if ((!FULL && !me.in) || !live) raw = make_uint4(0u, 0u, 0u, 0u);
-    };
-    auto finish = [&](const uint4& raw, T* dst, bool live) {
-      uint4 out = raw;
-      if (X < 2) {
-        float v[8], vp[8], rr = 1.f;
-        unpack_chunk<T>(raw, v);
-        if (w) {
-          float q = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) q = fmaf(v[i], v[i], q);
-          rr = rsqrtf(fmaf(group_sum<G>(q), inv_d, p.eps));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= rr;
-        }
-        if (FULL || p.rot) me.partners(p, raw, v, rr, stages[warp], vp);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= ca[i];
-        if (me.turns) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = fmaf(vp[i], cb[i], v[i]);
-        }
-        if (touched) out = pack_chunk<T>(v);
-      }
-      if (live && me.in) me.store(dst, out);
-    };
-    int h = sub * SIDE;  // (of the warp's first row; the same in all lanes)
-    uint4 raw[U];
-    auto load_rows = [&](auto count) {
-#pragma unroll
-      for (int u = 0; u < decltype(count)::value; ++u) load(raw[u], x + u * xstep, true);
-    };
-    auto finish_rows = [&](auto count) {
-      constexpr int N = decltype(count)::value;
-      x += N * xstep;
-#pragma unroll
-      for (int u = 0; u < N; ++u) finish(raw[u], y + u * ystep, true);
-      y += N * ystep;
-      h += N * step;
-    };
-    const std::integral_constant<int, U> many;
-    const std::integral_constant<int, U / 2> some;
-    const bool whole = h + (U - 1) * step + SIDE <= H;
-    if (whole) load_rows(many);
-    if (X < 2) me.template coefficients<1>(p, w, turns[warp], ca, cb);  // under the first loads
-    if (whole) {
-      finish_rows(many);
-      while (h + (U - 1) * step + SIDE <= H) {
-        load_rows(many);
-        finish_rows(many);
-      }
-    }
-    if (h + (U / 2 - 1) * step + SIDE <= H) {
-      load_rows(some);
-      finish_rows(some);
-    }
-#pragma unroll 1
-    for (; h < H; h += step, x += xstep, y += ystep) {
-      const bool live = h + lane / G < H;
-      load(raw[0], x, live);
-      finish(raw[0], y, live);
-    }
-  };
-  rows_of(std::integral_constant<int, 0>());
-  if (APPEND && !cached) return;
-  rows_of(std::integral_constant<int, 1>());
-  if constexpr (APPEND) {
-    rows_of(std::integral_constant<int, 2>());
-    for (int i = sub * 32 + lane; i < p.bias_heads * p.R; i += a.split * 32) {
-      const int h = i / p.R, c = i - h * p.R;
-      reinterpret_cast<T*>(p.bias_cache)[page * p.bias_cache_stride[0] + place * p.bias_cache_stride[1] + h * p.bias_cache_stride[2] + c] =
-          reinterpret_cast<const T*>(p.k_bias)[h * p.k_bias_stride[1] + s * p.k_bias_stride[2] + c];
-    }
-  }
-}
-
-// A block takes rows of one tensor, so that a lane keeps one set of weight sums: the first a.q_ctas blocks take q.
-template <typename T, int G, int PAIR, bool FULL>
-__global__ void __launch_bounds__(kRopeVThreads, 5) rope_bwd_vector_kernel(const __grid_constant__ RopeV a) {
-  constexpr int SIDE = 32 / G, U = 2;
-  __shared__ __align__(16) float turns[kRopeVWarps][kRopeMaxD];
-  __shared__ uint4 stages[kRopeVWarps][PAIR == 2 ? 32 : 1];
-  __shared__ float sums[kRopeVWarps * SIDE][G * 8 + 1];
-  const fb_rope_params& p = a.p;
-  const RopeLane<T, G, PAIR, FULL> me(p);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool is_q = (int)blockIdx.x < a.q_ctas;
-  const int block = is_q ? blockIdx.x : blockIdx.x - a.q_ctas, blocks = is_q ? a.q_ctas : gridDim.x - a.q_ctas;
-  const int H = is_q ? p.Hq : p.Hk;
-  const int64_t *xs = is_q ? p.q_stride : p.k_stride, *gs = is_q ? p.dq_out_stride : p.dk_out_stride, *ds = is_q ? p.dq_stride : p.dk_stride;
-  const T* x0 = reinterpret_cast<const T*>(is_q ? p.q : p.k);
-  const T* g0 = reinterpret_cast<const T*>(is_q ? p.dq_out : p.dk_out);
-  T* d0 = reinterpret_cast<T*>(is_q ? p.dq : p.dk);
-  const void* w = is_q ? p.q_weight : p.k_weight;
-  const bool touched = FULL || w || me.turns;
-  float dw[8] = {}, wt[8];
-  me.weights(w, p.weight_dtype, wt);
-  const float inv_d = 1.f / p.D;
-  const int64_t nwarps = (int64_t)a.tokens * a.split;
-  for (int64_t gw = (int64_t)block * kRopeVWarps + warp; gw < nwarps; gw += (int64_t)blocks * kRopeVWarps) {
-    const int tok = (int)(gw / a.split), sub = (int)(gw - (int64_t)tok * a.split);
-    const int h0 = sub * SIDE + lane / G, step = a.split * SIDE;
-    if (sub * SIDE >= H) continue;
-    const int b = a.s_div.quot32(tok), s = tok - b * p.S;
-    const T* x = x0 + b * xs[0] + s * xs[2] + h0 * xs[1];
-    const T* g = g0 + b * gs[0] + s * gs[2] + h0 * gs[1];
-    T* d = d0 + b * ds[0] + s * ds[2] + h0 * ds[1];
-    const int64_t xstep = step * xs[1], gstep = step * gs[1], dstep = step * ds[1];
-    float ca[8], cb[8];
-    uint4 xr[U], gr[U];
-    const T *const gfirst = g - (lane / G) * gs[1], *const xfirst = x - (lane / G) * xs[1];  // (the warp's first row exists)
-    auto load = [&](int u, const T* gsrc, const T* xsrc, bool live) {
-      gr[u] = me.load(live ? gsrc : gfirst);
-      if (w) xr[u] = me.load(live ? xsrc : xfirst);
-      if ((!FULL && !me.in) || !live) xr[u] = gr[u] = make_uint4(0u, 0u, 0u, 0u);
-    };
-    auto finish = [&](int u, T* dst, bool live) {
-      uint4 out = gr[u];
-      float v[8], vp[8];
-      unpack_chunk<T>(gr[u], v);
-      if (FULL || p.rot) me.partners(p, gr[u], v, 1.f, stages[warp], vp);
-      if (me.turns) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf(vp[i], cb[i], v[i] * ca[i]);
-      }
-      if (w) {
-        float x8[8], q = 0.f, t = 0.f;
-        unpack_chunk<T>(xr[u], x8);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          q = fmaf(x8[i], x8[i], q);
-          t = fmaf(v[i] * wt[i], x8[i], t);
-        }
-        const float rr = rsqrtf(fmaf(group_sum<G>(q), inv_d, p.eps)), k = -rr * (rr * (group_sum<G>(t) * inv_d));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float xn = x8[i] * rr;
-          dw[i] = fmaf(v[i], xn, dw[i]);
-          v[i] = fmaf(xn, k, v[i] * (wt[i] * rr));
-        }
-      }
-      if (touched) out = pack_chunk<T>(v);
-      if (live && me.in) me.store(dst, out);
-    };
-    int h = sub * SIDE;  // (of the warp's first row; the same in all lanes)
-    if (h + (U - 1) * step + SIDE <= H) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) load(u, g + u * gstep, x + u * xstep, true);
-    }
-    rope_turns(p, b, s, turns[warp]);  // under the first loads
-    me.template coefficients<-1>(p, nullptr, turns[warp], ca, cb);
-    for (bool first = true; h + (U - 1) * step + SIDE <= H; h += U * step, first = false) {
-      if (!first) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) load(u, g + u * gstep, x + u * xstep, true);
-      }
-      g += U * gstep;
-      x += U * xstep;
-#pragma unroll
-      for (int u = 0; u < U; ++u) finish(u, d + u * dstep, true);
-      d += U * dstep;
-    }
-#pragma unroll 1
-    for (; h < H; h += step, g += gstep, x += xstep, d += dstep) {
-      const bool live = h + lane / G < H;
-      load(0, g, x, live);
-      finish(0, d, live);
-    }
-  }
-  if (!p.workspace) return;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (me.in) sums[warp * SIDE + lane / G][i < 4 ? me.c0 + i : me.c1 + i - 4] = dw[i];
-  __syncthreads();
-  for (int c = threadIdx.x; c < p.D; c += kRopeVThreads) {
-    float v = 0.f;
-#pragma unroll 4
-    for (int r = 0; r < kRopeVWarps * SIDE; ++r) v += sums[r][c];
-    reinterpret_cast<float*>(p.workspace)[(int64_t)blockIdx.x * p.D + c] = v;
-  }
-}
-
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
@@ -660,7 +221,7 @@ int sm_count() {
 // Warps of a token: few tokens are spread over more warps, up to two rows for a lane.  A share has its own angles and
 // coefficients to take, five rows' worth, so no more shares than make two full GPUs.
 int rope_split(const fb_rope_params* p) {
-  const int G = p->D <= 8 ? 1 : p->D <= 16 ? 2 : p->D <= 32 ? 4 : p->D <= 64 ? 8 : 16, H = p->Hq > p->Hk ? p->Hq : p->Hk;
+  const int G = rope_lanes(p->D), H = p->Hq > p->Hk ? p->Hq : p->Hk;
   const int64_t tokens = (int64_t)p->B * p->S, want = 48ll * sm_count();
   int split = 1;
   while (split * 2 * (32 / G) <= H && tokens * split < want) split *= 2;
@@ -676,7 +237,7 @@ BwdGrid rope_bwd_grid(const fb_rope_params* p, bool vector) {
     const int64_t most = 8ll * sm_count();
     return {0, (int)(tokens < most ? tokens : most)};
   }
-  const int64_t most = 5ll * sm_count(), each = (tokens * rope_split(p) + kRopeVWarps - 1) / kRopeVWarps;
+  const int64_t most = (int64_t)rope_bwd_ctas(rope_run(*p)) * sm_count(), each = (tokens * rope_split(p) + kRopeVWarps - 1) / kRopeVWarps;
   int64_t q = most * p->Hq / (p->Hq + p->Hk), k;
   q = !p->Hq ? 0 : q < 1 ? 1 : !p->Hk ? most : q > most - 1 ? most - 1 : q;
   k = p->Hk ? most - q : 0;
@@ -686,7 +247,6 @@ BwdGrid rope_bwd_grid(const fb_rope_params* p, bool vector) {
 }
 bool wants_weights(const fb_rope_params* p) { return p->dq_weight || p->dk_weight; }
 
-enum { ROPE_FORWARD, ROPE_BACKWARD, ROPE_APPEND };
 // Rows of whole aligned chunks of 16 bytes in everything that the call touches.
 bool rope_vector(const fb_rope_params* p, int what) {
   if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 8) return false;
@@ -713,30 +273,6 @@ bool rope_vector(const fb_rope_params* p, int what) {
   return !(bits & 15);
 }
 
-template <typename T, int G, int PAIR, bool FULL>
-void launch_rope_v(const RopeV& a, int what, unsigned grid, cudaStream_t st) {
-  if (what == ROPE_FORWARD) rope_vector_kernel<T, G, PAIR, FULL, false><<<grid, kRopeVThreads, 0, st>>>(a);
-  else if (what == ROPE_APPEND) rope_vector_kernel<T, G, PAIR, FULL, true><<<grid, kRopeVThreads, 0, st>>>(a);
-  else rope_bwd_vector_kernel<T, G, PAIR, FULL><<<grid, kRopeVThreads, 0, st>>>(a);
-}
-template <typename T, int G>
-void launch_rope_g(const RopeV& a, int what, unsigned grid, cudaStream_t st) {
-  if constexpr (G >= 8) {
-    if (a.p.D == 8 * G && a.p.rot == a.p.D)
-      return a.p.interleaved ? launch_rope_v<T, G, 1, true>(a, what, grid, st) : launch_rope_v<T, G, 0, true>(a, what, grid, st);
-  }
-  if (a.p.interleaved) launch_rope_v<T, G, 1, false>(a, what, grid, st);
-  else if (a.p.rot % 8 == 0) launch_rope_v<T, G, 0, false>(a, what, grid, st);
-  else launch_rope_v<T, G, 2, false>(a, what, grid, st);
-}
-template <typename T>
-void launch_rope_t(const RopeV& a, int what, unsigned grid, cudaStream_t st) {
-  if (a.p.D <= 8) launch_rope_g<T, 1>(a, what, grid, st);
-  else if (a.p.D <= 16) launch_rope_g<T, 2>(a, what, grid, st);
-  else if (a.p.D <= 32) launch_rope_g<T, 4>(a, what, grid, st);
-  else if (a.p.D <= 64) launch_rope_g<T, 8>(a, what, grid, st);
-  else launch_rope_g<T, 16>(a, what, grid, st);
-}
 void launch_rope_vector(const fb_rope_params& p, int what, cudaStream_t st) {
   RopeV a = {};
   a.p = p;

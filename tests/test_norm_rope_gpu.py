@@ -41,6 +41,14 @@ CASES = [
     (1, 23, 2, 2, 72, 48, 4, False, torch.bfloat16, torch.float16),
     (1, 15, 2, 1, 128, 64, 1, True, torch.bfloat16, None),
     (1, 300, 40, 8, 128, 128, 1, False, torch.bfloat16, torch.float32),
+    (1, 31, 7, 4, 40, 40, 1, False, torch.float16, torch.float32),     # 5, 6, 9, 10 lanes a row: lanes of the warp that have none
+    (1, 31, 16, 5, 48, 24, 1, False, torch.bfloat16, torch.float32),
+    (2, 11, 25, 8, 72, 36, 2, False, torch.float16, torch.float16),    # runs of two columns
+    (1, 21, 10, 10, 80, 80, 1, True, torch.bfloat16, torch.float32),
+    (1, 90, 13, 2, 80, 20, 1, False, torch.bfloat16, torch.bfloat16),
+    (1, 13, 4, 3, 88, 22, 1, False, torch.float16, torch.float32),     # of one
+    (1, 13, 9, 1, 40, 10, 1, False, torch.bfloat16, None),
+    (1, 13, 5, 5, 24, 18, 1, True, torch.float16, torch.float16),      # the rotated columns end inside a lane's
 ]
 
 
@@ -120,6 +128,23 @@ def test_zero_rows_and_non_finite_values():
     assert out[0, 2].isnan().all()
     want = orc.norm_rope(x[:, 3:], w)
     assert_within("x", out[:, 3:], want, rounded(want, torch.bfloat16, want.abs().amax()))
+
+
+@pytest.mark.parametrize("D", [40, 64, 72, 80, 128, 20])
+@pytest.mark.parametrize("rot", [2, 4, 10, 12, 16, 20])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_columns_behind_the_rotated_ones_keep_their_bits_and_touch_nothing(D, rot, interleaved):
+    g = torch.Generator().manual_seed(D + rot)
+    x = torch.randn(1, 6, 11, D, generator=g).half()
+    x.view(torch.int16)[..., rot:] = torch.randint(-2 ** 15, 2 ** 15, x[..., rot:].shape, generator=g).short()  # any bits, NaN and inf too
+    pos, f = torch.arange(6).cuda(), torch.rand(rot // 2, generator=g).cuda()
+    xd = x.cuda().requires_grad_(True)
+    out, _ = norm_rope_func(xd, None, pos, f, interleaved=interleaved)
+    dx, = torch.autograd.grad(out, xd, x.cuda())
+    for y in (out, dx):
+        assert torch.equal(y.cpu()[..., rot:].view(torch.int16), x[..., rot:].view(torch.int16))
+        assert y[..., :rot].isfinite().all()
+    assert (out[..., :rot].float().norm(dim=-1).cpu() - x[..., :rot].float().norm(dim=-1)).abs().max() < 1e-2  # (20 roundings of 4 at most)
 
 
 def test_partial_gradients_and_expanded_ones():
