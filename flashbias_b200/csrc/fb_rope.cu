@@ -218,39 +218,14 @@ int sm_count() {
   return n > 0 ? n : 148;
 }
 
-// Warps of a token: few tokens are spread over more warps, up to two rows for a lane.  A share has its own angles and
-// coefficients to take, five rows' worth, so no more shares than make two full GPUs.
-int rope_split(const fb_rope_params* p) {
-  const int G = rope_lanes(p->D), H = p->Hq > p->Hk ? p->Hq : p->Hk;
-  const int64_t tokens = (int64_t)p->B * p->S, want = 48ll * sm_count();
-  int split = 1;
-  while (split * 2 * (32 / G) <= H && tokens * split < want) split *= 2;
-  return split;
-}
-// Blocks of the backward; vector kernels: those of q, then those of k, each by its share of the rows.
-struct BwdGrid {
-  int q, all;
-};
-BwdGrid rope_bwd_grid(const fb_rope_params* p, bool vector) {
-  const int64_t tokens = (int64_t)p->B * p->S;
-  if (!vector) {
-    const int64_t most = 8ll * sm_count();
-    return {0, (int)(tokens < most ? tokens : most)};
-  }
-  const int64_t most = (int64_t)rope_bwd_ctas(rope_run(*p)) * sm_count(), each = (tokens * rope_split(p) + kRopeVWarps - 1) / kRopeVWarps;
-  int64_t q = most * p->Hq / (p->Hq + p->Hk), k;
-  q = !p->Hq ? 0 : q < 1 ? 1 : !p->Hk ? most : q > most - 1 ? most - 1 : q;
-  k = p->Hk ? most - q : 0;
-  if (q > each) q = each;
-  if (k > each) k = each;
-  return {(int)q, (int)(q + k)};
-}
-bool wants_weights(const fb_rope_params* p) { return p->dq_weight || p->dk_weight; }
-
-// Rows of whole aligned chunks of 16 bytes in everything that the call touches.
-bool rope_vector(const fb_rope_params* p, int what) {
-  if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 8) return false;
-  uintptr_t bits = reinterpret_cast<uintptr_t>(p->q_weight) | reinterpret_cast<uintptr_t>(p->k_weight);
+// The columns that a lane of the vector kernels reads at once (W of RopeLane): as long as the alignment of everything that the
+// call touches and half of the rotated columns allow.  -1: the general kernel (odd D; neighbours that no word holds).  4001 tokens,
+// 160 heads, weights, us forward / backward: D 20 by ones 47 / 71, by words with checks of each 39 / 52 (which cost D 80 with 20
+// columns rotated 4 / 6 of 33 / 36, so W 2 has none); neighbours by words 39 / 49; D 19 by the general kernel 176 / 244.
+int rope_run(const fb_rope_params* p, int what) {
+  if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 2) return -1;
+  const uintptr_t w = reinterpret_cast<uintptr_t>(p->q_weight) | reinterpret_cast<uintptr_t>(p->k_weight);
+  uintptr_t bits = 0;
   auto add = [&](const void* ptr, const int64_t (&s)[3], bool used) {
     if (!used) return;
     bits |= reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(s[0] | s[1] | s[2]) * 2;
@@ -270,16 +245,49 @@ bool rope_vector(const fb_rope_params* p, int what) {
     add(p->dq, p->dq_stride, p->Hq);
     add(p->dk, p->dk_stride, p->Hk);
   }
-  return !(bits & 15);
+  const bool chunks = p->D % 8 == 0 && !((bits | w) & 15);
+  const bool words = !(bits & 3) && !(w & (p->weight_dtype == FB_DTYPE_F32 ? 7 : 3));
+  if (p->interleaved) return chunks ? 8 : words ? 0 : -1;
+  return chunks && p->rot % 8 == 0 ? 4 : words && p->D % 8 == 0 && p->rot % 4 == 0 ? 2 : 1;
 }
 
-void launch_rope_vector(const fb_rope_params& p, int what, cudaStream_t st) {
+// Warps of a token: few tokens are spread over more warps, up to two rows for a lane.  A share has its own angles and
+// coefficients to take, five rows' worth, so no more shares than make two full GPUs.
+int rope_split(const fb_rope_params* p) {
+  const int G = rope_lanes(p->D), H = p->Hq > p->Hk ? p->Hq : p->Hk;
+  const int64_t tokens = (int64_t)p->B * p->S, want = 48ll * sm_count();
+  int split = 1;
+  while (split * 2 * (32 / G) <= H && tokens * split < want) split *= 2;
+  return split;
+}
+// Blocks of the backward; vector kernels: those of q, then those of k, each by its share of the rows.
+struct BwdGrid {
+  int q, all;
+};
+BwdGrid rope_bwd_grid(const fb_rope_params* p, int run) {
+  const int64_t tokens = (int64_t)p->B * p->S;
+  if (run < 0) {
+    const int64_t most = 8ll * sm_count();
+    return {0, (int)(tokens < most ? tokens : most)};
+  }
+  const int64_t most = (int64_t)rope_bwd_ctas(run) * sm_count(), each = (tokens * rope_split(p) + kRopeVWarps - 1) / kRopeVWarps;
+  int64_t q = most * p->Hq / (p->Hq + p->Hk), k;
+  q = !p->Hq ? 0 : q < 1 ? 1 : !p->Hk ? most : q > most - 1 ? most - 1 : q;
+  k = p->Hk ? most - q : 0;
+  if (q > each) q = each;
+  if (k > each) k = each;
+  return {(int)q, (int)(q + k)};
+}
+bool wants_weights(const fb_rope_params* p) { return p->dq_weight || p->dk_weight; }
+
+void launch_rope_vector(const fb_rope_params& p, int what, int run, cudaStream_t st) {
   RopeV a = {};
   a.p = p;
   a.s_div = Div(p.S);
   a.tokens = p.B * p.S;
   a.split = rope_split(&p);
-  const BwdGrid bwd = rope_bwd_grid(&p, true);
+  a.run = run;
+  const BwdGrid bwd = rope_bwd_grid(&p, run);
   a.q_ctas = bwd.q;
   const unsigned grid = what == ROPE_BACKWARD ? (unsigned)bwd.all : (unsigned)(((int64_t)a.tokens * a.split + kRopeVWarps - 1) / kRopeVWarps);
   if (p.dtype == FB_DTYPE_F16) launch_rope_t<__half>(a, what, grid, st);
@@ -299,8 +307,8 @@ extern "C" int fb_norm_rope(const fb_rope_params* p, void* cuda_stream) {
   if ((p->Hq && !p->q_out) || (p->Hk && !p->k_out)) return FB_EINVAL_NULL;
   if (negative(p->q_out_stride) || negative(p->k_out_stride)) return FB_EINVAL_STRIDE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
-  if (rope_vector(p, ROPE_FORWARD)) {
-    launch_rope_vector(*p, ROPE_FORWARD, st);
+  if (const int run = rope_run(p, ROPE_FORWARD); run >= 0) {
+    launch_rope_vector(*p, ROPE_FORWARD, run, st);
     return (int)cudaGetLastError();
   }
   const unsigned grid = (unsigned)(p->B * p->S);
@@ -312,7 +320,7 @@ extern "C" int fb_norm_rope(const fb_rope_params* p, void* cuda_stream) {
 
 extern "C" size_t fb_norm_rope_bwd_workspace_bytes(const fb_rope_params* p) {
   if (validate_rope(p) || !wants_weights(p)) return 0;
-  return round256((size_t)rope_bwd_grid(p, rope_vector(p, ROPE_BACKWARD)).all * 2 * p->D * 4);
+  return round256((size_t)rope_bwd_grid(p, rope_run(p, ROPE_BACKWARD)).all * 2 * p->D * 4);
 }
 
 extern "C" int fb_norm_rope_bwd(const fb_rope_params* p, void* cuda_stream) {
@@ -325,19 +333,19 @@ extern "C" int fb_norm_rope_bwd(const fb_rope_params* p, void* cuda_stream) {
   if (need && (!p->workspace || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255))) return FB_EINVAL_WORKSPACE;
   if (!need) a.workspace = nullptr;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
-  const bool vector = rope_vector(p, ROPE_BACKWARD);
-  const BwdGrid grid = rope_bwd_grid(p, vector);
+  const int run = rope_run(p, ROPE_BACKWARD);
+  const BwdGrid grid = rope_bwd_grid(p, run);
   const int ctas = grid.all;
   const int64_t tokens = (int64_t)p->B * p->S;
-  if (vector) {
-    launch_rope_vector(a, ROPE_BACKWARD, st);
+  if (run >= 0) {
+    launch_rope_vector(a, ROPE_BACKWARD, run, st);
   } else {
     if (p->dtype == FB_DTYPE_F16) rope_bwd_general_kernel<__half><<<ctas, kRopeThreads, 0, st>>>(a, tokens);
     else rope_bwd_general_kernel<__nv_bfloat16><<<ctas, kRopeThreads, 0, st>>>(a, tokens);
     note_launch();
   }
   if (need) {
-    const WeightParts parts = vector ? WeightParts{{grid.q, ctas - grid.q}, (int64_t)grid.q * p->D, p->D} : WeightParts{{ctas, ctas}, p->D, 2 * p->D};
+    const WeightParts parts = run >= 0 ? WeightParts{{grid.q, ctas - grid.q}, (int64_t)grid.q * p->D, p->D} : WeightParts{{ctas, ctas}, p->D, 2 * p->D};
     rope_weight_kernel<<<dim3((p->D + 31) / 32, 2), dim3(32, 32), 0, st>>>(a, parts);
     note_launch();
   }
@@ -360,8 +368,8 @@ extern "C" int fb_paged_append(const fb_rope_params* p, void* cuda_stream) {
     return FB_EINVAL_BIAS;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
-  if (rope_vector(p, ROPE_APPEND)) {
-    launch_rope_vector(*p, ROPE_APPEND, st);
+  if (const int run = rope_run(p, ROPE_APPEND); run >= 0) {
+    launch_rope_vector(*p, ROPE_APPEND, run, st);
     return (int)cudaGetLastError();
   }
   if (p->dtype == FB_DTYPE_F16) rope_general_kernel<__half, true><<<p->S, kRopeThreads, 0, st>>>(*p);

@@ -55,6 +55,7 @@ struct RopeV {
   Div s_div;
   int tokens;  // B S
   int split;   // warps of a token
+  int run;     // W of RopeLane
   int q_ctas;  // backward: blocks that take rows of q, the others rows of k
 };
 
@@ -66,8 +67,6 @@ inline int rope_lanes(int D) {
     if (n <= g) return g;
   return 16;
 }
-// Columns that a lane reads in one go.
-inline int rope_run(const fb_rope_params& p) { return p.interleaved ? 8 : p.rot % 8 == 0 ? 4 : p.rot % 4 == 0 ? 2 : 1; }
 // Blocks of the backward per SM: short runs take more registers.
 constexpr int rope_bwd_ctas(int run) { return run <= 2 ? 4 : 5; }
 template <typename T>

@@ -1,4 +1,4 @@
-// Rotary passes over rows of whole aligned 16-byte chunks (instantiated in fb_rope_f16.cu and fb_rope_bf16.cu).
+// Rotary passes, a few lanes to a row (instantiated in fb_rope_f16.cu and fb_rope_bf16.cu).
 #pragma once
 
 #include <type_traits>
@@ -13,12 +13,12 @@ namespace fb {
 // the partner times sine) is folded into two coefficients per column that serve all heads of the token, the address is one
 // addition per row, and four rows (backward: two) are in flight per lane.
 // A lane holds both halves of its pairs: where they are half of the rotated columns apart it reads pairs of runs, where they
-// are neighbours eight columns in a row.  G is what a row has of chunks where that makes room for one more row.
+// are neighbours eight columns in a row (by twos, where rows are no whole aligned chunks of 16 bytes).  G is what a row has of chunks where that makes room for one more row.
 // B4 S4096 H32-8 D128 bf16, fp32 weights, us forward / backward: 64 (5.2 TB/s) / 117 (4.3 TB/s); with the other half by shuffle
 // 72 / 143, with coefficients from shared memory for every row and rows found by division 329 together.  Arithmetic on packed
 // pairs of fp32 issued as many instructions and was no faster; asking for the next token's rows ahead (L2) changed nothing.
-// 4001 tokens, H25-25 D80 fp16 with weights (64 MB each way, from a cold L2): 31.6 / 43.9, with 16 lanes a row 36.9 / 62.5;
-// without weights and 20 columns rotated 33.8 / 37.9, with 16 lanes and the other half through shared memory 41.0 / 59.4.
+// 4001 tokens, H25-25 D80 fp16 with weights (64 MB each way, from a cold L2): 30.7 / 43.9, with 16 lanes a row 36.9 / 62.5;
+// without weights and 20 columns rotated 32.8 / 35.9, with 16 lanes and the other half through shared memory 41.0 / 59.4.
 
 template <typename T>
 __device__ __forceinline__ void unpack_chunk(const uint4& raw, float (&x)[8]) {
@@ -73,41 +73,50 @@ __device__ __forceinline__ void load_floats(const float* p, float* out) {
   }
 }
 
-// What a lane holds of every row: eight columns, in runs of W, from col[] on.  W 4, 2, 1 (the largest that divides half of the
-// rotated columns): runs 2j and 2j + 1 are the two halves of W pairs, or neighbours behind the rotated columns.  W 8 (pairs are
-// neighbours): eight columns in a row.
+// What a lane holds of every row: up to eight columns, in runs of W, from col[] on.  W 4, 2, 1: runs 2j and 2j + 1 are the two
+// halves of W pairs, or neighbours behind the rotated columns.  W 8, 0 (pairs are neighbours): eight columns in a row, read at
+// once or (0) by twos.
 // FULL: the lanes' columns are those of the row, and all of them are rotated.
 template <typename T, int G, int W, bool FULL>
 struct RopeLane {
-  static constexpr int RUNS = 8 / W, SIDE = 32 / G;
+  static constexpr bool NEAR = W == 8 || W == 0, PARTIAL = W < 2;  // PARTIAL: rows may end inside a lane's columns
+  static constexpr int RUNS = NEAR ? 1 : 8 / W, SIDE = 32 / G;
   int col[RUNS];
-  int row;          // of the SIDE rows that a warp holds side by side
-  bool in;          // the columns exist
-  bool turns;       // some of them are rotated
+  int row;     // of the SIDE rows that a warp holds side by side
+  int have;    // values, two of a word together; 8 or 0 where not PARTIAL
+  bool in;     // any
+  bool turns;  // some of them are rotated
   __device__ __forceinline__ RopeLane(const fb_rope_params& p) {
     const int lane = threadIdx.x & 31, part = lane % G, half = p.rot >> 1;
     const bool mine = SIDE * G == 32 || lane < SIDE * G;
     row = mine ? lane / G : 0;
-    in = FULL || (mine && part * 8 < p.D);
-    if constexpr (W == 8) {
+    // (whole pairs of runs come first: where a row ends inside the last lane's columns that lane lacks its last ones)
+    have = FULL ? 8 : !mine ? 0 : max(0, min(8, p.D - part * 8));
+    in = FULL || have > 0;
+    if constexpr (NEAR) {
       col[0] = in ? part * 8 : 0;  // (a lane without columns reads what exists and drops it)
       turns = FULL || (in && col[0] < p.rot);
     } else {
 #pragma unroll
       for (int j = 0; j < RUNS / 2; ++j) {
         const int u = (part * (RUNS / 2) + j) * W;
-        col[2 * j] = !in ? 0 : FULL || u < half ? u : 2 * u;
-        col[2 * j + 1] = !in ? 0 : u < half || FULL ? u + (FULL ? 4 * G : half) : 2 * u + W;
+        const bool exists = FULL || (PARTIAL ? 2 * W * j < have : in);
+        col[2 * j] = !exists ? 0 : FULL || u < half ? u : 2 * u;
+        col[2 * j + 1] = !exists ? 0 : u < half || FULL ? u + (FULL ? 4 * G : half) : 2 * u + W;
       }
       turns = FULL || (in && part * 4 < half);
     }
   }
+  __device__ __forceinline__ int column(int i) const {
+    if constexpr (NEAR) return col[0] + i;
+    else return col[i / W] + i % W;
+  }
   // whether value i of the lane is rotated
   __device__ __forceinline__ bool turned(const fb_rope_params& p, int i) const {
-    if (FULL) return true;
-    if (W == 8) return turns && col[0] + i < p.rot;
-    if (W == 4) return turns;
-    return turns && col[i / (2 * W) * 2] < p.rot >> 1;
+    if constexpr (FULL) return true;
+    else if constexpr (NEAR) return turns && col[0] + i < p.rot;
+    else if constexpr (W == 4) return turns;
+    else return turns && (!PARTIAL || i < have) && col[i / (2 * W) * 2] < p.rot >> 1;
   }
   __device__ __forceinline__ uint4 load(const T* src) const {
     if constexpr (W == 8) {
@@ -115,12 +124,12 @@ struct RopeLane {
     } else if constexpr (W == 4) {
       const uint2 a = __ldcs(reinterpret_cast<const uint2*>(src + col[0])), b = __ldcs(reinterpret_cast<const uint2*>(src + col[1]));
       return make_uint4(a.x, a.y, b.x, b.y);
-    } else if constexpr (W == 2) {
-      auto word = [&](int j) { return __ldcs(reinterpret_cast<const uint32_t*>(src + col[j])); };
+    } else if constexpr (W == 1) {
+      auto one = [&](int j) { return (uint32_t)__ldcs(reinterpret_cast<const uint16_t*>(src + col[j])); };
+      auto word = [&](int j) { return 2 * j < have ? one(2 * j) | one(2 * j + 1) << 16 : 0u; };
       return make_uint4(word(0), word(1), word(2), word(3));
     } else {
-      auto half = [&](int j) { return (uint32_t)__ldcs(reinterpret_cast<const uint16_t*>(src + col[j])); };
-      auto word = [&](int j) { return half(2 * j) | half(2 * j + 1) << 16; };
+      auto word = [&](int j) { return !PARTIAL || 2 * j < have ? __ldcs(reinterpret_cast<const uint32_t*>(src + column(2 * j))) : 0u; };
       return make_uint4(word(0), word(1), word(2), word(3));
     }
   }
@@ -131,12 +140,17 @@ struct RopeLane {
     } else if constexpr (W == 4) {
       *reinterpret_cast<uint2*>(dst + col[0]) = make_uint2(v.x, v.y);
       *reinterpret_cast<uint2*>(dst + col[1]) = make_uint2(v.z, v.w);
-    } else if constexpr (W == 2) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(dst + col[j]) = w[j];
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) *reinterpret_cast<uint16_t*>(dst + col[j]) = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+      for (int j = 0; j < 4; ++j) {
+        if (PARTIAL && 2 * j >= have) continue;
+        if constexpr (W == 1) {
+          *reinterpret_cast<uint16_t*>(dst + col[2 * j]) = (uint16_t)w[j];
+          *reinterpret_cast<uint16_t*>(dst + col[2 * j + 1]) = (uint16_t)(w[j] >> 16);
+        } else {
+          *reinterpret_cast<uint32_t*>(dst + column(2 * j)) = w[j];
+        }
+      }
     }
   }
   // the weights of the columns (1 without weights)
@@ -145,9 +159,10 @@ struct RopeLane {
     for (int i = 0; i < 8; ++i) out[i] = 1.f;
     if (!w || !in) return;
     if (dtype == FB_DTYPE_F32) {
-      constexpr int N = W < 4 ? W : 4;
+      constexpr int N = W == 0 ? 2 : W < 4 ? W : 4;
 #pragma unroll
-      for (int i = 0; i < 8; i += N) load_floats<N>(reinterpret_cast<const float*>(w) + col[i / W] + i % W, out + i);
+      for (int i = 0; i < 8; i += N)
+        if (!PARTIAL || i < have) load_floats<N>(reinterpret_cast<const float*>(w) + column(i), out + i);
       return;
     }
     const uint4 raw = load(reinterpret_cast<const T*>(w));  // (both 16-bit types have the size of T)
@@ -166,17 +181,17 @@ struct RopeLane {
       b[i] = 0.f;
     }
     // N pairs at a time: the first of value i, its second value STEP on
-    constexpr int N = W == 8 ? 4 : W, STEP = W == 8 ? 1 : W;
+    constexpr int N = W == 8 ? 4 : W == 0 ? 1 : W, STEP = NEAR ? 1 : W;
 #pragma unroll
     for (int i = 0; i < 8; i += 2 * N) {
       float c[N], s[N];
       if (!turned(p, i)) continue;
-      const int pr = W == 8 ? col[0] >> 1 : col[i / W];
+      const int pr = NEAR ? column(i) >> 1 : column(i);
       load_floats<N>(turn + pr, c);
       load_floats<N>(turn + kRopeMaxD / 2 + pr, s);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const int lo = W == 8 ? 2 * e : i + e, hi = lo + STEP;
+        const int lo = i + (NEAR ? 2 * e : e), hi = lo + STEP;
         if (W == 8 && !turned(p, lo)) continue;
         a[lo] = wt[lo] * c[e];
         a[hi] = wt[hi] * c[e];
@@ -187,7 +202,7 @@ struct RopeLane {
   }
   // The rotation of a row by those coefficients; values that are not rotated are left with their own factor alone.
   __device__ __forceinline__ void rotate(const fb_rope_params& p, float (&v)[8], const float (&a)[8], const float (&b)[8]) const {
-    constexpr int OTHER = W == 8 ? 1 : W;
+    constexpr int OTHER = NEAR ? 1 : W;
     float o[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = v[i] * a[i];
@@ -423,7 +438,7 @@ __global__ void __launch_bounds__(kRopeVThreads, rope_bwd_ctas(W)) rope_bwd_vect
   if (!p.workspace) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (me.in) sums[warp * SIDE + me.row][me.col[i / W] + i % W] = dw[i];
+    if (i < me.have) sums[warp * SIDE + me.row][me.column(i)] = dw[i];
   __syncthreads();
   for (int c = threadIdx.x; c < p.D; c += kRopeVThreads) {
     float v = 0.f;
@@ -443,11 +458,12 @@ void launch_rope_v(const RopeV& a, int what, unsigned grid, cudaStream_t st) {
 template <typename T, int G>
 void launch_rope_g(const RopeV& a, int what, unsigned grid, cudaStream_t st) {
   if constexpr (G == 8 || G == 16) {
-    if (a.p.D == 8 * G && a.p.rot == a.p.D)
-      return a.p.interleaved ? launch_rope_v<T, G, 8, true>(a, what, grid, st) : launch_rope_v<T, G, 4, true>(a, what, grid, st);
+    if (a.run >= 4 && a.p.D == 8 * G && a.p.rot == a.p.D)
+      return a.run == 8 ? launch_rope_v<T, G, 8, true>(a, what, grid, st) : launch_rope_v<T, G, 4, true>(a, what, grid, st);
   }
-  switch (rope_run(a.p)) {
+  switch (a.run) {
     case 8: return launch_rope_v<T, G, 8, false>(a, what, grid, st);
+    case 0: return launch_rope_v<T, G, 0, false>(a, what, grid, st);
     case 4: return launch_rope_v<T, G, 4, false>(a, what, grid, st);
     case 2: return launch_rope_v<T, G, 2, false>(a, what, grid, st);
     default: return launch_rope_v<T, G, 1, false>(a, what, grid, st);

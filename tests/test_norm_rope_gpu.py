@@ -49,6 +49,12 @@ CASES = [
     (1, 13, 4, 3, 88, 22, 1, False, torch.float16, torch.float32),     # of one
     (1, 13, 9, 1, 40, 10, 1, False, torch.bfloat16, None),
     (1, 13, 5, 5, 24, 18, 1, True, torch.float16, torch.float16),      # the rotated columns end inside a lane's
+    (1, 37, 7, 3, 36, 36, 1, False, torch.bfloat16, torch.float32),    # rows end inside a lane's columns
+    (2, 9, 12, 4, 44, 20, 2, True, torch.float16, torch.float16),
+    (1, 9, 5, 2, 100, 100, 1, False, torch.float16, torch.float32),
+    (1, 9, 5, 2, 126, 126, 1, True, torch.bfloat16, torch.float32),
+    (2, 33, 7, 3, 20, 10, 1, False, torch.bfloat16, torch.bfloat16),
+    (1, 9, 33, 3, 6, 6, 1, False, torch.float16, torch.float16),
 ]
 
 
@@ -130,7 +136,7 @@ def test_zero_rows_and_non_finite_values():
     assert_within("x", out[:, 3:], want, rounded(want, torch.bfloat16, want.abs().amax()))
 
 
-@pytest.mark.parametrize("D", [40, 64, 72, 80, 128, 20])
+@pytest.mark.parametrize("D", [40, 64, 72, 80, 128, 20, 44, 102, 27])
 @pytest.mark.parametrize("rot", [2, 4, 10, 12, 16, 20])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_columns_behind_the_rotated_ones_keep_their_bits_and_touch_nothing(D, rot, interleaved):
