@@ -346,7 +346,16 @@ extern "C" int fb_norm_rope_bwd(const fb_rope_params* p, void* cuda_stream) {
   }
   if (need) {
     const WeightParts parts = run >= 0 ? WeightParts{{grid.q, ctas - grid.q}, (int64_t)grid.q * p->D, p->D} : WeightParts{{ctas, ctas}, p->D, 2 * p->D};
-    rope_weight_kernel<<<dim3((p->D + 31) / 32, 2), dim3(32, 32), 0, st>>>(a, parts);
+    cudaLaunchConfig_t cfg = {};  // (under the end of the first kernel)
+    cfg.gridDim = dim3((p->D + 31) / 32, 2);
+    cfg.blockDim = dim3(32, 32);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (const cudaError_t e = cudaLaunchKernelEx(&cfg, rope_weight_kernel, a, parts)) return (int)e;
     note_launch();
   }
   return (int)cudaGetLastError();

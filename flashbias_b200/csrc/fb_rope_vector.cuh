@@ -14,7 +14,7 @@ namespace fb {
 // addition per row, and four rows (backward: two) are in flight per lane.
 // A lane holds both halves of its pairs: where they are half of the rotated columns apart it reads pairs of runs, where they
 // are neighbours eight columns in a row (by twos, where rows are no whole aligned chunks of 16 bytes).  G is what a row has of chunks where that makes room for one more row.
-// B4 S4096 H32-8 D128 bf16, fp32 weights, us forward / backward: 64 (5.2 TB/s) / 117 (4.3 TB/s); with the other half by shuffle
+// B4 S4096 H32-8 D128 bf16, fp32 weights, us forward / backward: 64 (5.2 TB/s) / 114 (4.4 TB/s); with the other half by shuffle
 // 72 / 143, with coefficients from shared memory for every row and rows found by division 329 together.  Arithmetic on packed
 // pairs of fp32 issued as many instructions and was no faster; asking for the next token's rows ahead (L2) changed nothing.
 // 4001 tokens, H25-25 D80 fp16 with weights (64 MB each way, from a cold L2): 30.7 / 43.9, with 16 lanes a row 36.9 / 62.5;
