@@ -28,6 +28,7 @@ struct RopeArgs {
 // The parameter block without tensors q and k.  rows of (B, S): the tokens.
 void fill_rope(fb_rope_params& p, const RopeArgs& a, const Tensor& like, int64_t B, int64_t S, int64_t D) {
   FB_ASSERT(D >= 1 && D <= 128, "norm_rope supports head dimensions up to 128");
+  FB_ASSERT(B <= 0x7fff0000 && S <= 0x7fff0000 && (S == 0 || B <= 0x7fff0000 / S), "too many tokens");
   p.B = (int32_t)B;
   p.S = (int32_t)S;
   p.D = (int32_t)D;
@@ -85,6 +86,7 @@ void fill_rope(fb_rope_params& p, const RopeArgs& a, const Tensor& like, int64_t
   p.k_weight = a.k_weight.defined() ? a.k_weight.data_ptr() : nullptr;
 }
 
+constexpr int64_t kMaxRopeHeads = 65536;
 void check_rope_qk(const Tensor& q, const Tensor& k) {
   FB_ASSERT(q.dim() == 4 && (!k.defined() || k.dim() == 4), "q and k are (batch, seqlen, nheads, headdim)");
   check_16bit_cuda(q);
@@ -93,6 +95,7 @@ void check_rope_qk(const Tensor& q, const Tensor& k) {
     FB_ASSERT(k.scalar_type() == q.scalar_type(), "All tensors must have the same type");
     FB_ASSERT(k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3), "q and k differ in more than their heads");
   }
+  FB_ASSERT(q.size(2) <= kMaxRopeHeads && (!k.defined() || q.size(2) + k.size(2) <= kMaxRopeHeads), "too many heads");
 }
 
 // (q_out, k_out); k may be undefined
@@ -187,6 +190,7 @@ struct NormRopeNode : torch::autograd::Function<NormRopeNode> {
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const bool again = at::GradMode::is_enabled();  // (create_graph)
     at::NoGradGuard no_grad;
     const auto s = ctx->get_saved_variables();
     const RopeArgs a = {s[2], s[3], s[4], s[5],
@@ -198,6 +202,13 @@ struct NormRopeNode : torch::autograd::Function<NormRopeNode> {
     const bool want_kw = s[5].defined() && ctx->needs_input_grad(w0 + (s[4].defined() ? 1 : 0));
     auto [dq, dk, dqw, dkw] =
         rope_backward(grads[0], grads.size() > 1 ? grads[1] : Tensor(), s[0], s[1], a, want_qw, want_kw);
+    if (again) {  // there is no second derivative: to ask for it is an error, not a zero
+      // (with the edges of this node, so that a search for the inputs passes it)
+      auto edges = torch::autograd::get_current_node()->next_edges();
+      const auto stop = std::make_shared<torch::autograd::Error>("norm_rope_func cannot be differentiated twice", std::move(edges));
+      for (Tensor* t : {&dq, &dk, &dqw, &dkw})
+        if (t->defined()) torch::autograd::create_gradient_edge(*t, stop);
+    }
     return {dq, dk, Tensor(), Tensor(), dqw, dkw, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -240,6 +251,16 @@ void check_written(const Tensor& c) {
 void cache_strides(const Tensor& c, int64_t (&out)[3]) {
   for (int i = 0; i < 3; ++i) out[i] = c.stride(i);
 }
+// the same beside what is read: rows that lie in a cache may be those that another token overwrites
+void check_apart(const Tensor& cache, const Tensor& read) {
+  if (!read.defined() || !cache.is_alias_of(read)) return;
+  auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return reinterpret_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  FB_ASSERT(read.numel() == 0 || end(read) <= cache.data_ptr() || end(cache) <= read.data_ptr(), "what is appended may not lie in a cache itself: copy it first");
+}
 // a tensor that a kernel has written behind autograd's back
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -264,6 +285,7 @@ OptTensor paged_append(const OptTensor& q_, const Tensor& k_, const Tensor& v_, 
     FB_ASSERT(q_->scalar_type() == k_.scalar_type(), "All tensors must have the same type");
     FB_ASSERT(q_->size(0) == N && q_->size(2) == D, "q and k differ in more than their heads");
   }
+  FB_ASSERT(Hk <= kMaxRopeHeads && (!q_ || q_->size(1) + Hk <= kMaxRopeHeads), "too many heads");
   FB_ASSERT(key_cache.dim() == 4 && key_cache.size(0) > 0 && key_cache.size(1) > 0 && key_cache.size(1) <= 0x7fffffff,
             "caches are (pages, page size, heads, columns)");
   const int64_t pages = key_cache.size(0), page_size = key_cache.size(1);
@@ -275,6 +297,10 @@ OptTensor paged_append(const OptTensor& q_, const Tensor& k_, const Tensor& v_, 
   FB_ASSERT(slots.dim() == 1 && slots.size(0) == N && is_index(slots), "slots holds one int32 or int64 per token");
   FB_ASSERT(k_bias_.has_value() == bias_cache.has_value(), "k_bias and bias_cache must be given together");
   const Tensor k = unit_rows(k_), v = unit_rows(v_), q = unit_rows_or_undefined(q_), kb = unit_rows_or_undefined(k_bias_);
+  for (const Tensor* c : {&key_cache, &value_cache})
+    for (const Tensor* t : {&q, &k, &v, &kb}) check_apart(*c, *t);
+  if (bias_cache)
+    for (const Tensor* t : {&q, &k, &v, &kb}) check_apart(*bias_cache, *t);
   c10::cuda::CUDAGuard guard(k.device());
   const RopeArgs a = {or_undefined(positions), contiguous_or_undefined(inv_freq), contiguous_or_undefined(q_weight),
                       contiguous_or_undefined(k_weight), axes, interleaved, eps};
@@ -404,6 +430,7 @@ std::tuple<Tensor, OptTensor> paged_forward(const Tensor& q_, const Tensor& key_
   check_16bit_cuda(q_);
   const int64_t N = q_.size(0), Hq = q_.size(1), D = q_.size(2);
   FB_ASSERT(D >= 1 && D <= 128, "FlashAttention only support head dimensions up to 128");
+  FB_ASSERT(N <= 0x7fff0000 && Hq <= 65536, "too many tokens or heads");
   FB_ASSERT(key_cache.dim() == 4 && key_cache.size(0) > 0 && key_cache.size(1) > 0 && key_cache.size(2) > 0,
             "caches are (pages, page size, heads, columns)");
   const int64_t pages = key_cache.size(0), page_size = key_cache.size(1), Hk = key_cache.size(2);

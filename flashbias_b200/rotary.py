@@ -34,5 +34,6 @@ def norm_rope_func(q: torch.Tensor, k: Optional[torch.Tensor], positions: Option
     interleaved: pair p is columns (2p, 2p + 1) instead of (p, p + len(inv_freq)).
 
     Gradients for q, k and the weights (fp32 sums over all rows, in a fixed order); inv_freq and positions are constants.
+    They cannot be differentiated again.
     """
     return _op().norm_rope(q, k, positions, inv_freq, q_weight, k_weight, axes, interleaved, eps)

@@ -173,6 +173,18 @@ def test_partial_gradients_and_expanded_ones():
     assert torch.equal(dqw2, dqw)
 
 
+def test_a_second_derivative_is_refused():
+    q, k, w, pos, f, _ = inputs(1, 9, 2, 1, 64, 64, 1, torch.bfloat16, torch.float32, 4)
+    qd, wd = q.cuda().requires_grad_(True), w[0].cuda().requires_grad_(True)
+    out, _ = norm_rope_func(qd, None, pos.cuda(), f.cuda(), wd)
+    dq, dw = torch.autograd.grad(out, [qd, wd], torch.ones_like(out), create_graph=True)
+    for g in (dq, dw):
+        with pytest.raises(RuntimeError, match="twice"):
+            torch.autograd.grad(g.sum(), qd, retain_graph=True)
+    plain = torch.autograd.grad(norm_rope_func(qd, None, pos.cuda(), f.cuda(), wd)[0], [qd, wd], torch.ones_like(out))
+    assert torch.equal(dq, plain[0]) and torch.equal(dw, plain[1])
+
+
 def test_weight_gradients_repeat_bit_for_bit():
     q, k, w, pos, f, _ = inputs(1, 700, 8, 2, 128, 128, 1, torch.bfloat16, torch.float32, 6)
     leaves = [t.cuda().requires_grad_(True) for t in (q, k, *w)]

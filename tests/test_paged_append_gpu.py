@@ -146,3 +146,20 @@ def test_refusals(bad):
     paged_append(**dev)
     with pytest.raises(AssertionError):
         paged_append(**{**dev, **{n: v.cuda() if n != "value_cache" or v.stride(2) else v[:, :, :1].cuda().expand(v.shape) for n, v in bad.items()}})
+
+
+def test_rows_that_lie_in_a_cache_are_refused():
+    """Moving accepted tokens up: from a copy, because a slot may be another token's source; one arena for everything is fine."""
+    arena = torch.randn(2 * 4 * 8 * 2 * 16 + 4 * 2 * 16, generator=torch.Generator().manual_seed(5)).half().cuda()
+    kc, vc = arena[:1024].view(4, 8, 2, 16), arena[1024:2048].view(4, 8, 2, 16)
+    fresh = arena[2048:].view(4, 2, 16)
+    slots = torch.tensor([3, 4, 5, 6], device="cuda")
+    k, v = kc.view(32, 2, 16)[4:8], vc.view(32, 2, 16)[4:8]
+    for bad in ((k, fresh), (fresh, v), (fresh, k), (v, fresh)):
+        with pytest.raises(AssertionError):
+            paged_append(None, *bad, kc, vc, slots)
+    paged_append(None, fresh, fresh, kc, vc, slots)
+    assert torch.equal(kc.view(32, 2, 16)[3:7], fresh) and torch.equal(vc.view(32, 2, 16)[3:7], fresh)
+    want = kc.view(32, 2, 16)[4:8].clone(), vc.view(32, 2, 16)[4:8].clone()
+    paged_append(None, *want, kc, vc, slots)
+    assert torch.equal(kc.view(32, 2, 16)[3:7], want[0]) and torch.equal(vc.view(32, 2, 16)[3:7], want[1])
