@@ -166,10 +166,12 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
     plan.TD = p->D <= 32 ? 32 : p->D <= 64 ? 64 : 128;
     plan.MT = rows <= 16 ? 16 : 32;
     plan.ctas = split_ctas(plan.TD, plan.MT) * sms;
-    // The heads of a group are read side by side, whole rows of the cache; where the longest requests that the table can hold do
-    // not fill the GPU that way, one head is spread over the CTA's warps.
-    const int64_t tiles = (int64_t)p->B * (((int64_t)p->table_width * p->page_size + 63) / 64) * p->Hk;
-    plan.WH = p->Hk % 4 == 0 && tiles / 4 >= 4 * plan.ctas ? 4 : p->Hk % 2 == 0 && tiles / 2 >= 4 * plan.ctas ? 2 : 1;
+    // Key heads of an item, each a warp's (or, with fewer than four, several warps').  Four share the walk and the table and read
+    // the cache in the longest runs, and leave the fewest items; few items are cut in more parts, each with a beginning, an end and
+    // a place in the join.  us for 4 / 2 / 1 heads, D128 H32-8 but for the second: B256 L300..500 67.8 / 68.6 / 89.6, of 32 columns
+    // 19.6 / 23.3 / 32.1; B64 L1000 39.8 / 38.2 / 43.0, B16 L3000 43.3 / 35.3 / 35.3, B8 L4000 26.4 / 21.4 / 19.3.
+    const int64_t each = (int64_t)p->B * ((rows + plan.MT - 1) / plan.MT) * p->Hk;
+    plan.WH = p->Hk % 4 == 0 && each >= 4 * plan.ctas ? 4 : p->Hk % 2 == 0 && 2 * each > plan.ctas ? 2 : 1;
   }
   // items: row tiles (of every request at least one) times head groups
   const int64_t items = (int64_t)p->B * ((rows + plan.MT - 1) / plan.MT) * (p->Hk / plan.WH);
