@@ -150,10 +150,11 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
   const int sms = device_sm_count(dev) > 0 ? device_sm_count(dev) : 148;
   // Many rows: 128 of them in a tcgen05 tile, if a tile of 128 keys is made of whole pages (or a page of whole tiles) that TMA can
   // address, and the scale may be taken out of a maximum.  Wide rows sooner, because the other kernel's work grows with the columns
-  // and with every 32 rows, this one's hardly.  Tile / split kernel, us: 128 columns, 33 rows (B26 T11 H16-4, 747 keys) 27.3 / 29.2,
-  // 36 rows (B16 T24 H16-8, 8000 keys) 76.6 / 115; 64 columns, 45 rows (T30) over 1000 keys 25.1 / 21.0, over 8000 61.8 / 66.8, 68
-  // rows 25.4 / 24.0 and 62.0 / 76.8; 32 columns, 68 rows 24.9 / 18.7 and 59.9 / 57.2, 90 rows 24.9 / 22.5 and 61.2 / 73.8.
-  const int few = p->D <= 32 ? 80 : p->D <= 64 ? 48 : 32;
+  // and with every 32 rows, this one's hardly.  Tile / split kernel, us (rows on average, half as many more in the largest trees):
+  // 128 columns, 18 rows (B16 T12 H16-8) over 100 keys 14.1 / 14.9, over 1000 28.4 / 26.7, over 8000 74.9 / 87.3; 26 rows 14.2 / 16.7,
+  // 28.5 / 31.1, 75.7 / 103; 64 columns, 45 rows (T30) over 1000 keys 25.1 / 21.0, over 8000 61.8 / 66.8, 68 rows 25.4 / 24.0 and
+  // 62.0 / 76.8; 32 columns, 68 rows 24.9 / 18.7 and 59.9 / 57.2, 90 rows 24.9 / 22.5 and 61.2 / 73.8.
+  const int few = p->D <= 32 ? 80 : p->D <= 64 ? 48 : 24;
   const bool tma = tma_compatible(p->key_cache, p->key_cache_stride[1], p->key_cache_stride[2], p->key_cache_stride[0], p->Hk, p->num_pages) &&
                    tma_compatible(p->value_cache, p->value_cache_stride[1], p->value_cache_stride[2], p->value_cache_stride[0], p->Hk, p->num_pages);
   if (rows > few && !(p->flags & FB_FLAG_PAGED_SPLIT) && tma && p->R == 0 && p->softmax_scale > 1e-20f && p->page_size % 8 == 0 && (128 % p->page_size == 0 || p->page_size % 128 == 0) &&

@@ -1,4 +1,4 @@
-// Attention over pages with few rows per key head (32 to 80 by their width): decoding, and small trees or runs of drafted tokens.
+// Attention over pages with few rows per key head (24 to 80 by their width): decoding, and small trees or runs of drafted tokens.
 //
 // Bound by reading K and V once.  A warp works alone: it owns a head of the CTA's group and every WK-th tile of 16 or 32 keys, copies
 // them into a ring of its own in shared memory (cp.async, so that what is in flight is bounded by shared memory and not by

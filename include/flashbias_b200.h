@@ -321,7 +321,7 @@ typedef struct fb_paged_params {
 /* The kernel that fb_paged_fwd takes (FB_PAGED_*), or <0 on invalid arguments.  Fill in every pointer and stride of the call. */
 #define FB_PAGED_GENERAL 0 /* CUDA cores: head_dim not a multiple of 8, rows that are not whole aligned 16-byte chunks */
 #define FB_PAGED_SPLIT 1   /* mma.sync, up to 32 rows (tokens times heads per key head) of a request side by side */
-#define FB_PAGED_TILE 2    /* tcgen05 tiles of 128 rows: more than 32 rows per request on average, no factors, a positive scale,
+#define FB_PAGED_TILE 2    /* tcgen05 tiles of 128 rows: more than 24 rows per request on average (48, 80 at D up to 64, 32), no factors, a positive scale,
                               page_size a multiple of 8 that divides 128 or a multiple of 128 */
 int fb_paged_kernel(const fb_paged_params *p);
 

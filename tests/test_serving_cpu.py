@@ -168,7 +168,7 @@ def test_oracle_gradients_against_differences(norm, interleaved):
 
 @pytest.mark.parametrize("change,kernel", [
     (dict(), "split"), (dict(N=48), "split"), (dict(N=49), "tile"), (dict(N=96, Hq=2), "split"), (dict(N=97, Hq=2), "tile"), (dict(N=80, D=32), "split"),
-    (dict(N=81, D=32), "tile"), (dict(N=32, D=128), "split"),
+    (dict(N=81, D=32), "tile"), (dict(N=24, D=128), "split"), (dict(N=25, D=128), "tile"),
     (dict(N=50, page_size=8), "tile"), (dict(N=50, page_size=24), "split"), (dict(N=50, page_size=4), "split"), (dict(N=50, page_size=256), "tile"),
     (dict(N=50, softmax_scale=-1.0), "split"), (dict(N=50, flags=_lib.FB_FLAG_PAGED_SPLIT), "split"), (dict(D=20), "general"),
     (dict(N=34, D=128, o_stride=_lib.I64x2(512, 128)), "tile"), (dict(key_cache=0x1008), "general"), (dict(key_cache_stride=_lib.I64x3(4096, 64, 257)), "general"),
