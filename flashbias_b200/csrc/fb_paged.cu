@@ -64,15 +64,14 @@ __global__ void __launch_bounds__(128) paged_general_kernel(const __grid_constan
                       (p.bias_heads > 1 ? hk * p.bias_cache_stride[2] : 0);
         for (int c = 0; c < p.R; ++c) s = fmaf(qbs[c], to_f32(kb[c]), s);
       }
-      s *= kLog2eP;
     }
     float mx = s;
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mx = fmaxf(m, mx);
-    const float msub = fmaxf(mx, -FLT_MAX), alpha = fast_exp2(m - msub);
+    const float msub = fmaxf(mx, -FLT_MAX), alpha = fast_exp2((m - msub) * kLog2eP);
     m = mx;
-    const float e = seen ? fast_exp2(s - msub) : 0.f;
+    const float e = seen ? fast_exp2((s - msub) * kLog2eP) : 0.f;
     l = l * alpha + e;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] *= alpha;
@@ -100,13 +99,13 @@ __global__ void __launch_bounds__(128) paged_general_kernel(const __grid_constan
   l = 0.f;
   float o = 0.f;
   for (int w = 0; w < 4; ++w) {
-    const float f = fast_exp2(s_m[w] - msub);
+    const float f = fast_exp2((s_m[w] - msub) * kLog2eP);
     l += s_l[w] * f;
     o += s_acc[w][threadIdx.x] * f;
   }
   if (threadIdx.x < p.D)
     reinterpret_cast<T*>(p.o)[n * p.o_stride[0] + h * p.o_stride[1] + threadIdx.x] = from_f32<T>(l > 0.f ? o / l : l == 0.f ? 0.f : l);
-  if (p.lse && threadIdx.x == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
+  if (p.lse && threadIdx.x == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? fmaf(fast_log2(l), kLn2P, m) : l == 0.f ? -INFINITY : l;
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -33,9 +33,9 @@ struct PagedArgs {
   uint32_t pages32;         // num_pages, within 31 bits: what a page of the table is compared with
   int factor_words;         // split kernel: factor rows can be read two columns at a time
   int factor_bytes;         // split kernel: pieces in which a key's factors are copied; 0: not
-  float scale_log2;
+  float scale_log2;         // tile kernel
   float* part;    // (CTAs, 2, heads of a group, rows of a tile, columns): sums of items that span CTAs
-  float2* ml;     // the same without columns: maximum (log2 units) and sum
+  float2* ml;     // the same without columns: maximum (split kernel: of the logits, tile kernel: in log2 units) and sum
   int4* desc;     // (CTAs, 2): the item that begins in a CTA and ends in another: row tile, head group, last CTA, -; first token,
                   // rows of the request; a row tile of -1: none
 };
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i0 + u >= parts) break;
-        const float f = fast_exp2(s[u].x - ms);
+        const float f = fast_exp2((s[u].x - ms) * kLog2eP);
         l = fmaf(s[u].y, f, l);
         acc = make_float4(fmaf(v[u].x, f, acc.x), fmaf(v[u].y, f, acc.y), fmaf(v[u].z, f, acc.z), fmaf(v[u].w, f, acc.w));
       }
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     l = 0.f;
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int g = 0; g < SHARE; ++g) {
-      const float f = fast_exp2(s_ml[g].x - ms);
+      const float f = fast_exp2((s_ml[g].x - ms) * kLog2eP);
       const float4 v = s_acc[g * LANES + lane];
       l = fmaf(s_ml[g].y, f, l);
       acc = make_float4(fmaf(v.x, f, acc.x), fmaf(v.y, f, acc.y), fmaf(v.z, f, acc.z), fmaf(v.w, f, acc.w));
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   if (lane * 4 < p.D)  // D is a multiple of 8
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1] + lane * 4) =
         l == 0.f ? make_uint2(0u, 0u) : make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
-  if (p.lse && lane == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
+  if (p.lse && lane == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? fmaf(fast_log2(l), kLn2P, m) : l == 0.f ? -INFINITY : l;
 }
 
 // launch_pdl (fb_internal.h) with a grid of two dimensions and no dynamic shared memory

@@ -108,7 +108,7 @@ __device__ __forceinline__ void join_cluster(const PagedArgs& a, const Segment& 
       const float* from = cluster.map_shared_rank(part, c);
       const float2 s = reinterpret_cast<const float2*>(from + MT * TD)[r];
       const float4 v = *reinterpret_cast<const float4*>(from + r * TD + col);
-      const float f = fast_exp2(s.x - ms);
+      const float f = fast_exp2((s.x - ms) * kLog2eP);
       sum = fmaf(s.y, f, sum);
       acc = make_float4(fmaf(v.x, f, acc.x), fmaf(v.y, f, acc.y), fmaf(v.z, f, acc.z), fmaf(v.w, f, acc.w));
     }
@@ -117,7 +117,7 @@ __device__ __forceinline__ void join_cluster(const PagedArgs& a, const Segment& 
     if (col < p.D)
       *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1] + col) =
           sum == 0.f ? make_uint2(0u, 0u) : make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
-    if (p.lse && col == 0) p.lse[(int64_t)n * p.Hq + h] = sum > 0.f ? (mx + fast_log2(sum)) * kLn2P : sum == 0.f ? -INFINITY : sum;
+    if (p.lse && col == 0) p.lse[(int64_t)n * p.Hq + h] = sum > 0.f ? fmaf(fast_log2(sum), kLn2P, mx) : sum == 0.f ? -INFINITY : sum;
   }
   cluster.sync();  // the parts have been read
 }
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
     // ---- query rows, as fragments of the products' first operand
     uint32_t q[NM][KS][4], qb[NM][4] = {};
     int row_tok[NM][2];               // token of the request, -1 for rows of padding
-    float slope2[NM][2] = {}, m[NM][2], l[NM][2];
+    float slope[NM][2] = {}, m[NM][2], l[NM][2];
     int my_pos[NM][2] = {};
     const T* qbrow[NM][2] = {};
 #pragma unroll
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
           for (int x = 0; x < 2; ++x)
             q[im][ks][e + 2 * x] = live && ks * 16 + x * 8 < p.D ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + x * 8 + qc) : 0u;
         if (BIAS == PAGED_SLOPES && live) {
-          slope2[im][e] = p.slopes[h] * kLog2eP;
+          slope[im][e] = p.slopes[h];
           my_pos[im][e] = p.positions ? p.positions[n] : rq.len + t;
         }
         if (BIAS >= PAGED_FACTORS) {
@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
         factor_pages(tile + 2 * WK);
       }
 
-      // ---- logits in log2 units; masks where the tile holds new tokens' keys or keys that do not exist
+      // ---- logits; masks where the tile holds new tokens' keys or keys that do not exist.  In their own units: in those of log2
+      // what lies below -2.36e38 (a mask of the type's lowest value among the factors) would be -inf, a key that is not seen
       const int j0 = tile * KT + qc;
       const bool masked = okm != ALL || tile * KT + KT > rq.len;
 #pragma unroll
@@ -416,9 +417,9 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
         for (int nt = 0; nt < 2 * NK; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v = s[im][nt][i] * a.scale_log2;
-            if (BIAS == PAGED_SLOPES) v = fmaf(slope2[im][i >> 1], (float)(j0 + nt * 8 + (i & 1) - my_pos[im][i >> 1]), v);
-            if (BIAS >= PAGED_FACTORS) v = fmaf(f[im][nt][i], kLog2eP, v);
+            float v = s[im][nt][i] * p.softmax_scale;
+            if (BIAS == PAGED_SLOPES) v = fmaf(slope[im][i >> 1], (float)(j0 + nt * 8 + (i & 1) - my_pos[im][i >> 1]), v);
+            if (BIAS >= PAGED_FACTORS) v += f[im][nt][i];
             s[im][nt][i] = v;
           }
       if (masked) {
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
               for (int x = 0; x < 2; ++x) {
                 const int i = 2 * e + x, k = nt * 8 + qc + x, j = tile * KT + k;
                 if (BIAS == PAGED_SLOPES && p.positions && j >= rq.len && j < rq.keys)  // the key's position instead of its place
-                  s[im][nt][i] = fmaf(slope2[im][e], (float)(p.positions[rq.first + j - rq.len] - j), s[im][nt][i]);
+                  s[im][nt][i] = fmaf(slope[im][e], (float)(p.positions[rq.first + j - rq.len] - j), s[im][nt][i]);
                 if (!(bits >> k & 1)) s[im][nt][i] = -INFINITY;
               }
           }
@@ -456,12 +457,12 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           grown |= mx > m[im][e];
           const float msub = fmaxf(mx, -FLT_MAX);  // no visible key yet: every exponential is zero
-          alpha[im][e] = fast_exp2(m[im][e] - msub);
+          alpha[im][e] = fast_exp2((m[im][e] - msub) * kLog2eP);
           m[im][e] = mx;
           float sum = 0.f;
 #pragma unroll
           for (int nt = 0; nt < 2 * NK; ++nt) {
-            const float p0 = fast_exp2(s[im][nt][2 * e] - msub), p1 = fast_exp2(s[im][nt][2 * e + 1] - msub);
+            const float p0 = fast_exp2((s[im][nt][2 * e] - msub) * kLog2eP), p1 = fast_exp2((s[im][nt][2 * e + 1] - msub) * kLog2eP);
             sum += p0 + p1;
             // the probabilities are rounded to the 16 bits of V: half a step of relative error each, what the result is rounded by
             pf[im][nt >> 1][2 * (nt & 1) + e] = Pack2<T>::pack(p0, p1);
@@ -579,8 +580,8 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
             for (int e = 0; e < 2; ++e) {
               const float2 s2 = reinterpret_cast<const float2*>(from + MT * TD)[im * 16 + e * 8 + qr];
               const float mn = fmaxf(m[im][e], s2.x), ms = fmaxf(mn, -FLT_MAX);
-              fa[e] = fast_exp2(m[im][e] - ms);
-              fb[e] = fast_exp2(s2.x - ms);
+              fa[e] = fast_exp2((m[im][e] - ms) * kLog2eP);
+              fb[e] = fast_exp2((s2.x - ms) * kLog2eP);
               m[im][e] = mn;
               l[im][e] = l[im][e] * fa[e] + s2.y * fb[e];
             }
@@ -616,7 +617,7 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
               if (i * 8 < p.D)
                 *reinterpret_cast<uint32_t*>(dst + i * 8 + qc) =
                     ls == 0.f ? 0u : Pack2<T>::pack(o[im][i][2 * e] * inv, o[im][i][2 * e + 1] * inv);
-            if (p.lse && qc == 0) p.lse[(int64_t)n * p.Hq + h] = ls > 0.f ? (m[im][e] + fast_log2(ls)) * kLn2P : ls == 0.f ? -INFINITY : ls;
+            if (p.lse && qc == 0) p.lse[(int64_t)n * p.Hq + h] = ls > 0.f ? fmaf(fast_log2(ls), kLn2P, m[im][e]) : ls == 0.f ? -INFINITY : ls;
           } else {
             // slot 1: the CTA in which the item begins; 0: the others
             const int64_t row = (((int64_t)blockIdx.x * 2 + (seg.t0 == 0 ? 1 : 0)) * WH + wh) * MT + r;

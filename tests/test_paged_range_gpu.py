@@ -1,0 +1,90 @@
+"""Attention over pages at the ends of the number range, against 64 bits."""
+import pytest
+import torch
+
+from flashbias_b200 import _lib, check_device_status
+from flashbias_b200.flash_bias import _op
+from oracle import serving_oracle as orc
+from tests.serving_helpers import FP32, assert_within, half_step, paged_inputs
+
+pytestmark = pytest.mark.gpu
+
+FLAGS = {"own": 0, "split": _lib.FB_FLAG_PAGED_SPLIT, "general": _lib.FB_FLAG_FORCE_GENERAL}
+
+
+def forward(kw, kernel):
+    d = {n: v.cuda() if isinstance(v, torch.Tensor) else v for n, v in kw.items()}
+    o, lse = _op().paged_forward(*[d.get(n) for n in ("q", "key_cache", "value_cache", "block_table", "lens", "cu_tokens", "tree_mask", "positions",
+                                                      "slopes", "q_bias", "bias_cache", "softmax_scale")], True, FLAGS[kernel])
+    torch.cuda.synchronize()
+    check_device_status()
+    return o.cpu(), lse.cpu()
+
+
+def oracle(kw):
+    return orc.paged_attention(**{{"block_table": "table", "cu_tokens": "cu", "softmax_scale": "scale"}.get(n, n): v for n, v in kw.items()})
+
+
+def weights_alone(want, weight, dtype):
+    """bounds() of rows whose logits are equal or so far apart that the lower ones weigh nothing: no error of a logit counts."""
+    u = half_step(dtype)
+    return u * want.abs() + (1.01 * u + 2.0 ** -19) * weight + torch.finfo(dtype).smallest_normal * u
+
+
+def used_places(kw, b=0):
+    page = kw["key_cache"].shape[1]
+    n = int(kw["lens"][b]) + int(kw["cu_tokens"][b + 1] - kw["cu_tokens"][b])
+    return [(int(kw["block_table"][b, j // page]), j % page) for j in range(n)]
+
+
+@pytest.mark.parametrize("kernel", ["own", "general"])
+@pytest.mark.parametrize("lens,T,width", [(200, 3, 0), (900, 1, 0), (900, 2, 600), (4000, 12, 600)])
+@pytest.mark.parametrize("value", [torch.finfo(torch.bfloat16).min, -3.0e38, -2.4e38, 3.0e38])
+def test_a_bias_of_any_finite_size_in_all_keys(kernel, lens, T, width, value):
+    """A padding mask of the type's lowest value as a factor: beside it the rest of a logit vanishes, so a row whose keys all carry
+    it is the mean of its values (a step of 2.4e38 is 2e31 in 32 bits and 2.7e22 in 64; q.k is below 1e3)."""
+    kw = paged_inputs([lens], [T], 2, 2, 64, 16, torch.bfloat16, 31, R=2)
+    kw["block_table"] = torch.nn.functional.pad(kw["block_table"], (0, width), value=-1)
+    kw["bias_cache"][..., 0] = value
+    kw["q_bias"][..., 0] = 1.0
+    want, lse, weight, _ = oracle(kw)
+    assert lse.isfinite().all() and want.abs().max() > 0.01
+    o, got = forward(kw, kernel)
+    assert_within("o", o, want, weights_alone(want, weight, torch.bfloat16))
+    assert_within("lse", got, lse, 8 * FP32 * lse.abs())
+
+
+@pytest.mark.parametrize("kernel", ["own", "general"])
+def test_huge_biases_keep_their_order(kernel):
+    """Every third key carries -2.5e38, the others -3.3e38: the first kind alone counts."""
+    kw = paged_inputs([400], [3], 4, 2, 64, 16, torch.bfloat16, 32, R=1)
+    kw["bias_cache"][:] = -3.3e38
+    for j, at in enumerate(used_places(kw)):
+        if j % 3 == 0:
+            kw["bias_cache"][at] = -2.5e38
+    kw["q_bias"][:] = 1.0
+    want, lse, weight, _ = oracle(kw)
+    o, got = forward(kw, kernel)
+    assert_within("o", o, want, weights_alone(want, weight, torch.bfloat16))
+    assert_within("lse", got, lse, 8 * FP32 * lse.abs())
+
+
+@pytest.mark.parametrize("kernel", ["split", "general"])
+@pytest.mark.parametrize("exponent,scale", [(40, None), (70, 0.3), (123, 24.0)])
+@pytest.mark.parametrize("dtype,T,lens", [(torch.bfloat16, 40, 500), (torch.bfloat16, 1, 300), (torch.bfloat16, 64, 0)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_equal_logits_of_any_finite_size(kernel, exponent, scale, dtype, T, lens, sign):
+    """All keys alike: however large q.k is, the values' mean.  (Logits up to 2.5e38: 24 * 2^123.)"""
+    kw = paged_inputs([lens], [T], 4, 2, 128, 16, dtype, 33)
+    for at in used_places(kw):
+        kw["key_cache"][at] = 0.0
+        kw["key_cache"][at][..., 5] = 2.0 ** (exponent // 2)
+    kw["q"] = torch.randn(kw["q"].shape, generator=torch.Generator().manual_seed(1)).to(dtype)
+    kw["q"][..., 5] = sign * 2.0 ** (exponent - exponent // 2)
+    kw["q"][1:, 1:, 5] *= 0.7109375  # (exact in bf16) and logits that are no powers of two
+    if scale:
+        kw["softmax_scale"] = scale
+    want, lse, weight, _ = oracle(kw)
+    o, got = forward(kw, kernel)
+    assert_within("o", o, want, weights_alone(want, weight, dtype))
+    assert_within("lse", got, lse, 8 * FP32 * lse.abs())
