@@ -35,7 +35,7 @@ struct PagedArgs {
   int factor_bytes;         // split kernel: pieces in which a key's factors are copied; 0: not
   float scale_log2;         // tile kernel
   float* part;    // (CTAs, 2, heads of a group, rows of a tile, columns): sums of items that span CTAs
-  float2* ml;     // the same without columns: maximum (split kernel: of the logits, tile kernel: in log2 units) and sum
+  float2* ml;     // the same without columns: maximum (tile kernel: in quarters of log2 units) and sum
   int4* desc;     // (CTAs, 2): the item that begins in a CTA and ends in another: row tile, head group, last CTA, -; first token,
                   // rows of the request; a row tile of -1: none
 };

@@ -334,8 +334,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + Cfg::T_S + 128 * x + lane_off, tP = tmem + Cfg::T_P + 64 * x + lane_off, tO = tmem + Cfg::T_O + lane_off;
     const uint32_t m_own = sbase + Cfg::OFF_M + (x * 128 + row) * 4, m_other = sbase + Cfg::OFF_M + ((x ^ 1) * 128 + row) * 4;
-    const float sl2 = a.scale_log2;
-    const uint64_t sl2p = f2(sl2, sl2);
+    // Maxima are kept in quarters of a log2 unit, in which no finite logit overflows.
+    const float sl2 = a.scale_log2, sl2q = 0.25f * sl2;
     int c = 0, co = 0, n = 0, t0 = 0;  // key tiles of this stream and of the other, segments and key tiles so far
     uint32_t s[4][32];                 // the thread's row of the logit tile
     auto segment_both = [&](int n) {  // (the warpgroups leave together: behind an expired wait, too)
@@ -356,9 +356,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       // the row's token (of the request, -1: padding) and query head
       const int gr = sg->rt * 128 + row, tk = gr < sg->tokens * a.G ? a.group_div.quot32(gr) : -1, gn = sg->first + max(tk, 0);
       const int hd = sg->hg * a.G + (tk >= 0 ? gr - tk * a.G : 0);
-      float m_used = -INFINITY, l = 0.f;  // reference maximum (log2 units: logit * log2 e); row sum of this stream's tiles, relative to it
+      float m_used = -INFINITY, l = 0.f;  // reference maximum (logit * log2 e / 4); row sum of this stream's tiles, relative to it
       const int c0 = c, co0 = co;
-      // the bias in units of q.k, so that a logit costs one product more: s + slope_r (pos - k0), times sl2, plus abase
+      // the bias in units of q.k, so that a logit costs one product more: s + slope_r (pos - k0), times sl2, plus 4 baseq
       const float slope2 = SLOPES && tk >= 0 ? p.slopes[hd] * kLog2eP : 0.f, slope_r = slope2 / sl2;
       const int my_pos = SLOPES && tk >= 0 ? (p.positions ? p.positions[gn] : len + tk) : 0;
       for (int j = x; j < n_kv; j += 2, ++c) {
@@ -387,7 +387,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               if (!(there >> ((ch * 32 + i) / rows) & 1)) bits[ch] &= ~(1u << i);
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const float abase = SLOPES ? slope2 * (float)(k0 - my_pos) : 0.f;
+        const float baseq = SLOPES ? 0.25f * slope2 * (float)(k0 - my_pos) : 0.f;
         auto complete = [&](int ch) {
           if (dead) {
             if (SLOPES) {
@@ -437,7 +437,24 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         tc_fence_before_sync();
         mbar_arrive_warp(s_read + 8 * x);  // the tensor core may start on the stream's next tile
         complete(3);
-        const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sl2, abase);  // sl2 > 0
+        const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sl2q, baseq);  // sl2 > 0
+        // Far from zero the rounding of the maximum, a 2^-24 of it, would be a factor that P cannot hold.  There the logits are
+        // rounded as their maximum was (and beyond 2^100, where two of them are equal or nothing beside one another, left in quarters).
+        float unit = sl2;
+        const bool far = __any_sync(0xffffffffu, (fabsf(mx) >= 262144.f && mx > -INFINITY) || (SLOPES && fabsf(baseq) >= 262144.f));
+        if (far) {
+          unit = fabsf(mx) < 1.2676506e30f ? 4.f : 1.f;
+          const uint64_t q2 = f2(sl2q, sl2q), b2 = f2(baseq, baseq);
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float v0, v1;
+              f2_unpack(f2_fma(f2(__uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1])), q2, b2), v0, v1);
+              s[ch][i] = __float_as_uint(v0);
+              s[ch][i + 1] = __float_as_uint(v1);
+            }
+        }
         // ---- the reference maximum, from tile to tile: it moves only when the maximum has grown by more than 2^8 (exact: the row
         // sums carry the same reference)
         const float m_last = m_used;
@@ -445,13 +462,13 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           asm volatile("bar.sync %0, 256;" ::"r"(2 + (x ^ 1)) : "memory");
           m_used = __uint_as_float(ld_shared_flag(m_other));
           const float m_new = fmaxf(m_used, mx);
-          if (__any_sync(0xffffffffu, m_new - m_used > 8.f)) {  // (from -inf: the difference is +inf, or NaN where both are)
+          if (__any_sync(0xffffffffu, m_new - m_used > 2.f)) {  // (from -inf: the difference is +inf, or NaN where both are)
             // O is stable behind the product of tile j - 1, which is the other stream's.  (The one two before it on that barrier,
             // tile j - 5, has completed: the other stream has waited for it ahead of its P of tile j - 3.)
             const int cp = co0 + ((j - 1) >> 1);
             mbar_wait(pv_bar(x ^ 1, cp), (cp >> 1) & 1, abort_flag);
             tc_fence_after_sync();
-            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(4.f * (m_used - m_new));
             m_used = m_new;
 #pragma unroll 1
             for (int ch = 0; ch < TD / 32; ++ch) {
@@ -474,9 +491,10 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (c > 0) mbar_wait(pv_bar(x, c - 1), ((c - 1) >> 1) & 1, abort_flag);  // P has been read
         // ---- p = exp2(logit2 - m), row sum, P -> tensor memory (the A operand of O += P.V), rounded to the 16 bits of V
         const float msub = m_used == -INFINITY ? 0.f : m_used;
-        l *= fast_exp2(m_last - msub);  // (0 at the stream's first tile, where l is 0)
+        l *= fast_exp2(4.f * (m_last - msub));  // (0 at the stream's first tile, where l is 0)
         uint64_t l2a = f2(0.f, 0.f), l2b = f2(0.f, 0.f);
-        const uint64_t nm = f2(abase - msub, abase - msub);
+        const float off = far ? -unit * msub : 4.f * (baseq - msub);
+        const uint64_t nm = f2(off, off), unit2 = f2(unit, unit);
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
           uint32_t pw[16];  // 32 keys = 16 packed words
@@ -484,7 +502,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           for (int i = 0; i < 32; i += 2) {
             const uint64_t v = f2(__uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1]));
             float a0, a1;
-            f2_unpack(f2_fma(v, sl2p, nm), a0, a1);
+            f2_unpack(f2_fma(v, unit2, nm), a0, a1);
             const float p0 = fast_exp2(a0), p1 = fast_exp2(a1);
             if (i & 2) l2b = f2_add(l2b, f2(p0, p1)); else l2a = f2_add(l2a, f2(p0, p1));
             pw[i / 2] = Pack2<T>::pack(p0, p1);
@@ -514,7 +532,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       tc_fence_after_sync();
       const float2 other = ml[(x ^ 1) * 128 + row];
       const float m = fmaxf(m_used, other.x), ms = m == -INFINITY ? 0.f : m;  // the last reference is the largest
-      const float ls = l * fast_exp2(m_used - ms) + other.y * fast_exp2(other.x - ms);
+      const float ls = l * fast_exp2(4.f * (m_used - ms)) + other.y * fast_exp2(4.f * (other.x - ms));
       const bool begins = sg->t0 == 0, whole = begins && t1 == sg->tiles, taken = s_taken[n & 7] == n + 1;
       const float inv = !whole ? 1.f : ls > 0.f ? 1.f / ls : ls == 0.f ? 0.f : ls;
       const int64_t slot = (int64_t)blockIdx.x * 2 + (begins ? 1 : 0);  // slot 1: the CTA in which the item begins
@@ -560,7 +578,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       }
       if (x == 0 && tk >= 0) {
         if (!whole) a.ml[slot * 128 + row] = make_float2(m, ls);
-        else if (p.lse) p.lse[(int64_t)gn * p.Hq + hd] = ls > 0.f ? (m + fast_log2(ls)) * kLn2P : ls == 0.f ? -INFINITY : ls;
+        else if (p.lse) p.lse[(int64_t)gn * p.Hq + hd] = ls > 0.f ? fmaf(4.f * kLn2P, m, fast_log2(ls) * kLn2P) : ls == 0.f ? -INFINITY : ls;
       }
       if (!whole && begins && threadIdx.x == 0) {
         a.desc[2 * blockIdx.x] = make_int4(sg->rt, sg->hg, sg->last_cta, 0);
@@ -605,7 +623,7 @@ __global__ void __launch_bounds__(128 * SHARE) paged_join_tile_kernel(const __gr
 #pragma unroll U
     for (int i = 0; i < parts; ++i) {
       const float2 s = a.ml[slot_of(i) * 128 + row];
-      const float f = fast_exp2(s.x - ms);
+      const float f = fast_exp2(4.f * (s.x - ms));
       l = fmaf(s.y, f, l);
       const float4* src = reinterpret_cast<const float4*>(a.part) + (slot_of(i) * (TD / 4) + col0 / 4) * 128 + row;
 #pragma unroll
@@ -628,7 +646,7 @@ __global__ void __launch_bounds__(128 * SHARE) paged_join_tile_kernel(const __gr
     for (int g = 0; g < G; ++g) acc[g] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int x = 0; x < SHARE; ++x) {
       const float2 s = s_ml[x][row];
-      const float f = fast_exp2(s.x - ms);
+      const float f = fast_exp2(4.f * (s.x - ms));
       l = fmaf(s.y, f, l);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -647,7 +665,7 @@ __global__ void __launch_bounds__(128 * SHARE) paged_join_tile_kernel(const __gr
     if (col0 + g * 8 < p.D)
       *reinterpret_cast<uint4*>(dst + g * 8) = make_uint4(p2(acc[2 * g].x, acc[2 * g].y), p2(acc[2 * g].z, acc[2 * g].w), p2(acc[2 * g + 1].x, acc[2 * g + 1].y),
                                                           p2(acc[2 * g + 1].z, acc[2 * g + 1].w));
-  if (p.lse && blockIdx.y == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? (m + fast_log2(l)) * kLn2P : l == 0.f ? -INFINITY : l;
+  if (p.lse && blockIdx.y == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? fmaf(4.f * kLn2P, m, fast_log2(l) * kLn2P) : l == 0.f ? -INFINITY : l;
 }
 
 template <typename T, int TD, bool SLOPES>

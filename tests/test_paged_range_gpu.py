@@ -6,6 +6,7 @@ from flashbias_b200 import _lib, check_device_status
 from flashbias_b200.flash_bias import _op
 from oracle import serving_oracle as orc
 from tests.serving_helpers import FP32, assert_within, half_step, paged_inputs
+from tests.test_paged_attention_gpu import kernel_of
 
 pytestmark = pytest.mark.gpu
 
@@ -69,7 +70,7 @@ def test_huge_biases_keep_their_order(kernel):
     assert_within("lse", got, lse, 8 * FP32 * lse.abs())
 
 
-@pytest.mark.parametrize("kernel", ["split", "general"])
+@pytest.mark.parametrize("kernel", ["own", "split", "general"])
 @pytest.mark.parametrize("exponent,scale", [(40, None), (70, 0.3), (123, 24.0)])
 @pytest.mark.parametrize("dtype,T,lens", [(torch.bfloat16, 40, 500), (torch.bfloat16, 1, 300), (torch.bfloat16, 64, 0)])
 @pytest.mark.parametrize("sign", [1.0, -1.0])
@@ -84,7 +85,27 @@ def test_equal_logits_of_any_finite_size(kernel, exponent, scale, dtype, T, lens
     kw["q"][1:, 1:, 5] *= 0.7109375  # (exact in bf16) and logits that are no powers of two
     if scale:
         kw["softmax_scale"] = scale
+    if kernel == "own":
+        assert kernel_of(kw) == ("tile" if T > 12 else "split")
     want, lse, weight, _ = oracle(kw)
     o, got = forward(kw, kernel)
     assert_within("o", o, want, weights_alone(want, weight, dtype))
+    assert_within("lse", got, lse, 8 * FP32 * lse.abs())
+
+
+@pytest.mark.parametrize("kernel", ["own", "split"])
+@pytest.mark.parametrize("T", [30, 64])
+def test_large_logits_of_two_kinds(kernel, T):
+    """Logits near 2^50 with steps of their own between the keys: the largest of a row takes all, the earlier tiles' are forgotten."""
+    kw = paged_inputs([700], [T], 4, 2, 128, 16, torch.bfloat16, 34)
+    best = {}
+    for j, at in enumerate(used_places(kw)):
+        kw["key_cache"][at] = 0.0
+        size = (j * 37 % 101) + 128  # 8 bits: exact in bf16
+        kw["key_cache"][at][..., 3] = size * 2.0 ** 17
+        best.setdefault(size, []).append(j)
+    kw["q"][..., 3] = 2.0 ** 26
+    want, lse, weight, _ = oracle(kw)
+    o, got = forward(kw, kernel)
+    assert_within("o", o, want, weights_alone(want, weight, torch.bfloat16))
     assert_within("lse", got, lse, 8 * FP32 * lse.abs())
