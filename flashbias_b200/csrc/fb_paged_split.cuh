@@ -481,8 +481,8 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
           }
       }
 
-      // ---- O += P V.  A value that is not finite must not reach the rows that do not see its key (0 x inf): such a tile of new
-      // tokens goes through a loop over its keys.
+      // ---- O += P V.  A value that is not finite must not reach the rows that do not see its key (0 x inf), and must reach those
+      // that do, however small their P: such a tile of new tokens goes through a loop over its keys.
       bool odd = false;
       if (masked) {
         bool mine = false;
@@ -507,6 +507,13 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
             }
           }
       } else {
+        uint32_t sees[NM][2];
+#pragma unroll
+        for (int im = 0; im < NM; ++im)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sees[im][e] = row_tok[im][e] < 0 ? 0u : okm & seen_bits(p, rq.first + row_tok[im][e], row_tok[im][e], tile * KT - rq.len);
+        auto add = [](float& acc, float pk, float v) { acc = fabsf(v) <= FLT_MAX ? fmaf(pk, v, acc) : acc + v; };
 #pragma unroll 1
         for (int k = 0; k < KT; ++k) {
           const int src = (lane & ~3) | ((k & 7) >> 1), at = k >> 3;  // the fragment's lane and half
@@ -530,13 +537,13 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
             const float v0 = to_f32(v[0]), v1 = to_f32(v[1]);
 #pragma unroll
             for (int im = 0; im < NM; ++im) {
-              if (pk[im][0] != 0.f) {
-                o[im][i][0] = fmaf(pk[im][0], v0, o[im][i][0]);
-                o[im][i][1] = fmaf(pk[im][0], v1, o[im][i][1]);
+              if (sees[im][0] >> k & 1) {
+                add(o[im][i][0], pk[im][0], v0);
+                add(o[im][i][1], pk[im][0], v1);
               }
-              if (pk[im][1] != 0.f) {
-                o[im][i][2] = fmaf(pk[im][1], v0, o[im][i][2]);
-                o[im][i][3] = fmaf(pk[im][1], v1, o[im][i][3]);
+              if (sees[im][1] >> k & 1) {
+                add(o[im][i][2], pk[im][1], v0);
+                add(o[im][i][3], pk[im][1], v1);
               }
             }
           }

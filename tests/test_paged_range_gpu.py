@@ -1,11 +1,13 @@
 """Attention over pages at the ends of the number range, against 64 bits."""
+import math
+
 import pytest
 import torch
 
 from flashbias_b200 import _lib, check_device_status
 from flashbias_b200.flash_bias import _op
 from oracle import serving_oracle as orc
-from tests.serving_helpers import FP32, assert_within, half_step, paged_inputs
+from tests.serving_helpers import FP32, assert_within, half_step, paged_inputs, tree
 from tests.test_paged_attention_gpu import kernel_of
 
 pytestmark = pytest.mark.gpu
@@ -109,3 +111,30 @@ def test_large_logits_of_two_kinds(kernel, T):
     o, got = forward(kw, kernel)
     assert_within("o", o, want, weights_alone(want, weight, torch.bfloat16))
     assert_within("lse", got, lse, 8 * FP32 * lse.abs())
+
+
+@pytest.mark.parametrize("kernel", ["own", "split", "general"])
+@pytest.mark.parametrize("T,D", [(5, 64), (9, 128), (64, 128), (5, 32)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("depth", [19.0, 150.0])
+def test_a_value_that_is_not_finite_counts_however_small_its_weight(kernel, T, D, dtype, depth):
+    """A drafted key with a logit of `depth` below the others (a weight that fp16, or 32 bits, cannot hold) and a value that is not
+    finite: the rows that see it are not finite, the others as if it were not there (but for the order of their fp32 sums: the kernel
+    for few rows adds such a tile key by key.  Two orders of a sum of n terms p v differ by 2 n 2^-24 of the sum of |p v|, which is
+    |v|'s largest at most, and each result is rounded once)."""
+    kw = paged_inputs([70], [T], 4, 2, D, 16, dtype, 39)
+    g = torch.Generator().manual_seed(40)
+    kw["q"] = (1.0 + 0.05 * torch.randn(kw["q"].shape, generator=g)).to(dtype)
+    _, mask, _ = tree([T], 41)
+    kw["tree_mask"] = mask
+    at = used_places(kw)[70 + 1]
+    kw["key_cache"][at] = -depth / math.sqrt(D)
+    clean, _ = forward(kw, kernel)
+    largest = max(float(kw["value_cache"][p].abs().max()) for p in used_places(kw))
+    allowed = 2 * half_step(dtype) * clean.double().abs() + 2 * (70 + T) * FP32 * largest
+    for what in (float("inf"), float("nan"), -float("inf")):
+        kw["value_cache"][at] = what
+        o, _ = forward(kw, kernel)
+        seen = (mask[:, 0] >> 1 & 1).bool()
+        assert seen.any() and not seen.all()
+        assert ((o.double() - clean.double()).abs() <= allowed)[~seen].all() and not o[seen].isfinite().any()
