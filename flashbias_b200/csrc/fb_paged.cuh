@@ -19,6 +19,14 @@ namespace fb {
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kLn2P = 0.6931471805599453f;
 
+// P is rounded to the 16 bits of V.  fp16 ends at 2^-24, and many keys of less than that beside a large one may be all of a row's
+// result: there the probabilities, and the row's sum with them, are 2^15 times as large in the split kernel (which has them at most
+// one) and 2^7 times in the tile kernel (2^8).
+template <typename T>
+constexpr float kSplitLift = std::is_same<T, __half>::value ? 15.f : 0.f;
+template <typename T>
+constexpr float kTileLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+
 // 16 bytes to shared memory; zeros, and nothing is read, where they do not exist
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16u : 0u) : "memory");
@@ -286,7 +294,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   if (lane * 4 < p.D)  // D is a multiple of 8
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1] + lane * 4) =
         l == 0.f ? make_uint2(0u, 0u) : make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
-  if (p.lse && lane == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? fmaf(fast_log2(l), kLn2P, m) : l == 0.f ? -INFINITY : l;
+  if (p.lse && lane == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? fmaf(fast_log2(l) - kSplitLift<T>, kLn2P, m) : l == 0.f ? -INFINITY : l;
 }
 
 // launch_pdl (fb_internal.h) with a grid of two dimensions and no dynamic shared memory

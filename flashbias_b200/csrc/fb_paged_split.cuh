@@ -117,7 +117,7 @@ __device__ __forceinline__ void join_cluster(const PagedArgs& a, const Segment& 
     if (col < p.D)
       *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + n * p.o_stride[0] + h * p.o_stride[1] + col) =
           sum == 0.f ? make_uint2(0u, 0u) : make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
-    if (p.lse && col == 0) p.lse[(int64_t)n * p.Hq + h] = sum > 0.f ? fmaf(fast_log2(sum), kLn2P, mx) : sum == 0.f ? -INFINITY : sum;
+    if (p.lse && col == 0) p.lse[(int64_t)n * p.Hq + h] = sum > 0.f ? fmaf(fast_log2(sum) - kSplitLift<T>, kLn2P, mx) : sum == 0.f ? -INFINITY : sum;
   }
   cluster.sync();  // the parts have been read
 }
@@ -462,7 +462,8 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
           float sum = 0.f;
 #pragma unroll
           for (int nt = 0; nt < 2 * NK; ++nt) {
-            const float p0 = fast_exp2((s[im][nt][2 * e] - msub) * kLog2eP), p1 = fast_exp2((s[im][nt][2 * e + 1] - msub) * kLog2eP);
+            const float p0 = fast_exp2(fmaf(s[im][nt][2 * e] - msub, kLog2eP, kSplitLift<T>)),
+                        p1 = fast_exp2(fmaf(s[im][nt][2 * e + 1] - msub, kLog2eP, kSplitLift<T>));
             sum += p0 + p1;
             // the probabilities are rounded to the 16 bits of V: half a step of relative error each, what the result is rounded by
             pf[im][nt >> 1][2 * (nt & 1) + e] = Pack2<T>::pack(p0, p1);
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
               if (i * 8 < p.D)
                 *reinterpret_cast<uint32_t*>(dst + i * 8 + qc) =
                     ls == 0.f ? 0u : Pack2<T>::pack(o[im][i][2 * e] * inv, o[im][i][2 * e + 1] * inv);
-            if (p.lse && qc == 0) p.lse[(int64_t)n * p.Hq + h] = ls > 0.f ? fmaf(fast_log2(ls), kLn2P, m[im][e]) : ls == 0.f ? -INFINITY : ls;
+            if (p.lse && qc == 0) p.lse[(int64_t)n * p.Hq + h] = ls > 0.f ? fmaf(fast_log2(ls) - kSplitLift<T>, kLn2P, m[im][e]) : ls == 0.f ? -INFINITY : ls;
           } else {
             // slot 1: the CTA in which the item begins; 0: the others
             const int64_t row = (((int64_t)blockIdx.x * 2 + (seg.t0 == 0 ? 1 : 0)) * WH + wh) * MT + r;

@@ -438,23 +438,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         mbar_arrive_warp(s_read + 8 * x);  // the tensor core may start on the stream's next tile
         complete(3);
         const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sl2q, baseq);  // sl2 > 0
-        // Far from zero the rounding of the maximum, a 2^-24 of it, would be a factor that P cannot hold.  There the logits are
-        // rounded as their maximum was (and beyond 2^100, where two of them are equal or nothing beside one another, left in quarters).
-        float unit = sl2;
         const bool far = __any_sync(0xffffffffu, (fabsf(mx) >= 262144.f && mx > -INFINITY) || (SLOPES && fabsf(baseq) >= 262144.f));
-        if (far) {
-          unit = fabsf(mx) < 1.2676506e30f ? 4.f : 1.f;
-          const uint64_t q2 = f2(sl2q, sl2q), b2 = f2(baseq, baseq);
-#pragma unroll
-          for (int ch = 0; ch < 4; ++ch)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float v0, v1;
-              f2_unpack(f2_fma(f2(__uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1])), q2, b2), v0, v1);
-              s[ch][i] = __float_as_uint(v0);
-              s[ch][i + 1] = __float_as_uint(v1);
-            }
-        }
         // ---- the reference maximum, from tile to tile: it moves only when the maximum has grown by more than 2^8 (exact: the row
         // sums carry the same reference)
         const float m_last = m_used;
@@ -493,7 +477,23 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const float msub = m_used == -INFINITY ? 0.f : m_used;
         l *= fast_exp2(4.f * (m_last - msub));  // (0 at the stream's first tile, where l is 0)
         uint64_t l2a = f2(0.f, 0.f), l2b = f2(0.f, 0.f);
-        const float off = far ? -unit * msub : 4.f * (baseq - msub);
+        float unit = sl2, off = 4.f * (baseq - msub) + kTileLift<T>;
+        // Far from zero the rounding of the maximum, a 2^-24 of it, would be a factor that P cannot hold: there the logits are rounded
+        // as their maximum was before it is subtracted.
+        if (far) {
+          unit = 4.f;
+          off = kTileLift<T>;
+          const uint64_t q2 = f2(sl2q, sl2q), b2 = f2(baseq, baseq), m2 = f2(-msub, -msub);
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float v0, v1;
+              f2_unpack(f2_add(f2_fma(f2(__uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1])), q2, b2), m2), v0, v1);
+              s[ch][i] = __float_as_uint(v0);
+              s[ch][i + 1] = __float_as_uint(v1);
+            }
+        }
         const uint64_t nm = f2(off, off), unit2 = f2(unit, unit);
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
@@ -578,7 +578,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       }
       if (x == 0 && tk >= 0) {
         if (!whole) a.ml[slot * 128 + row] = make_float2(m, ls);
-        else if (p.lse) p.lse[(int64_t)gn * p.Hq + hd] = ls > 0.f ? fmaf(4.f * kLn2P, m, fast_log2(ls) * kLn2P) : ls == 0.f ? -INFINITY : ls;
+        else if (p.lse) p.lse[(int64_t)gn * p.Hq + hd] = ls > 0.f ? fmaf(4.f * kLn2P, m, (fast_log2(ls) - kTileLift<T>) * kLn2P) : ls == 0.f ? -INFINITY : ls;
       }
       if (!whole && begins && threadIdx.x == 0) {
         a.desc[2 * blockIdx.x] = make_int4(sg->rt, sg->hg, sg->last_cta, 0);
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(128 * SHARE) paged_join_tile_kernel(const __gr
     if (col0 + g * 8 < p.D)
       *reinterpret_cast<uint4*>(dst + g * 8) = make_uint4(p2(acc[2 * g].x, acc[2 * g].y), p2(acc[2 * g].z, acc[2 * g].w), p2(acc[2 * g + 1].x, acc[2 * g + 1].y),
                                                           p2(acc[2 * g + 1].z, acc[2 * g + 1].w));
-  if (p.lse && blockIdx.y == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? fmaf(4.f * kLn2P, m, fast_log2(l) * kLn2P) : l == 0.f ? -INFINITY : l;
+  if (p.lse && blockIdx.y == 0) p.lse[(int64_t)n * p.Hq + h] = l > 0.f ? fmaf(4.f * kLn2P, m, (fast_log2(l) - kTileLift<T>) * kLn2P) : l == 0.f ? -INFINITY : l;
 }
 
 template <typename T, int TD, bool SLOPES>

@@ -8,7 +8,7 @@ from flashbias_b200 import _lib, check_device_status
 from flashbias_b200.flash_bias import _op
 from oracle import serving_oracle as orc
 from tests.serving_helpers import FP32, assert_within, half_step, paged_inputs, tree
-from tests.test_paged_attention_gpu import kernel_of
+from tests.test_paged_attention_gpu import bounds, kernel_of
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,25 @@ def test_a_value_that_is_not_finite_counts_however_small_its_weight(kernel, T, D
         seen = (mask[:, 0] >> 1 & 1).bool()
         assert seen.any() and not seen.all()
         assert ((o.double() - clean.double()).abs() <= allowed)[~seen].all() and not o[seen].isfinite().any()
+
+
+@pytest.mark.parametrize("kernel", ["own", "split", "general"])
+@pytest.mark.parametrize("lens,T,width", [(9000, 1, 0), (6000, 1, 600), (7000, 30, 0), (3000, 2, 600)])
+def test_many_small_weights_beside_a_large_one(kernel, lens, T, width):
+    """fp16: the first key takes nearly all of the softmax and holds zeros; the rest weighs e^-19 = 2^-27.4 each, less than the
+    smallest 16-bit number (2^-24), and is all of the result."""
+    kw = paged_inputs([lens], [T], 4, 2, 128, 16, torch.float16, 35)
+    kw["block_table"] = torch.nn.functional.pad(kw["block_table"], (0, width), value=-1)
+    g = torch.Generator().manual_seed(36)
+    kw["q"] = (1.0 + 0.02 * torch.randn(kw["q"].shape, generator=g)).half()
+    for at in used_places(kw):
+        kw["key_cache"][at] = 0.02 * torch.randn(2, 128, generator=g).half()
+        kw["value_cache"][at] = (400.0 + 20.0 * torch.randn(2, 128, generator=g)).half()
+    kw["key_cache"][used_places(kw)[0]] = 19.0 / math.sqrt(128)
+    kw["value_cache"][used_places(kw)[0]] = 0.0
+    want, lse, weight, size = oracle(kw)
+    assert (want.abs() > 2.0 ** -14).all()
+    o, got = forward(kw, kernel)
+    bo, bl = bounds(want, weight, size, 128, torch.float16)
+    assert_within("o", o, want, bo)
+    assert_within("lse", got, lse, bl + 8 * FP32 * lse.abs() + 1e-6)
