@@ -477,7 +477,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const float msub = m_used == -INFINITY ? 0.f : m_used;
         l *= fast_exp2(4.f * (m_last - msub));  // (0 at the stream's first tile, where l is 0)
         uint64_t l2a = f2(0.f, 0.f), l2b = f2(0.f, 0.f);
-        float unit = sl2, off = 4.f * (baseq - msub) + kTileLift<T>;
+        float unit = sl2, off = fminf(4.f * (baseq - msub), FLT_MAX) + kTileLift<T>;  // (finite: there may be no key, all -inf)
         // Far from zero the rounding of the maximum, a 2^-24 of it, would be a factor that P cannot hold: there the logits are rounded
         // as their maximum was before it is subtracted.
         if (far) {

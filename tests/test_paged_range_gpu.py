@@ -95,6 +95,25 @@ def test_equal_logits_of_any_finite_size(kernel, exponent, scale, dtype, T, lens
     assert_within("lse", got, lse, 8 * FP32 * lse.abs())
 
 
+@pytest.mark.parametrize("kernel", ["own", "split", "general"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_huge_logits_beside_tiles_of_which_a_row_sees_nothing(kernel, sign):
+    """400 new tokens whose rows see the keys of one stretch of 64 alone, with logits of 2.5e38; 512 key tiles, several in a row per CTA."""
+    kw = paged_inputs([0], [400], 32, 32, 128, 16, torch.bfloat16, 42)
+    for at in used_places(kw):
+        kw["key_cache"][at] = 0.0
+        kw["key_cache"][at][..., 5] = 2.0 ** 61
+    kw["q"][..., 5] = sign * 2.0 ** 62
+    kw["softmax_scale"] = 24.0
+    kw["tree_mask"] = torch.zeros(400, 7, dtype=torch.int64)
+    for n in range(400):
+        kw["tree_mask"][n, n // 32 % 6] = -1
+    want, lse, weight, _ = oracle(kw)
+    o, got = forward(kw, kernel)
+    assert_within("o", o, want, weights_alone(want, weight, torch.bfloat16))
+    assert_within("lse", got, lse, 8 * FP32 * lse.abs())
+
+
 @pytest.mark.parametrize("kernel", ["own", "split"])
 @pytest.mark.parametrize("T", [30, 64])
 def test_large_logits_of_two_kinds(kernel, T):
