@@ -411,17 +411,34 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
       // what lies below -2.36e38 (a mask of the type's lowest value among the factors) would be -inf, a key that is not seen
       const int j0 = tile * KT + qc;
       const bool masked = okm != ALL || tile * KT + KT > rq.len;
-#pragma unroll
-      for (int im = 0; im < NM; ++im)
+      // keys of new tokens, whose position may lie anywhere: the difference is taken of whole numbers
+      const bool moved = BIAS == PAGED_SLOPES && p.positions && tile * KT + KT > rq.len;
+      if (moved) {
 #pragma unroll
         for (int nt = 0; nt < 2 * NK; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v = s[im][nt][i] * p.softmax_scale;
-            if (BIAS == PAGED_SLOPES) v = fmaf(slope[im][i >> 1], (float)(j0 + nt * 8 + (i & 1) - my_pos[im][i >> 1]), v);
-            if (BIAS >= PAGED_FACTORS) v += f[im][nt][i];
-            s[im][nt][i] = v;
+          for (int x = 0; x < 2; ++x) {
+            const int j = j0 + nt * 8 + x, at = j >= rq.len && j < rq.keys ? p.positions[rq.first + j - rq.len] : j;
+#pragma unroll
+            for (int im = 0; im < NM; ++im)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                s[im][nt][2 * e + x] = fmaf(slope[im][e], (float)(at - my_pos[im][e]), s[im][nt][2 * e + x] * p.softmax_scale);
           }
+      }
+      if (!moved) {
+#pragma unroll
+        for (int im = 0; im < NM; ++im)
+#pragma unroll
+          for (int nt = 0; nt < 2 * NK; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float v = s[im][nt][i] * p.softmax_scale;
+              if (BIAS == PAGED_SLOPES) v = fmaf(slope[im][i >> 1], (float)(j0 + nt * 8 + (i & 1) - my_pos[im][i >> 1]), v);
+              if (BIAS >= PAGED_FACTORS) v += f[im][nt][i];
+              s[im][nt][i] = v;
+            }
+      }
       if (masked) {
         const int td0 = tile * KT - rq.len;
 #pragma unroll
@@ -433,12 +450,8 @@ __global__ void __launch_bounds__(kSplitThreads, split_ctas(TD, MT)) paged_split
 #pragma unroll
             for (int nt = 0; nt < 2 * NK; ++nt)
 #pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int i = 2 * e + x, k = nt * 8 + qc + x, j = tile * KT + k;
-                if (BIAS == PAGED_SLOPES && p.positions && j >= rq.len && j < rq.keys)  // the key's position instead of its place
-                  s[im][nt][i] = fmaf(slope[im][e], (float)(p.positions[rq.first + j - rq.len] - j), s[im][nt][i]);
-                if (!(bits >> k & 1)) s[im][nt][i] = -INFINITY;
-              }
+              for (int x = 0; x < 2; ++x)
+                if (!(bits >> (nt * 8 + qc + x) & 1)) s[im][nt][2 * e + x] = -INFINITY;
           }
       }
 

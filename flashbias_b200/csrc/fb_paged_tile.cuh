@@ -60,7 +60,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 200);
   const uint32_t abort_flag = bar0 + 204;
   // per tile, eight deep (the producer is four tiles ahead of a softmax at most): which of the tile's pages exist, and the
-  // positions of its keys behind its first place, where they are not their places
+  // positions of its keys behind its first place, where they are not their places (behind the first new token's where positions are
+  // given: they may lie anywhere, and what counts between new tokens is small beside that)
   volatile uint32_t* s_pages = reinterpret_cast<volatile uint32_t*>(smem + Cfg::OFF_BAR + 208);
   float* s_pos = reinterpret_cast<float*>(smem + Cfg::OFF_POS);
   // per segment, eight deep: its number + 1 if it has values that were taken out; the segment
@@ -182,11 +183,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             const uint32_t there = ~__ballot_sync(0xffffffffu, bad);
             if (t >= KST && !wait_all(k_free + 8 * st, (t / KST - 1) & 1)) return;
             if (SLOPES && k0 + 128 > seg.r.len) {
+              const int at0 = p.positions ? p.positions[seg.r.first] : k0;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int k = k0 + e * 32 + lane;
                 s_pos[(t & 7) * 128 + e * 32 + lane] =
-                    (float)((p.positions && k >= seg.r.len && k < seg.r.keys ? p.positions[seg.r.first + k - seg.r.len] : k) - k0);
+                    (float)((p.positions && k >= seg.r.len && k < seg.r.keys ? p.positions[seg.r.first + k - seg.r.len] : k) - at0);
               }
             }
             if (lane == 0) s_pages[t & 7] = there;
@@ -361,6 +363,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       // the bias in units of q.k, so that a logit costs one product more: s + slope_r (pos - k0), times sl2, plus 4 baseq
       const float slope2 = SLOPES && tk >= 0 ? p.slopes[hd] * kLog2eP : 0.f, slope_r = slope2 / sl2;
       const int my_pos = SLOPES && tk >= 0 ? (p.positions ? p.positions[gn] : len + tk) : 0;
+      const int own_pos = SLOPES && p.positions && tk >= 0 ? p.positions[sg->first] - my_pos : 0;
       for (int j = x; j < n_kv; j += 2, ++c) {
         const int k0 = (t1 - 1 - j) * 128;
         const bool own = k0 + 128 > len;  // the tile holds new tokens' keys, or places behind them
@@ -387,7 +390,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               if (!(there >> ((ch * 32 + i) / rows) & 1)) bits[ch] &= ~(1u << i);
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const float baseq = SLOPES ? 0.25f * slope2 * (float)(k0 - my_pos) : 0.f;
+        const float baseq = SLOPES ? 0.25f * slope2 * (float)(own && p.positions ? own_pos : k0 - my_pos) : 0.f;
         auto complete = [&](int ch) {
           if (dead) {
             if (SLOPES) {

@@ -179,3 +179,29 @@ def test_many_small_weights_beside_a_large_one(kernel, lens, T, width):
     bo, bl = bounds(want, weight, size, 128, torch.float16)
     assert_within("o", o, want, bo)
     assert_within("lse", got, lse, bl + 8 * FP32 * lse.abs() + 1e-6)
+
+
+@pytest.mark.parametrize("kernel", ["own", "split", "general"])
+@pytest.mark.parametrize("T,lens", [(7, 0), (60, 0), (12, 100), (130, 300)])
+@pytest.mark.parametrize("offset", [1_000_000, 12_345_678, -700_001])
+def test_positions_far_from_the_places(kernel, T, lens, offset):
+    """Positions count by their differences: a request whose tokens stand far from their places (or whose cached keys, at theirs,
+    weigh nothing) sees small biases between its new tokens."""
+    kw = paged_inputs([lens], [T], 4, 2, 64, 16, torch.bfloat16, 37)
+    _, mask, depth = tree([T], 38, 3)
+    kw["tree_mask"] = mask
+    kw["positions"] = (depth + offset).int()
+    kw["slopes"] = torch.tensor([0.7, 0.31, 0.11, 0.05]) * (1 if offset > 0 else -1)
+    want, lse, weight, size = oracle(kw)
+    if lens:  # the cached keys' logits are below -20000 and weigh nothing: what counts is the size of the others
+        kw0 = dict(kw, lens=kw["lens"] * 0)
+        at = used_places(kw)
+        for c in ("key_cache", "value_cache"):
+            kw0[c] = torch.stack([kw[c][p] for p in at[lens:]]).unsqueeze(1)
+        kw0["block_table"] = torch.arange(T, dtype=torch.int32)[None]
+        w0, l0, weight, size = oracle(kw0)
+        assert (w0 - want).abs().max() < 1e-12
+    o, got = forward(kw, kernel)
+    bo, bl = bounds(want, weight, size, 64, torch.bfloat16)
+    assert_within("o", o, want, bo)
+    assert_within("lse", got, lse, bl + 8 * FP32 * lse.abs() + 1e-6)
