@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(NT) paged_plan_kernel(const __grid_constant__ 
   const int free_raw = *p.free_count;
   Ask a = plan_load(p, threadIdx.x);
   const int64_t free0 = min(max(free_raw, 0), p.stack_size);
+  if (free0 != free_raw && threadIdx.x == 0 && p.status) *reinterpret_cast<volatile int32_t*>(p.status) = FB_DEV_BAD_INDEX;
   if (threadIdx.x == 0) sh.taken = 0;
 
   // ---- token offsets, pages that come back, pages that are missing

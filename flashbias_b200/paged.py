@@ -38,7 +38,8 @@ def paged_plan(block_table: torch.Tensor, pages_held: torch.Tensor, free_pages: 
 
     block_table (requests, width), pages_held (requests), free_pages (pool, a stack) and free_count (1): int32, the state of
         the pool, updated in place.  Pages that a request no longer needs go back to the stack (``lens = new_lens = 0`` frees
-        a request), missing ones are taken from its top, in the order of the requests.
+        a request), missing ones are taken from its top, in the order of the requests.  Counts that do not fit the table
+        or the stack are reported as device-side errors.
     lens, new_lens: (requests) int32.  num_tokens: rows of the step's token tensors; what the requests do not fill is padding.
     parents: (num_tokens) int32, for trees of drafted tokens: index within its request of each token's parent, which comes
         before it; negative for the cached context.  None: each token follows the one before.

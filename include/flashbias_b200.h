@@ -268,7 +268,7 @@ typedef struct fb_plan_params {
   int64_t table_stride;
   int32_t *pages_held; /* (B), updated */
   int32_t *free_pages; /* (stack_size), the first *free_count of them are free; updated */
-  int32_t *free_count; /* (1), updated */
+  int32_t *free_count; /* (1), updated; outside [0, stack_size] it sets FB_DEV_BAD_INDEX and counts as the nearest */
   const int32_t *lens, *new_lens;
   const int32_t *parents; /* optional (num_tokens): index within its request of a token's parent, before the token's own; < 0: the
                              cached context.  Null: each token follows the one before. */

@@ -119,6 +119,21 @@ def test_a_page_count_beyond_the_row_is_refused_and_reported():
     assert step.lens.tolist() == [-1, 8] and h.tolist() == [9, 2] and c.tolist() == [count - 1]
 
 
+@pytest.mark.parametrize("B", [2, 1500])
+@pytest.mark.parametrize("count,counted", [(-3, 0), (10 ** 9, None)])
+def test_a_count_of_free_pages_beyond_the_stack_is_reported(B, count, counted):
+    """Taken for the nearest one that the stack can have."""
+    lens, new = [8] * B, [1] * B
+    table, held, stack, _ = pool_of(lens, new, 8, 3, 10)
+    stack = stack[:next(i for i, x in enumerate(stack + [-9]) if x < 0)]  # free pages alone
+    want = orc.plan(table, held, stack, len(stack) if counted is None else counted, lens, new, 8, B)
+    (t, h, _, c), step = run((table, held, stack, count), lens, new, 8, B)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="out of range"):
+        check_device_status()
+    assert t.tolist() == want["table"] and h.tolist() == want["held"] and c.tolist() == [want["count"]] and step.lens.tolist() == want["lens"]
+
+
 def test_a_graph_of_the_plan_follows_the_lengths():
     page, lens, new = 16, [30, 50], [1, 1]
     state = pool_of(lens, [60, 60], page, 10, 9)
