@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(1024) rope_weight_kernel(const __grid_constant
 namespace {
 bool negative(const int64_t (&s)[3]) { return s[0] < 0 || s[1] < 0 || s[2] < 0; }
 
-int validate_rope(const fb_rope_params* p) {
+int validate_rope(const fb_rope_params* p, bool backward = false) {
   if (!p) return FB_EINVAL_NULL;
   if (p->B <= 0 || p->S <= 0 || p->Hq < 0 || p->Hk < 0 || p->Hq + (int64_t)p->Hk <= 0 || p->Hq + (int64_t)p->Hk > 65536) return FB_EINVAL_SHAPE;
   if (p->D <= 0 || p->D > kRopeMaxD || (int64_t)p->B * p->S > 0x7fff0000LL) return FB_EINVAL_SHAPE;
@@ -206,7 +206,8 @@ int validate_rope(const fb_rope_params* p) {
     for (int i = 0; i < p->rot / 2; ++i)
       if (p->pair_axis[i] >= p->naxes) return FB_EINVAL_ROPE;
   }
-  if ((p->Hq && !p->q) || (p->Hk && !p->k)) return FB_EINVAL_NULL;
+  // (the backward reads q and k for the norm alone)
+  if ((p->Hq && !p->q && (!backward || p->q_weight)) || (p->Hk && !p->k && (!backward || p->k_weight))) return FB_EINVAL_NULL;
   if (negative(p->q_stride) || negative(p->k_stride)) return FB_EINVAL_STRIDE;
   return 0;
 }
@@ -319,12 +320,12 @@ extern "C" int fb_norm_rope(const fb_rope_params* p, void* cuda_stream) {
 }
 
 extern "C" size_t fb_norm_rope_bwd_workspace_bytes(const fb_rope_params* p) {
-  if (validate_rope(p) || !wants_weights(p)) return 0;
+  if (validate_rope(p, true) || !wants_weights(p)) return 0;
   return round256((size_t)rope_bwd_grid(p, rope_run(p, ROPE_BACKWARD)).all * 2 * p->D * 4);
 }
 
 extern "C" int fb_norm_rope_bwd(const fb_rope_params* p, void* cuda_stream) {
-  if (const int rc = validate_rope(p)) return rc;
+  if (const int rc = validate_rope(p, true)) return rc;
   if ((p->Hq && (!p->dq_out || !p->dq)) || (p->Hk && (!p->dk_out || !p->dk))) return FB_EINVAL_NULL;
   if (negative(p->dq_out_stride) || negative(p->dk_out_stride) || negative(p->dq_stride) || negative(p->dk_stride)) return FB_EINVAL_STRIDE;
   if ((p->dq_weight && !p->q_weight) || (p->dk_weight && !p->k_weight)) return FB_EINVAL_NULL;

@@ -122,26 +122,46 @@ std::tuple<Tensor, Tensor> rope_forward(const Tensor& q, const Tensor& k, const 
   return {qo, ko};
 }
 
+// A tensor whose gradient is taken: itself where the backward reads it (norm weights), else its layout alone.
+struct RopeSource {
+  Tensor x;  // undefined where it is not read
+  std::vector<int64_t> sizes, strides;  // empty without the tensor; strides empty where its gradient is contiguous
+};
+RopeSource rope_source(const Tensor& x, bool read) {
+  if (!x.defined()) return {};
+  return {read ? x : Tensor(), x.sizes().vec(), x.is_non_overlapping_and_dense() ? x.strides().vec() : std::vector<int64_t>()};
+}
+Tensor empty_dense_as(const RopeSource& s, const Tensor& like) {
+  if (s.strides.empty()) return empty_on(s.sizes, like.scalar_type(), like);
+  if (c10::impl::dispatch_mode_enabled()) return at::empty_strided(s.sizes, s.strides, like.options());
+  return Tensor(at::detail::empty_strided_cuda(s.sizes, s.strides, like.scalar_type(), like.device()));
+}
+
 // Gradients of (q, k, q_weight, k_weight); dq_out or dk_out may be undefined: that tensor is left out.
-std::tuple<Tensor, Tensor, Tensor, Tensor> rope_backward(Tensor dqo, Tensor dko, const Tensor& q, const Tensor& k, const RopeArgs& a,
-                                                         bool want_qw, bool want_kw) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> rope_backward(Tensor dqo, Tensor dko, const RopeSource& q, const RopeSource& k, at::ScalarType type,
+                                                         const RopeArgs& a, bool want_qw, bool want_kw) {
   check_device_status();
-  check_rope_qk(q, k);
-  c10::cuda::CUDAGuard guard(q.device());
-  fb_rope_params p{};
-  fill_rope(p, a, q, q.size(0), q.size(1), q.size(3));
   Tensor dq, dk, dqw, dkw;
-  auto take = [&](Tensor& g, const Tensor& x, const Tensor& w, bool want_w, int32_t& H, const void*& xp, int64_t(&xs)[3], const void*& gp,
+  if (!dqo.defined() && !dko.defined()) return {dq, dk, dqw, dkw};
+  const Tensor& like = dqo.defined() ? dqo : dko;
+  c10::cuda::CUDAGuard guard(like.device());
+  fb_rope_params p{};
+  FB_ASSERT(like.scalar_type() == type, "");
+  fill_rope(p, a, like, q.sizes[0], q.sizes[1], q.sizes[3]);
+  auto take = [&](Tensor& g, const RopeSource& s, const Tensor& w, bool want_w, int32_t& H, const void*& xp, int64_t(&xs)[3], const void*& gp,
                   int64_t(&gs)[3], Tensor& dx, void*& dxp, int64_t(&dxs)[3], Tensor& dw, void*& dwp) {
-    if (!g.defined() || !x.defined()) return;
-    FB_ASSERT(g.sizes() == x.sizes() && g.scalar_type() == x.scalar_type() && g.device() == x.device(), "");
+    if (!g.defined() || s.sizes.empty()) return;
+    FB_ASSERT(g.sizes() == s.sizes && g.scalar_type() == type && g.device() == like.device(), "");
     if (g.stride(-1) != 1) g = g.contiguous();
-    H = (int32_t)x.size(2);
-    xp = x.data_ptr();
-    strides_bhs(x, xs);
+    H = (int32_t)s.sizes[2];
+    if (s.x.defined()) {
+      FB_ASSERT(s.x.device() == g.device(), "");
+      xp = s.x.data_ptr();
+      strides_bhs(s.x, xs);
+    }
     gp = g.data_ptr();
     strides_bhs(g, gs);
-    dx = empty_dense_as(x);
+    dx = empty_dense_as(s, g);
     dxp = dx.data_ptr();
     strides_bhs(dx, dxs);
     if (want_w && w.defined()) {
@@ -158,7 +178,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rope_backward(Tensor dqo, Tensor dko,
   }
   Tensor ws;
   if (const size_t need = fb_norm_rope_bwd_workspace_bytes(&p)) {
-    ws = workspace(need, q);
+    ws = workspace(need, like);
     p.workspace = ws.data_ptr();
     p.workspace_bytes = need;
   }
@@ -180,7 +200,14 @@ struct NormRopeNode : torch::autograd::Function<NormRopeNode> {
                         contiguous_or_undefined(k_weight), has_axes ? OptAxes(axes) : std::nullopt, interleaved, eps};
     auto [qo, ko] = rope_forward(q, k, a);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, a.positions, a.inv_freq, a.q_weight, a.k_weight});
+    // (a tensor without a weight is not read again: kept, it would hold on to the projection it is a slice of)
+    const RopeSource qs = rope_source(q, a.q_weight.defined()), ks = rope_source(k, a.k_weight.defined());
+    ctx->save_for_backward({qs.x, ks.x, a.positions, a.inv_freq, a.q_weight, a.k_weight});
+    ctx->saved_data["q_sizes"] = qs.sizes;
+    ctx->saved_data["q_strides"] = qs.strides;
+    ctx->saved_data["k_sizes"] = ks.sizes;
+    ctx->saved_data["k_strides"] = ks.strides;
+    ctx->saved_data["type"] = (int64_t)q.scalar_type();
     ctx->saved_data["axes"] = axes;
     ctx->saved_data["has_axes"] = has_axes;
     ctx->saved_data["interleaved"] = interleaved;
@@ -196,12 +223,14 @@ struct NormRopeNode : torch::autograd::Function<NormRopeNode> {
     const RopeArgs a = {s[2], s[3], s[4], s[5],
                         ctx->saved_data["has_axes"].toBool() ? OptAxes(ctx->saved_data["axes"].toIntVector()) : std::nullopt,
                         ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble()};
+    const RopeSource q = {s[0], ctx->saved_data["q_sizes"].toIntVector(), ctx->saved_data["q_strides"].toIntVector()};
+    const RopeSource k = {s[1], ctx->saved_data["k_sizes"].toIntVector(), ctx->saved_data["k_strides"].toIntVector()};
     // (edges are counted over the tensors that were given)
-    const int w0 = 1 + (s[1].defined() ? 1 : 0) + (s[2].defined() ? 1 : 0) + (s[3].defined() ? 1 : 0);
+    const int w0 = 1 + (k.sizes.empty() ? 0 : 1) + (s[2].defined() ? 1 : 0) + (s[3].defined() ? 1 : 0);
     const bool want_qw = s[4].defined() && ctx->needs_input_grad(w0);
     const bool want_kw = s[5].defined() && ctx->needs_input_grad(w0 + (s[4].defined() ? 1 : 0));
     auto [dq, dk, dqw, dkw] =
-        rope_backward(grads[0], grads.size() > 1 ? grads[1] : Tensor(), s[0], s[1], a, want_qw, want_kw);
+        rope_backward(grads[0], grads.size() > 1 ? grads[1] : Tensor(), q, k, (at::ScalarType)ctx->saved_data["type"].toInt(), a, want_qw, want_kw);
     if (again) {  // there is no second derivative: to ask for it is an error, not a zero
       // (with the edges of this node, so that a search for the inputs passes it)
       auto edges = torch::autograd::get_current_node()->next_edges();

@@ -218,7 +218,8 @@ typedef struct fb_rope_params {
   void *q_out, *k_out;
   int64_t q_out_stride[3], k_out_stride[3];
 
-  /* backward only: gradients of q_out and k_out in, of q, k and the weights (weight_dtype, D values) out */
+  /* backward only: gradients of q_out and k_out in, of q, k and the weights (weight_dtype, D values) out; q or k itself may be null
+   * where it has no weight */
   const void *dq_out, *dk_out;
   int64_t dq_out_stride[3], dk_out_stride[3];
   void *dq, *dk, *dq_weight, *dk_weight; /* a weight gradient may be null */

@@ -173,6 +173,60 @@ def test_partial_gradients_and_expanded_ones():
     assert torch.equal(dqw2, dqw)
 
 
+@pytest.mark.parametrize("normed", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("heads_first", [False, True])
+def test_tensors_without_a_weight_may_change_before_the_backward(normed, heads_first):
+    """Their gradient needs the upstream one alone; that of a tensor with a weight reads it again, and autograd finds the change."""
+    q, k, w, pos, f, _ = inputs(2, 300, 8, 4, 64, 48, 1, torch.bfloat16, torch.float32, 7)
+    if heads_first:
+        q, k = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k))
+    gq, gk = (torch.randn(t.shape, generator=torch.Generator().manual_seed(1)).to(t.dtype) for t in (q, k))
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k)]
+    rows = [t * 1 for t in leaves]
+    w = [x.cuda() if n else None for x, n in zip(w, normed)]
+    out = norm_rope_func(*rows, pos.cuda(), f.cuda(), *w)
+    with torch.no_grad():
+        for t, n in zip(rows, normed):
+            if not n:
+                t.zero_()
+    grads = torch.autograd.grad(out, leaves, (gq.cuda(), gk.cuda()), retain_graph=True)
+    ang = orc.rope_angles(pos, f)
+    for name, got, leaf, t, go, wt in (("dq", grads[0], leaves[0], q, gq, w[0]), ("dk", grads[1], leaves[1], k, gk, w[1])):
+        want, _, size, _ = orc.norm_rope_grads(t, go, wt, ang)
+        assert_within(name, got, want, rounded(want, torch.bfloat16, size.amax(-1, keepdim=True)))
+        assert got.stride() == leaf.stride()
+    for t, n in zip(rows, normed):
+        if n:
+            with torch.no_grad():
+                t.zero_()
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                torch.autograd.grad(out, leaves, (gq.cuda(), gk.cuda()))
+
+
+def test_gradients_of_expanded_tensors_without_a_weight():
+    q, k, _, pos, f, _ = inputs(1, 50, 4, 2, 64, 64, 1, torch.float16, None, 8)
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k)]
+    out = norm_rope_func(*[t.expand(3, -1, -1, -1) for t in leaves], pos.cuda(), f.cuda())
+    go = [torch.randn(t.shape, generator=torch.Generator().manual_seed(2)).half() for t in out]
+    for x, g, got in zip((q, k), go, torch.autograd.grad(out, leaves, [g.cuda() for g in go])):
+        want = orc.norm_rope_grads(x, g, None, orc.rope_angles(pos, f))[0]
+        # each of three gradients is rounded, and so are their two sums
+        assert_within("dx", got, want.sum(0, keepdim=True), 5 * rounded(want, torch.float16, g.double().abs().amax(-1, keepdim=True)).sum(0, keepdim=True))
+
+
+def test_a_fused_projection_is_freed_between_the_passes():
+    pos, f = torch.arange(4096).cuda(), torch.rand(32).cuda()
+    leaf = torch.randn(1, 4096, 24 * 64, device="cuda").half().requires_grad_(True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    qkv = leaf * 1
+    out = norm_rope_func(qkv[..., :512].unflatten(-1, (8, 64)), qkv[..., 512:1024].unflatten(-1, (8, 64)), pos, f)
+    del qkv
+    held = torch.cuda.memory_allocated() - before - sum(t.numel() * 2 for t in out)
+    assert held < 2 ** 20  # (the projection is 12 MB)
+    torch.autograd.grad(out, leaf, [torch.ones_like(t) for t in out])
+
+
 def test_a_second_derivative_is_refused():
     q, k, w, pos, f, _ = inputs(1, 9, 2, 1, 64, 64, 1, torch.bfloat16, torch.float32, 4)
     qd, wd = q.cuda().requires_grad_(True), w[0].cuda().requires_grad_(True)
