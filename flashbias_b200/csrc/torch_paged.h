@@ -290,6 +290,12 @@ void check_apart(const Tensor& cache, const Tensor& read) {
   };
   FB_ASSERT(read.numel() == 0 || end(read) <= cache.data_ptr() || end(cache) <= read.data_ptr(), "what is appended may not lie in a cache itself: copy it first");
 }
+// Caches of one call that certainly share elements (views that interleave, like keys beside values in one pool, do not).
+void check_distinct(const Tensor& a, const Tensor& b) {
+  const at::MemOverlapStatus o = at::get_overlap_status(a, b);
+  FB_ASSERT(o != at::MemOverlapStatus::Full && o != at::MemOverlapStatus::Partial && (a.numel() == 0 || b.numel() == 0 || a.data_ptr() != b.data_ptr()),
+            "the caches of a call may not share memory");
+}
 // a tensor that a kernel has written behind autograd's back
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -322,6 +328,7 @@ OptTensor paged_append(const OptTensor& q_, const Tensor& k_, const Tensor& v_, 
   check_cache(value_cache, k_, pages, page_size, Hk, D);
   check_written(key_cache);
   check_written(value_cache);
+  check_distinct(key_cache, value_cache);
   check_beside(slots, k_);
   FB_ASSERT(slots.dim() == 1 && slots.size(0) == N && is_index(slots), "slots holds one int32 or int64 per token");
   FB_ASSERT(k_bias_.has_value() == bias_cache.has_value(), "k_bias and bias_cache must be given together");
@@ -370,6 +377,8 @@ OptTensor paged_append(const OptTensor& q_, const Tensor& k_, const Tensor& v_, 
     FB_ASSERT(kb.scalar_type() == k.scalar_type(), "All tensors must have the same type");
     check_cache(*bias_cache, k, pages, page_size, kb.size(1), kb.size(2));
     check_written(*bias_cache);
+    check_distinct(key_cache, *bias_cache);
+    check_distinct(value_cache, *bias_cache);
     p.R = (int32_t)kb.size(2);
     p.bias_heads = (int32_t)kb.size(1);
     p.k_bias = kb.data_ptr();

@@ -63,7 +63,7 @@ def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, ke
     q: (tokens, nheads, headdim) or None; k, v: (tokens, nheads_k, headdim); k_bias: (tokens, nheads_k | 1, rank).
     slots: (tokens) int32 or int64, ``page * page_size + place``; negative: the token is padding and nothing is written.  A slot
         behind the cache is not written either and reported as a device-side error.  No slot may occur twice in a call, and
-        what is appended may not lie in a cache itself.
+        what is appended may not lie in a cache itself, nor may two caches share elements.
     positions: (tokens), or with axes (A, tokens).  The other arguments are those of ``norm_rope_func``; without positions and
         weights the keys are stored as they are.
 

@@ -163,3 +163,24 @@ def test_rows_that_lie_in_a_cache_are_refused():
     want = kc.view(32, 2, 16)[4:8].clone(), vc.view(32, 2, 16)[4:8].clone()
     paged_append(None, *want, kc, vc, slots)
     assert torch.equal(kc.view(32, 2, 16)[3:7], want[0]) and torch.equal(vc.view(32, 2, 16)[3:7], want[1])
+
+
+def test_caches_that_share_elements_are_refused_and_interleaved_ones_are_not():
+    _, k, v, _, _, _, kb = inputs(9, 2, 2, 16, 0, 16, torch.float16, 11)
+    pool = torch.zeros(6, 2, 8, 2, 16, device="cuda", dtype=torch.float16)  # keys beside values, page by page
+    slots = torch.arange(9, device="cuda") + 5
+    for kc, vc in ((pool[:, 0], pool[:, 0]), (pool.flatten(0, 1)[:6], pool.flatten(0, 1)[2:8])):
+        with pytest.raises(AssertionError, match="share"):
+            paged_append(None, k, v, kc, vc, slots)
+    other = torch.zeros(6, 8, 2, 16, device="cuda", dtype=torch.float16)
+    for bc in (pool[:, 0], pool[:, 1]):
+        with pytest.raises(AssertionError, match="share"):
+            paged_append(None, k, v, pool[:, 0], pool[:, 1], slots, k_bias=kb, bias_cache=bc)
+    assert pool.count_nonzero() == 0
+    paged_append(None, k, v, pool[:, 0], pool[:, 1], slots, k_bias=kb, bias_cache=other)
+    torch.cuda.synchronize()
+    for c, rows in ((pool[:, 0], k), (pool[:, 1], v), (other, kb)):
+        assert torch.equal(c.flatten(0, 1)[5:14], rows) and c.count_nonzero() == rows.count_nonzero()
+    wide = torch.zeros(6, 8, 2, 32, device="cuda", dtype=torch.float16)  # ... column by column
+    paged_append(None, k, v, wide[..., :16], wide[..., 16:], slots)
+    assert torch.equal(wide.flatten(0, 1)[5:14], torch.cat([k, v], -1))
