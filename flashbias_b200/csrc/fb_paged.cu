@@ -111,12 +111,15 @@ __global__ void __launch_bounds__(128) paged_general_kernel(const __grid_constan
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
+// Rows of a call and places of a request: 31 bits, less what the last tile and the copies ahead of it count beyond them.
+constexpr int64_t kMostPlaces = 0x7fff0000LL;
+
 static int validate_paged(const fb_paged_params* p) {
   if (!p) return FB_EINVAL_NULL;
-  if (p->N <= 0 || p->B <= 0 || p->Hq <= 0 || p->Hk <= 0 || p->Hq % p->Hk || (int64_t)p->N * p->Hq > 0x7fffffffLL) return FB_EINVAL_SHAPE;
+  if (p->N <= 0 || p->B <= 0 || p->Hq <= 0 || p->Hk <= 0 || p->Hq % p->Hk || (int64_t)p->N * p->Hq > kMostPlaces) return FB_EINVAL_SHAPE;
   if (p->D <= 0 || p->D > 128 || p->R < 0 || p->R > 256) return FB_EINVAL_SHAPE;
   if (p->dtype != FB_DTYPE_F16 && p->dtype != FB_DTYPE_BF16) return FB_EINVAL_DTYPE;
-  if (p->page_size <= 0 || p->table_width <= 0 || p->num_pages <= 0 || (int64_t)p->table_width * p->page_size > 0x7fffffffLL) return FB_EINVAL_PAGE;
+  if (p->page_size <= 0 || p->table_width <= 0 || p->num_pages <= 0 || (int64_t)p->table_width * p->page_size > kMostPlaces) return FB_EINVAL_PAGE;
   if (!p->q || !p->key_cache || !p->value_cache || !p->block_table || !p->lens || !p->cu_tokens || !p->o) return FB_EINVAL_NULL;
   if (p->R) {
     if (!p->q_bias || !p->bias_cache || p->slopes || (p->bias_heads != 1 && p->bias_heads != p->Hk)) return FB_EINVAL_BIAS;
@@ -142,7 +145,7 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
     if (i < 2) bits |= (uintptr_t)(p->q_stride[i] | p->o_stride[i]) * 2;
   }
   const int G = p->Hq / p->Hk;
-  if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 8 || (bits & 15) || (int64_t)p->N * G > 0x7fffffffLL) return plan;
+  if ((p->flags & FB_FLAG_FORCE_GENERAL) || p->D % 8 || (bits & 15)) return plan;
   const int64_t rows = ((int64_t)p->N * G + p->B - 1) / p->B;  // per request on average
   int dev = 0;
   cudaGetDevice(&dev);

@@ -480,7 +480,7 @@ std::tuple<Tensor, OptTensor> paged_forward(const Tensor& q_, const Tensor& key_
                 (block_table.stride(1) == 1 || block_table.size(1) == 1),
             "the block table is (requests, pages) of int32 with contiguous rows");
   const int64_t B = block_table.size(0), M = block_table.size(1);
-  FB_ASSERT(page_size <= 0x7fffffff && M <= 0x7fffffff && M * page_size <= 0x7fffffff, "a row of the block table holds at most 2^31 - 1 tokens");
+  FB_ASSERT(page_size <= 0x7fffffff && M <= 0x7fffffff && M * page_size <= 0x7fff0000, "a row of the block table holds at most 2^31 - 2^16 tokens");
   check_ints(lens, q_, B);
   check_ints(cu_tokens, q_, B + 1);
   const Tensor q = unit_rows(q_), qb = unit_rows_or_undefined(q_bias_);

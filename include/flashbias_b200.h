@@ -65,7 +65,7 @@ extern "C" {
 #define FB_EDEVICE -10         /* a kernel reported a device-side error through the status word */
 #define FB_EINVAL_SIZE -11     /* the problem needs more scratch than a fixed-capacity entry point holds */
 #define FB_EINVAL_ROPE -12     /* rotated columns, axes, frequencies or positions do not fit each other */
-#define FB_EINVAL_PAGE -13     /* page size, page count or table width not positive, or too many slots */
+#define FB_EINVAL_PAGE -13     /* page size, page count or table width not positive, or too many slots (attention: over 2^31 - 2^16 in a row of the table) */
 
 /*
  * One problem description, shared by forward and backward.

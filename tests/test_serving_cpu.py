@@ -105,6 +105,14 @@ def test_paged_attention_refuses(change, code):
     assert refused("fb_paged_fwd", paged_params, change) == code
 
 
+@pytest.mark.parametrize("change,code", [(dict(page_size=65537, table_width=32767), -13), (dict(page_size=1, table_width=2 ** 31 - 1), -13),
+                                         (dict(page_size=65536, table_width=32768 - 1), -6), (dict(N=2147450000 // 4), -2),
+                                         (dict(N=2147410000 // 4), -6)], ids=str)
+def test_paged_attention_refuses_what_its_tiles_would_count_beyond_31_bits(change, code):
+    """The last tile of the keys or rows, and copies that run ahead of it, are counted in 32 bits."""
+    assert refused("fb_paged_fwd", paged_params, change) == code
+
+
 def test_null_parameter_blocks_are_refused():
     lib = _lib.load()
     for call in ("fb_norm_rope", "fb_norm_rope_bwd", "fb_paged_append", "fb_paged_plan", "fb_paged_fwd"):
