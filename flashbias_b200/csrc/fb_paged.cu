@@ -116,7 +116,7 @@ constexpr int64_t kMostPlaces = 0x7fff0000LL;
 
 static int validate_paged(const fb_paged_params* p) {
   if (!p) return FB_EINVAL_NULL;
-  if (p->N <= 0 || p->B <= 0 || p->Hq <= 0 || p->Hk <= 0 || p->Hq % p->Hk || (int64_t)p->N * p->Hq > kMostPlaces) return FB_EINVAL_SHAPE;
+  if (p->N <= 0 || p->B <= 0 || p->B > kMostPlaces || p->Hq <= 0 || p->Hk <= 0 || p->Hq % p->Hk || (int64_t)p->N * p->Hq > kMostPlaces) return FB_EINVAL_SHAPE;
   if (p->D <= 0 || p->D > 128 || p->R < 0 || p->R > 256) return FB_EINVAL_SHAPE;
   if (p->dtype != FB_DTYPE_F16 && p->dtype != FB_DTYPE_BF16) return FB_EINVAL_DTYPE;
   if (p->page_size <= 0 || p->table_width <= 0 || p->num_pages <= 0 || (int64_t)p->table_width * p->page_size > kMostPlaces) return FB_EINVAL_PAGE;

@@ -15,6 +15,7 @@ namespace fb {
 
 constexpr int kPlanThreads = 1024, kPlanFewThreads = 128;
 constexpr int kPlanMaxCluster = 8;  // blocks of a portable cluster
+constexpr int kPlanMost = 0x7fff0000;  // tokens, requests: their counters go on by a cluster's threads, in 32 bits
 
 // What a request asks for.  int64 where int32 inputs can pass 32 bits.
 struct Ask {
@@ -291,7 +292,7 @@ extern "C" size_t fb_plan_params_size(void) { return sizeof(fb_plan_params); }
 
 extern "C" int fb_paged_plan(const fb_plan_params* p, void* cuda_stream) {
   if (!p) return FB_EINVAL_NULL;
-  if (p->B <= 0 || p->num_tokens < 0 || p->stack_size < 0) return FB_EINVAL_SHAPE;
+  if (p->B <= 0 || p->num_tokens < 0 || p->stack_size < 0 || p->B > kPlanMost || p->num_tokens > kPlanMost) return FB_EINVAL_SHAPE;
   if (p->page_size <= 0 || p->table_width <= 0 || (int64_t)p->table_width * p->page_size > 0x7fffffffLL) return FB_EINVAL_PAGE;
   if (p->table_stride < p->table_width) return FB_EINVAL_STRIDE;
   if (!p->block_table || !p->pages_held || !p->free_count || !p->lens || !p->new_lens || !p->cu_tokens || !p->lens_out) return FB_EINVAL_NULL;

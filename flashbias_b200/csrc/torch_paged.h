@@ -411,9 +411,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor> paged_plan(const Tensor& b
                 block_table.stride(1) == 1 && (block_table.size(0) == 1 || block_table.stride(0) >= block_table.size(1)),
             "the block table is (requests, pages) of int32 with contiguous rows");
   const int64_t B = block_table.size(0), M = block_table.size(1);
-  FB_ASSERT(B < 0x7fffffff && page_size > 0 && M <= 0x7fffffff && page_size <= 0x7fffffff && M * page_size <= 0x7fffffff,
+  FB_ASSERT(B <= 0x7fff0000 && page_size > 0 && M <= 0x7fffffff && page_size <= 0x7fffffff && M * page_size <= 0x7fffffff,
             "a row of the block table holds at most 2^31 - 1 tokens");
-  FB_ASSERT(num_tokens >= 0 && num_tokens < 0x7fffffff, "num_tokens out of range");
+  FB_ASSERT(num_tokens >= 0 && num_tokens <= 0x7fff0000, "num_tokens out of range");
   check_ints(pages_held, block_table, B);
   check_ints(lens, block_table, B);
   check_ints(new_lens, block_table, B);
@@ -480,6 +480,7 @@ std::tuple<Tensor, OptTensor> paged_forward(const Tensor& q_, const Tensor& key_
                 (block_table.stride(1) == 1 || block_table.size(1) == 1),
             "the block table is (requests, pages) of int32 with contiguous rows");
   const int64_t B = block_table.size(0), M = block_table.size(1);
+  FB_ASSERT(B <= 0x7fff0000, "too many requests");
   FB_ASSERT(page_size <= 0x7fffffff && M <= 0x7fffffff && M * page_size <= 0x7fff0000, "a row of the block table holds at most 2^31 - 2^16 tokens");
   check_ints(lens, q_, B);
   check_ints(cu_tokens, q_, B + 1);

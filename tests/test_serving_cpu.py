@@ -113,6 +113,14 @@ def test_paged_attention_refuses_what_its_tiles_would_count_beyond_31_bits(chang
     assert refused("fb_paged_fwd", paged_params, change) == code
 
 
+@pytest.mark.parametrize("change", [dict(num_tokens=2 ** 31 - 2), dict(num_tokens=2 ** 31 - 2 ** 16 + 1), dict(B=2 ** 31 - 2)], ids=str)
+def test_paged_plan_refuses_what_its_counters_would_pass(change):
+    """A thread's next token is as far on as a cluster has threads, counted in 32 bits."""
+    assert refused("fb_paged_plan", plan_params, change) == -2
+    if "B" in change:
+        assert refused("fb_paged_fwd", paged_params, change) == -2
+
+
 def test_null_parameter_blocks_are_refused():
     lib = _lib.load()
     for call in ("fb_norm_rope", "fb_norm_rope_bwd", "fb_paged_append", "fb_paged_plan", "fb_paged_fwd"):
