@@ -50,6 +50,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   using Cfg = TileCfg<TD>;
   constexpr int KST = Cfg::KST, VST = Cfg::VST, NB = TD / 64, CH = TD / 8;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  static_assert(KST + 3 < 8, "rings of pages and positions");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem), sQ = sbase, sK = sbase + Cfg::OFF_K, sV = sbase + Cfg::OFF_V, bar0 = sbase + Cfg::OFF_BAR;
@@ -59,7 +60,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                  seg_full = bar0 + 384;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BAR + 200);
   const uint32_t abort_flag = bar0 + 204;
-  // per tile, eight deep (the producer is four tiles ahead of a softmax at most): which of the tile's pages exist, and the
+  // per tile, eight deep: K's place is filled again when S of KST tiles before is done, for which a stream has taken the logits of
+  // the tile before that, or two before, and may still read positions (it signals ahead of its last 32 keys): the producer is up to
+  // KST + 3 tiles ahead of a softmax.  Which of the tile's pages exist, and the
   // positions of its keys behind its first place, where they are not their places (behind the first new token's where positions are
   // given: they may lie anywhere, and what counts between new tokens is small beside that)
   volatile uint32_t* s_pages = reinterpret_cast<volatile uint32_t*>(smem + Cfg::OFF_BAR + 208);

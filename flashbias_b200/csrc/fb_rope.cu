@@ -5,8 +5,10 @@
 //   g = rotation of dout by the opposite angle,  dw = sum over rows of g x r,  dx = r (w g - x r^2 mean(w g x))
 //
 // Bound by reading x (and dout) once and writing the result once.  The angle position * inv_freq is taken in 64 bits and
-// reduced to a fraction of a turn before its sine and cosine are taken in 32 (by the functions of the hardware, off by 2^-21,
-// an eighth of a percent of a step of fp16): at position 1e6 a 32-bit product is off by up to 0.03 rad.  It costs one pair of
+// reduced to a fraction of a turn before its sine and cosine are taken in 32, by the functions of the hardware: off by 2^-21, and the
+// rounding of the fraction and of its product with 2 pi by half as much again.  Results of 16 bits do not show it (an eighth of a
+// percent of a step of fp16); a term of a weight's gradient in fp32 carries it, several roundings of its own.  At position 1e6 a
+// 32-bit product is off by up to 0.03 rad.  It costs one pair of
 // functions per token and frequency, shared by the token's heads, so no table is kept.
 #include "fb_rope.cuh"
 

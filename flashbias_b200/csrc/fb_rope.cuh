@@ -30,7 +30,7 @@ __device__ __forceinline__ float2 rope_turn(const fb_rope_params& p, int b, int 
                                                 : (double)reinterpret_cast<const float*>(p.inv_freq)[pr];
   const double turns = pos * (f * kInv2Pi);
   float2 cs;
-  __sincosf((float)(turns - rint(turns)) * k2Pi, &cs.y, &cs.x);  // within +-pi: off by 2^-21
+  __sincosf((float)(turns - rint(turns)) * k2Pi, &cs.y, &cs.x);  // within +-pi: off by 2^-21, half as much again by the argument's roundings
   return cs;
 }
 
