@@ -341,6 +341,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const uint32_t m_own = sbase + Cfg::OFF_M + (x * 128 + row) * 4, m_other = sbase + Cfg::OFF_M + ((x ^ 1) * 128 + row) * 4;
     // Maxima are kept in quarters of a log2 unit, in which no finite logit overflows.
     const float sl2 = a.scale_log2, sl2q = 0.25f * sl2;
+    const uint64_t sl2p = f2(sl2, sl2);
     int c = 0, co = 0, n = 0, t0 = 0;  // key tiles of this stream and of the other, segments and key tiles so far
     uint32_t s[4][32];                 // the thread's row of the logit tile
     auto segment_both = [&](int n) {  // (the warpgroups leave together: behind an expired wait, too)
@@ -393,7 +394,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               if (!(there >> ((ch * 32 + i) / rows) & 1)) bits[ch] &= ~(1u << i);
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const float baseq = SLOPES ? 0.25f * slope2 * (float)(own && p.positions ? own_pos : k0 - my_pos) : 0.f;
+        float baseq = SLOPES ? 0.25f * slope2 * (float)(own && p.positions ? own_pos : k0 - my_pos) : 0.f;
         auto complete = [&](int ch) {
           if (dead) {
             if (SLOPES) {
@@ -444,7 +445,24 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         mbar_arrive_warp(s_read + 8 * x);  // the tensor core may start on the stream's next tile
         complete(3);
         const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), sl2q, baseq);  // sl2 > 0
-        const bool far = __any_sync(0xffffffffu, (fabsf(mx) >= 262144.f && mx > -INFINITY) || (SLOPES && fabsf(baseq) >= 262144.f));
+        // Far from zero the rounding of the maximum, a 2^-24 of it, would be a factor that P cannot hold: there the logits are rounded
+        // as their maximum was, and it is subtracted, before they are scaled.
+        const bool far = mx > -INFINITY && fmaxf(fabsf(mx), fabsf(baseq)) >= 262144.f;
+        auto subtract_far = [&] {
+          if (!__any_sync(0xffffffffu, far)) return;
+          const float msub = m_used == -INFINITY ? 0.f : m_used, back = 4.f / sl2;
+          const uint64_t q2 = f2(sl2q, sl2q), b2 = f2(baseq, baseq), m2 = f2(-msub, -msub);
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float v0, v1;
+              f2_unpack(f2_add(f2_fma(f2(__uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1])), q2, b2), m2), v0, v1);
+              s[ch][i] = __float_as_uint(v0 * back);
+              s[ch][i + 1] = __float_as_uint(v1 * back);
+            }
+          baseq = msub;
+        };
         // ---- the reference maximum, from tile to tile: it moves only when the maximum has grown by more than 2^8 (exact: the row
         // sums carry the same reference)
         const float m_last = m_used;
@@ -452,7 +470,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           asm volatile("bar.sync %0, 256;" ::"r"(2 + (x ^ 1)) : "memory");
           m_used = __uint_as_float(ld_shared_flag(m_other));
           const float m_new = fmaxf(m_used, mx);
-          if (__any_sync(0xffffffffu, m_new - m_used > 2.f)) {  // (from -inf: the difference is +inf, or NaN where both are)
+          if (__any_sync(0xffffffffu, m_new - m_used > 2.f || far)) {  // (from -inf: the difference is +inf, or NaN where both are)
             // O is stable behind the product of tile j - 1, which is the other stream's.  (The one two before it on that barrier,
             // tile j - 5, has completed: the other stream has waited for it ahead of its P of tile j - 3.)
             const int cp = co0 + ((j - 1) >> 1);
@@ -470,9 +488,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               tmem_st32(tO + ch * 32, r);
             }
             tmem_wait_st();
+            subtract_far();
           }
         } else {
           m_used = mx;
+          subtract_far();
         }
         if (j + 1 < n_kv) {
           st_shared_f32(m_own, m_used);
@@ -483,24 +503,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const float msub = m_used == -INFINITY ? 0.f : m_used;
         l *= fast_exp2(4.f * (m_last - msub));  // (0 at the stream's first tile, where l is 0)
         uint64_t l2a = f2(0.f, 0.f), l2b = f2(0.f, 0.f);
-        float unit = sl2, off = fminf(4.f * (baseq - msub), FLT_MAX) + kTileLift<T>;  // (finite: there may be no key, all -inf)
-        // Far from zero the rounding of the maximum, a 2^-24 of it, would be a factor that P cannot hold: there the logits are rounded
-        // as their maximum was before it is subtracted.
-        if (far) {
-          unit = 4.f;
-          off = kTileLift<T>;
-          const uint64_t q2 = f2(sl2q, sl2q), b2 = f2(baseq, baseq), m2 = f2(-msub, -msub);
-#pragma unroll
-          for (int ch = 0; ch < 4; ++ch)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float v0, v1;
-              f2_unpack(f2_add(f2_fma(f2(__uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1])), q2, b2), m2), v0, v1);
-              s[ch][i] = __float_as_uint(v0);
-              s[ch][i + 1] = __float_as_uint(v1);
-            }
-        }
-        const uint64_t nm = f2(off, off), unit2 = f2(unit, unit);
+        const float off = fminf(4.f * (baseq - msub), FLT_MAX) + kTileLift<T>;  // (finite: there may be no key, all -inf)
+        const uint64_t nm = f2(off, off);
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {
           uint32_t pw[16];  // 32 keys = 16 packed words
@@ -508,7 +512,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           for (int i = 0; i < 32; i += 2) {
             const uint64_t v = f2(__uint_as_float(s[ch][i]), __uint_as_float(s[ch][i + 1]));
             float a0, a1;
-            f2_unpack(f2_fma(v, unit2, nm), a0, a1);
+            f2_unpack(f2_fma(v, sl2p, nm), a0, a1);
             const float p0 = fast_exp2(a0), p1 = fast_exp2(a1);
             if (i & 2) l2b = f2_add(l2b, f2(p0, p1)); else l2a = f2_add(l2a, f2(p0, p1));
             pw[i / 2] = Pack2<T>::pack(p0, p1);
