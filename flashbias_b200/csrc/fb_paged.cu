@@ -155,7 +155,10 @@ static PagedPlan plan_paged(const fb_paged_params* p) {
   // and with every 32 rows, this one's hardly.  Tile / split kernel, us (rows on average, half as many more in the largest trees):
   // 128 columns, 18 rows (B16 T12 H16-8) over 100 keys 14.1 / 14.9, over 1000 28.4 / 26.7, over 8000 74.9 / 87.3; 26 rows 14.2 / 16.7,
   // 28.5 / 31.1, 75.7 / 103; 64 columns, 45 rows (T30) over 1000 keys 25.1 / 21.0, over 8000 61.8 / 66.8, 68 rows 25.4 / 24.0 and
-  // 62.0 / 76.8; 32 columns, 68 rows 24.9 / 18.7 and 59.9 / 57.2, 90 rows 24.9 / 22.5 and 61.2 / 73.8.
+  // 62.0 / 76.8; 32 columns, 68 rows 24.9 / 18.7 and 59.9 / 57.2, 90 rows 24.9 / 22.5 and 61.2 / 73.8.  The lines weigh a
+  // few per cent over 1000 keys against a fifth over 8000.  Just below those of 128 and 64 columns the tile kernel would be ahead over
+  // 8000 keys and behind over 1000; a line that follows the table's length, which the host knows, has not been measured, nor have
+  // batches of very uneven requests, which the average sends to one kernel.
   const int few = p->D <= 32 ? 80 : p->D <= 64 ? 48 : 24;
   const bool tma = tma_compatible(p->key_cache, p->key_cache_stride[1], p->key_cache_stride[2], p->key_cache_stride[0], p->Hk, p->num_pages) &&
                    tma_compatible(p->value_cache, p->value_cache_stride[1], p->value_cache_stride[2], p->value_cache_stride[0], p->Hk, p->num_pages);
