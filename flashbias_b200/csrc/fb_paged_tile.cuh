@@ -364,10 +364,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const int hd = sg->hg * a.G + (tk >= 0 ? gr - tk * a.G : 0);
       float m_used = -INFINITY, l = 0.f;  // reference maximum (logit * log2 e / 4); row sum of this stream's tiles, relative to it
       const int c0 = c, co0 = co;
-      // the bias in units of q.k, so that a logit costs one product more: s + slope_r (pos - k0), times sl2, plus 4 baseq
+      // the bias in units of q.k, so that a logit costs one product more: s + slope_r (pos - k0), times sl2, plus 4 baseq; in a tile of new
+      // tokens s + slope_r (pos - mine)
       const float slope2 = SLOPES && tk >= 0 ? p.slopes[hd] * kLog2eP : 0.f, slope_r = slope2 / sl2;
       const int my_pos = SLOPES && tk >= 0 ? (p.positions ? p.positions[gn] : len + tk) : 0;
-      const int own_pos = SLOPES && p.positions && tk >= 0 ? p.positions[sg->first] - my_pos : 0;
+      const int own_pos = SLOPES && p.positions && tk >= 0 ? my_pos - p.positions[sg->first] : 0;
       for (int j = x; j < n_kv; j += 2, ++c) {
         const int k0 = (t1 - 1 - j) * 128;
         const bool own = k0 + 128 > len;  // the tile holds new tokens' keys, or places behind them
@@ -394,18 +395,26 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
               if (!(there >> ((ch * 32 + i) / rows) & 1)) bits[ch] &= ~(1u << i);
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        float baseq = SLOPES ? 0.25f * slope2 * (float)(own && p.positions ? own_pos : k0 - my_pos) : 0.f;
+        // A tile of new tokens takes every difference by itself (whole numbers, exact to 2^24), since a row may see the near keys alone
+        // that a shared part of the bias would cancel with.
+        float baseq = SLOPES && !own ? 0.25f * slope2 * (float)(k0 - my_pos) : 0.f;
+        const float mine = SLOPES && own ? (float)(p.positions ? own_pos : my_pos - k0) : 0.f;
         auto complete = [&](int ch) {
           if (dead) {
             if (SLOPES) {
+              const uint64_t less = f2(-mine, -mine), slope_p = f2(slope_r, slope_r);
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const float4 f = own ? *reinterpret_cast<const float4*>(pos + ch * 32 + i)
                                      : make_float4((float)(ch * 32 + i), (float)(ch * 32 + i + 1), (float)(ch * 32 + i + 2), (float)(ch * 32 + i + 3));
-                s[ch][i] = __float_as_uint(fmaf(slope_r, f.x, __uint_as_float(s[ch][i])));
-                s[ch][i + 1] = __float_as_uint(fmaf(slope_r, f.y, __uint_as_float(s[ch][i + 1])));
-                s[ch][i + 2] = __float_as_uint(fmaf(slope_r, f.z, __uint_as_float(s[ch][i + 2])));
-                s[ch][i + 3] = __float_as_uint(fmaf(slope_r, f.w, __uint_as_float(s[ch][i + 3])));
+                auto add = [&](int e, float p0, float p1) {
+                  float v0, v1;
+                  f2_unpack(f2_fma(slope_p, f2_add(f2(p0, p1), less), f2(__uint_as_float(s[ch][e]), __uint_as_float(s[ch][e + 1]))), v0, v1);
+                  s[ch][e] = __float_as_uint(v0);
+                  s[ch][e + 1] = __float_as_uint(v1);
+                };
+                add(i, f.x, f.y);
+                add(i + 2, f.z, f.w);
               }
             }
             if (__any_sync(0xffffffffu, bits[ch] != 0xffffffffu)) {

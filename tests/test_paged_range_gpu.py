@@ -133,6 +133,34 @@ def test_large_logits_of_two_kinds(kernel, T):
 
 
 @pytest.mark.parametrize("kernel", ["own", "split", "general"])
+@pytest.mark.parametrize("T,lens,slope", [(60, 0, 0.7), (130, 70, 0.7), (7, 0, 0.7), (60, 0, 20.0)])
+def test_positions_of_one_request_that_are_far_from_one_another(kernel, T, lens, slope):
+    """Two groups of new tokens, each near itself, that do not see one another."""
+    kw = paged_inputs([lens], [T], 4, 2, 64, 16, torch.float16, 43)
+    t = torch.arange(T)
+    far = t % 3 != 0
+    kw["positions"] = (t // 5 + torch.where(far, 1_234_567, lens)).int()
+    kw["slopes"] = slope * torch.tensor([1.0, 0.4, 0.2, 0.1])
+    seen = (far[:, None] == far) & (t[:, None] >= t)
+    kw["tree_mask"] = torch.zeros(T, -(-T // 64), dtype=torch.int64)
+    for i in range(T):
+        word = kw["tree_mask"][:, i // 64]
+        word |= torch.where(seen[:, i], -2 ** 63 if i % 64 == 63 else 2 ** (i % 64), 0)
+    want, lse, weight, size = oracle(kw)
+    if lens:  # the far tokens' cached keys weigh nothing: a request without them has the size of what counts
+        kw0 = dict(kw, lens=kw["lens"] * 0, block_table=torch.arange(T, dtype=torch.int32)[None])
+        for c in ("key_cache", "value_cache"):
+            kw0[c] = torch.stack([kw[c][p] for p in used_places(kw)[lens:]]).unsqueeze(1)
+        w0, _, weight0, size0 = oracle(kw0)
+        assert (w0 - want)[far].abs().max() < 1e-12
+        weight[far], size[far] = weight0[far], size0[far]
+    o, got = forward(kw, kernel)
+    bo, bl = bounds(want, weight, size, 64, torch.float16)
+    assert_within("o", o, want, bo)
+    assert_within("lse", got, lse, bl + 8 * FP32 * lse.abs() + 1e-6)
+
+
+@pytest.mark.parametrize("kernel", ["own", "split", "general"])
 @pytest.mark.parametrize("T,D", [(5, 64), (9, 128), (64, 128), (5, 32)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("depth", [19.0, 150.0])
