@@ -16,7 +16,7 @@
 // The schedule is that of fb_paged.cuh: equal parts of all key tiles per CTA, parts of an item joined by a second launch.
 // Key tiles are taken from the newest down: a bias that falls with the distance then shows its maximum first.
 // 8 trees of up to 60 tokens over up to 6000, H32-8 D128, slopes: 64 us (139 MB, 24 GFLOP; the general kernel 24059).  Bound by a
-// tile's chain of steps (tensor pipe 34 %) and, 25 us of it, by the segments' beginnings and ends and the join.
+// tile's chain of steps (tensor pipe 33 %) and, 25 us of it, by the segments' beginnings and ends and the join.
 #pragma once
 
 #include <mutex>

@@ -85,8 +85,8 @@ def flash_bias_paged_func(q: torch.Tensor, key_cache: torch.Tensor, value_cache:
     tree_mask: (tokens, words) int64; bit j % 64 of word j / 64 lets a token see the request's j-th new token.  None: a token
         sees the new ones up to itself.  The cached keys are seen by all.
     slopes: (nheads): adds ``slope * (key position - token position)``, where a cached key's position is its place and a new
-        token's is ``positions`` (int32; None: its place).  Positions may lie
-        anywhere; what is exact are differences up to 2^24, to the other tokens of the request.
+        token's is ``positions`` (int32; None: its place).  Positions may lie anywhere; differences up to 2^24 between the tokens
+        of a request are exact.
     q_bias (tokens, nheads | 1, rank) with bias_cache: adds ``q_bias . k_bias``.  Not together with slopes.
     softmax_scale: multiplies q.k only; None or 0: 1 / sqrt(headdim).
 
